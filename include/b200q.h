@@ -487,6 +487,85 @@ int b200q_attn_decode_batch(const float* qkv, void* k_cache, void* v_cache, int 
                             int n_kv_heads, int head_dim, int rope_dim, int max_context, void* q_scratch, void* out, int out_dtype, void* stream);
 int b200q_tc_status_read_clear(int* status);
 
+/* ---- paged KV cache ------------------------------------------------------------------------------------------------------
+ * The cache of tinygrad/llm/model.py:200-207 in pages of page_size positions that sequences own one by one, and the row-wise pieces of
+ * `_attention` (model.py:167-198) over it, for batches whose sequences have different lengths.
+ *
+ * b200q_paged_cache: one block's pages.  Element (page, KV head, slot, d) of k and of v stands at page * page_stride + head * head_stride + slot * row_stride + d
+ *   (elements; 16-byte multiples, so that [page][head][slot][d], [page][slot][head][d] and k and v side by side in one pool all work).  dtype B200Q_F16 | B200Q_BF16 | B200Q_F32.
+ * b200q_paged_batch: which rows and pages belong to which sequence, all tables on the device.  Sequence s has the rows row_off[s] .. row_off[s + 1] - 1 of the
+ *   row arrays (new tokens, in the order of their positions) and length[s] tokens in all, the new ones among them: row i of n stands at position
+ *   length - n + i.  Position p is slot p % page_size of page pages[s * table_stride + p / page_size].  The host gives bounds: n_rows rows in the arrays,
+ *   max_new rows and max_len tokens of any sequence.
+ * What the tables say is checked on the device; nothing outside the arrays is read or written, and the status word (b200q_status_read_clear) becomes 2 where they
+ * are wrong: a page that does not exist takes no writes and reads as zeros; a position outside the table's row, below 0 or (append) outside the
+ * rotation's table has no cache row; tokens past max_len are not attended; rows past max_new of a sequence get no attention.  Rows that belong to no sequence (n_rows >
+ * row_off[n_seqs]: a padded batch in a captured graph) are left as they were.
+ *
+ * b200q_paged_append: rows x = [q | k | v] (x_dtype; x_stride elements apart, 0: back to back) -> per head RMSNorm(q) * q_norm, RMSNorm(k) * k_norm (fp16 [head_dim], NULL: no norm;
+ *   tinygrad/nn/__init__.py:300-304 over the head's values), RoPE with half-split pairs in the first rope_dim values (model.py:29-33; rope fp32 [rope_len][rope_dim] cos || sin, NULL: none), then q to
+ *   the rows of q (q_dtype, q_stride; may be x's own q part if types and strides agree) and k, v to the sequence's pages.  32-bit arithmetic, each value rounded once.  A row whose position has no
+ *   entry in `rope` gets zeros in q.
+ * b200q_head_norm_rope: the same norms and rotation of the first n_heads + n_kv_heads heads of every row, from x to out (may be x), for callers whose cache is not paged
+ *   (b200q_attn_prefill and _decode rotate themselves: rope NULL).  positions [n_rows] (device) is asked for with rope only; one outside the table gives zeros and status 2.
+ * b200q_paged_attention: out[row][head] = softmax(scale * q . k) v over positions 0 .. the row's own, query head h on KV head h / (n_heads / n_kv_heads).  scale 0: head_dim^-1/2.  A row
+ *   without a position (length < its sequence's rows) gets zeros.  Values behind a row's own position are not read into it, whatever they are (NaN among them).
+ *   q, out: B200Q_F32 | F16 | BF16, strides in elements (0: back to back).  Scores, sums and the running maximum are 32-bit; rows of fp32 meet fp16 keys as two
+ *   fp16 halves (bf16 keys: three).  workspace: b200q_paged_attention_workspace_bytes bytes, 256-byte aligned, zeroed once; the call leaves it as
+ *   it has to be for the next one.  Calls that may run at the same time (two streams, two graphs) need one each.
+ * head_dim 16, 32, 64 or 128.  flags: B200Q_FLAG_PDL (the launch before it on the stream is a kernel of this library). */
+typedef struct b200q_paged_cache {
+  void* k;
+  void* v;
+  int dtype, n_pages, page_size, n_kv_heads, head_dim;
+  int64_t page_stride, head_stride, row_stride;
+} b200q_paged_cache;
+typedef struct b200q_paged_batch {
+  const int32_t* row_off;   /* [n_seqs + 1] */
+  const int32_t* length;    /* [n_seqs] */
+  const int32_t* pages;     /* [n_seqs][table_stride] */
+  int n_seqs, table_stride, n_rows, max_new, max_len;
+} b200q_paged_batch;
+typedef struct b200q_paged_append_args {
+  const void* x;
+  void* q;
+  int x_dtype, q_dtype;
+  int64_t x_stride, q_stride;
+  int n_heads;
+  float norm_eps;
+  const void* q_norm;
+  const void* k_norm;
+  const float* rope;
+  int rope_dim, rope_len;
+} b200q_paged_append_args;
+int b200q_paged_append(const b200q_paged_cache* cache, const b200q_paged_batch* batch, const b200q_paged_append_args* args, int flags, void* stream);
+typedef struct b200q_head_norm_args {
+  const void* x;
+  void* out;
+  int x_dtype, out_dtype;
+  int64_t x_stride, out_stride;
+  int n_rows, n_heads, n_kv_heads, head_dim;
+  float norm_eps;
+  const void* q_norm;
+  const void* k_norm;
+  const float* rope;
+  int rope_dim, rope_len;
+  const int32_t* positions;
+} b200q_head_norm_args;
+int b200q_head_norm_rope(const b200q_head_norm_args* args, int flags, void* stream);
+typedef struct b200q_paged_attn_args {
+  const void* q;
+  void* out;
+  int q_dtype, out_dtype;
+  int64_t q_stride, out_stride;
+  int n_heads;
+  float scale;
+  void* workspace;
+  size_t workspace_bytes;
+} b200q_paged_attn_args;
+size_t b200q_paged_attention_workspace_bytes(const b200q_paged_cache* cache, const b200q_paged_batch* batch, int n_heads);
+int b200q_paged_attention(const b200q_paged_cache* cache, const b200q_paged_batch* batch, const b200q_paged_attn_args* args, int flags, void* stream);
+
 /* ---- MXFP8 mixture-of-experts path --------------------------------------
  * E4M3 values with one E8M0 exponent per 32 along the last axis.
  *

@@ -1,0 +1,475 @@
+"""The paged KV cache on the device against 64-bit numpy: appending (norms of heads, rotation, pages), attention of ragged batches, and both in a row."""
+import numpy as np
+import pytest
+from gpu_util import need_gpu
+from oracle import paged as ref
+
+pytestmark = pytest.mark.gpu
+
+EPS = {"float32": 2.0 ** -23, "float16": 2.0 ** -10, "bfloat16": 2.0 ** -7}
+TINY = {"float32": 0.0, "float16": 2.0 ** -25, "bfloat16": 0.0}       # half a step of fp16's subnormals
+
+
+def put(x, dtype):
+  """values -> (device buffer, the values that it holds, float64)"""
+  from tinygrad_b200.runtime import DeviceBuffer
+  x = np.asarray(x)
+  if dtype == "bfloat16":
+    b = ref.bf16_bits(x.astype(np.float32))
+    return DeviceBuffer.from_numpy(b), ref.bf16_values(b).astype(np.float64)
+  with np.errstate(over="ignore"): a = x.astype(dtype)
+  return DeviceBuffer.from_numpy(a), a.astype(np.float64)
+
+
+def get(buf, shape, dtype):
+  a = buf.numpy(shape, np.uint16 if dtype == "bfloat16" else np.dtype(dtype))
+  return (ref.bf16_values(a) if dtype == "bfloat16" else a).astype(np.float64)
+
+
+def table(rng, length, page_size, spare=3):
+  """Pages of every sequence in random order -> (table, number of pages); entries behind a sequence's pages are no pages at all."""
+  need = [-(-l // page_size) for l in length]
+  order = rng.permutation(sum(need) + spare)
+  t = np.full((len(length), max(need + [1])), -7, np.int32)
+  at = 0
+  for s, n in enumerate(need):
+    t[s, :n] = order[at:at + n]
+    at += n
+  return t, sum(need) + spare
+
+
+def i32(a):
+  from tinygrad_b200.runtime import DeviceBuffer
+  return DeviceBuffer.from_numpy(np.asarray(a, np.int32))
+
+
+def cos_sin(rows, dim):
+  a = np.arange(rows)[:, None] * (10000.0 ** (-np.arange(0, dim, 2) / dim))[None]
+  return np.concatenate([np.cos(a), np.sin(a)], -1).astype(np.float32)
+
+
+def layout(name, pages, heads, size, dim):
+  """(strides, size of a pool in elements, where the pool begins in it)"""
+  if name == "head-major": return (heads * size * dim, size * dim, dim), pages * heads * size * dim
+  if name == "slot-major": return (heads * size * dim, dim, heads * dim), pages * heads * size * dim
+  return (3 * heads * size * (dim + 8), size * (dim + 8), dim + 8), 3 * pages * heads * size * (dim + 8)      # rows with room between, every third page
+
+
+def in_layout(flat, strides, pages, heads, size, dim):
+  return np.lib.stride_tricks.as_strided(flat, (pages, heads, size, dim), tuple(s * flat.itemsize for s in (*strides, 1)))
+
+
+def status():
+  from tinygrad_b200 import runtime
+  return runtime.device_status()
+
+
+# ---- norms and rotation ----
+# Tolerance: a value is one of a c - b s: both products' roundings, the sum's, and what a and b lost in the norm.  The 128 squares are added in a tree of 4 + 5 levels and a chain of at most 16
+# (25 roundings of 2^-24, halved by the root), the mean, eps, root, quotient and two products add 6: below 24 x 2^-24 of |a| + |b|.  Then half a step of the output's type.
+def close_rows(got, want, reach, dtype, what):
+  tol = 24 * 2.0 ** -24 * reach + EPS[dtype] / 2 * (np.abs(want) + 24 * 2.0 ** -24 * reach) + TINY[dtype]
+  bad = np.abs(got - want) > tol
+  assert not bad.any(), f"{what}: {bad.sum()} of {bad.size}, worst {np.max(np.abs(got - want) / np.maximum(tol, 1e-300)):.2f} tolerances"
+
+
+def reach_of(x, w, eps, rot):
+  """|a| + |b| of every value's pair (itself where nothing is rotated)."""
+  a = np.abs(ref.head_norm(x, w, eps))
+  r = 0 if rot is None else rot.shape[-1] // 2
+  both = a[..., :r] + a[..., r:2 * r]
+  return np.concatenate([both, both, a[..., 2 * r:]], -1)
+
+
+APPEND = [   # seqs' (new, length), heads, KV heads, dim, page size, rotated, types of x / q / pages, norms, layout
+  ([(1, 1)], 4, 2, 64, 16, 64, "float32", "float32", "float16", "", "head-major"),
+  ([(1, 513)], 32, 8, 128, 16, 128, "float32", "float32", "float16", "qk", "head-major"),
+  ([(5, 9), (1, 40), (17, 17)], 6, 3, 128, 8, 64, "float32", "float16", "float32", "qk", "slot-major"),
+  ([(3, 3), (33, 70), (0, 12), (2, 66)], 7, 1, 32, 5, 32, "float16", "float16", "float16", "k", "loose"),
+  ([(129, 300)], 4, 4, 16, 1, 16, "bfloat16", "bfloat16", "bfloat16", "q", "head-major"),
+  ([(1, 64)] * 37, 28, 4, 128, 64, 32, "bfloat16", "float32", "bfloat16", "qk", "loose"),
+  ([(2, 1000), (40, 41)], 5, 5, 64, 100, 6, "float16", "float32", "float16", "qk", "slot-major"),      # pairs that are not on 16-byte boundaries
+  ([(4, 4)], 3, 1, 128, 3, 0, "float32", "float32", "float16", "qk", "head-major"),                    # no rotation
+]
+
+
+@pytest.mark.parametrize("case", range(len(APPEND)))
+def test_append(case):
+  need_gpu()
+  from tinygrad_b200 import paged
+  from tinygrad_b200.runtime import DeviceBuffer
+  seqs, h, hk, d, ps, r, xt, qt, ct, norms, lay = APPEND[case]
+  rng = np.random.default_rng(case)
+  new, length = [n for n, _ in seqs], [l for _, l in seqs]
+  off, n = np.concatenate([[0], np.cumsum(new)]), sum(new)
+  t, n_pages = table(rng, length, ps)
+  pad = 3                                     # rows of no sequence
+  x, xv = put(rng.standard_normal((n + pad, h + 2 * hk, d)) * 2, xt)
+  strides, size = layout(lay, n_pages, hk, ps, d)
+  before = rng.standard_normal(size).astype(np.float32)
+  (k, kv0), (v, vv0) = put(before, ct), put(before + 1, ct)
+  q, q0 = put(np.full((n + pad, h, d), 7.0), qt)
+  wq, wk = (None if c not in norms else rng.uniform(0.5, 1.5, d).astype(np.float16) for c in "qk")
+  rope = cos_sin(max(length), r) if r else None
+  dev = lambda a: None if a is None else DeviceBuffer.from_numpy(a)
+  status()
+  cache = paged.PagedCache(n_pages, ps, hk, d, ct, k=k, v=v, strides=strides)
+  batch = paged.PagedBatch(i32(off), i32(length), i32(t), n_rows=n + pad, max_new=max(new), max_len=max(length))
+  paged.append(cache, batch, x, q, h, xt, q_dtype=qt, rope=dev(rope), q_norm=dev(wq), k_norm=dev(wk), norm_eps=1e-5)
+  places = ref.rows_of(off, length)
+  rot = rope[[p for _, p in places]] if r else None
+  xs = xv[:n]
+  got = get(q, (n + pad, h, d), qt)
+  close_rows(got[:n], ref.rotate(ref.head_norm(xs[:, :h], wq, 1e-5), rot), reach_of(xs[:, :h], wq, 1e-5, rot), qt, "q")
+  assert (got[n:] == 7).all(), "rows behind the last sequence are left as they were"
+  kw, kr = ref.rotate(ref.head_norm(xs[:, h:h + hk], wk, 1e-5), rot), reach_of(xs[:, h:h + hk], wk, 1e-5, rot)
+  kg, vg = get(k, (size,), ct), get(v, (size,), ct)
+  for flat in (kg, vg): assert np.isfinite(flat).all()
+  kp, vp = in_layout(kg, strides, n_pages, hk, ps, d), in_layout(vg, strides, n_pages, hk, ps, d)
+  where = [(t[s, p // ps], p % ps) for s, p in places]
+  pg, sl = (np.array(c, int) for c in zip(*where))
+  close_rows(kp[pg, :, sl], kw, kr, ct, "k")
+  vw = xs[:, h + hk:]
+  assert (np.abs(vp[pg, :, sl] - vw) <= EPS[ct] / 2 * np.abs(vw) + TINY[ct]).all(), "v"
+  kp[pg, :, sl], vp[pg, :, sl] = in_layout(kv0, strides, n_pages, hk, ps, d)[pg, :, sl], in_layout(vv0, strides, n_pages, hk, ps, d)[pg, :, sl]
+  assert (kg == kv0).all() and (vg == vv0).all(), "everything else in the pools is as it was"
+  assert status() == 0
+
+
+def test_append_where_the_tables_are_wrong():
+  """A page that does not exist, a position outside the table's row, before 0 or past the rotation's: no writes, status 2."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  from tinygrad_b200.runtime import DeviceBuffer
+  rng = np.random.default_rng(5)
+  h, hk, d, ps, n_pages = 2, 1, 32, 4, 6
+  x, xv = put(rng.standard_normal((4, h + 2 * hk, d)), "float32")
+  for length, t, zero in (([9, 3], [[0, 1, 6], [-1, 2, 3]], []), ([9, 3], [[0, 1], [-5, 3]], []), ([1, 9], [[4], [6]], [0]), ([30, 31], [[0, 1], [2, 3]], [0, 1, 2, 3])):
+    status()
+    cache = paged.PagedCache(n_pages, ps, hk, d, "float32")
+    q = DeviceBuffer.empty((4, h, d), np.float32, zero=True)
+    batch = paged.PagedBatch(i32([0, 2, 4]), i32(length), i32(t), n_rows=4, max_new=2, max_len=31)
+    paged.append(cache, batch, x, q, h, rope=DeviceBuffer.from_numpy(cos_sin(12, d)))
+    got = get(q, (4, h, d), "float32")
+    assert [i for i in range(4) if (got[i] == 0).all()] == zero, (length, t)
+    want = np.zeros((n_pages, ps))
+    for s, p in ref.rows_of([0, 2, 4], length):
+      if 0 <= p < 12 and p // ps < len(t[s]) and 0 <= t[s][p // ps] < n_pages: want[t[s][p // ps], p % ps] = 1
+    for buf in (cache.k, cache.v): assert ((get(buf, (n_pages, ps, d), "float32") != 0).any(-1) == want).all(), (length, t)
+    assert status() == 2
+
+
+def test_append_in_place_and_strided():
+  need_gpu()
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(2)
+  h, hk, d, ps, n, stride = 3, 1, 64, 16, 21, 5 * 64 + 24
+  x, xv = put(rng.standard_normal((n, stride)), "float16")
+  cache = paged.PagedCache(4, ps, hk, d)
+  batch = paged.PagedBatch(i32([0, n]), i32([n]), i32([[2, 0]]), n_rows=n, max_new=n, max_len=n)
+  from tinygrad_b200.runtime import DeviceBuffer
+  rope = cos_sin(n, d)
+  paged.append(cache, batch, x, x, h, "float16", rope=DeviceBuffer.from_numpy(rope), x_stride=stride, q_stride=stride)
+  got = get(x, (n, stride), "float16")
+  xs = xv[:, :5 * d].reshape(n, 5, d)
+  close_rows(got[:, :h * d].reshape(n, h, d), ref.rotate(xs[:, :h], rope), reach_of(xs[:, :h], None, 0, rope), "float16", "q")
+  assert (got[:, h * d:] == xv[:, h * d:]).all()
+  k = get(cache.k, (4, ps, d), "float16")
+  close_rows(np.concatenate([k[2], k[0]])[:n, None], ref.rotate(xs[:, h:h + 1], rope), reach_of(xs[:, h:h + 1], None, 0, rope), "float16", "k")
+
+
+@pytest.mark.parametrize("rows,h,hk,d,r,xt,ot,in_place", [(1, 32, 8, 128, 128, "float32", "float32", False), (300, 28, 4, 128, 0, "float16", "float16", True), (77, 5, 0, 64, 10, "bfloat16", "float32", False),
+                                                         (9, 0, 3, 32, 32, "float32", "bfloat16", False), (2, 3, 3, 16, 8, "float16", "float16", True)])
+def test_head_norm_rope(rows, h, hk, d, r, xt, ot, in_place):
+  need_gpu()
+  from tinygrad_b200 import paged
+  from tinygrad_b200.runtime import DeviceBuffer
+  rng = np.random.default_rng(rows)
+  x, xv = put(rng.standard_normal((rows, h + 2 * hk + 1, d)) * 3, xt)
+  stride = (h + 2 * hk + 1) * d
+  out, ov = (x, xv) if in_place else put(np.full((rows, h + hk, d), 5.0), ot)
+  wq, wk = (rng.uniform(0.5, 1.5, d).astype(np.float16) for _ in "qk")
+  rope, pos = (cos_sin(50, r), rng.integers(0, 50, rows).astype(np.int32)) if r else (None, None)
+  paged.head_norm_rope(x, out, rows, h, hk, d, xt, out_dtype=ot, q_norm=DeviceBuffer.from_numpy(wq), k_norm=DeviceBuffer.from_numpy(wk), norm_eps=1e-6,
+                       rope=rope is not None and DeviceBuffer.from_numpy(rope) or None, positions=pos is not None and i32(pos) or None, x_stride=stride, out_stride=stride if in_place else 0)
+  rot = rope[pos] if r else None
+  got = get(out, (rows, h + 2 * hk + 1 if in_place else h + hk, d), ot)
+  for a, b, w in ((0, h, wq), (h, h + hk, wk)): close_rows(got[:, a:b], ref.rotate(ref.head_norm(xv[:, a:b], w, 1e-6), rot), reach_of(xv[:, a:b], w, 1e-6, rot), ot, str(a))
+  if in_place: assert (got[:, h + hk:] == xv[:, h + hk:]).all()
+
+
+def test_head_norm_rope_position_outside_the_table():
+  need_gpu()
+  from tinygrad_b200 import paged
+  from tinygrad_b200.runtime import DeviceBuffer
+  x, xv = put(np.ones((3, 2, 32)), "float32")
+  status()
+  paged.head_norm_rope(x, x, 3, 1, 1, 32, rope=DeviceBuffer.from_numpy(cos_sin(4, 32)), positions=i32([-1, 0, 4]))
+  got = get(x, (3, 64), "float32")
+  assert (got[1] == 1).all() and not got[0].any() and not got[2].any() and status() == 2
+
+
+# ---- attention ----
+# Tolerance.  Scores: products of `dim` values added in 32 bits, in an order of the kernel's choice, tensor cores cutting where others round: a walk of dim steps of at most 2^-23 of the sum of
+# magnitudes, 4 sqrt(dim) of them; a step of a score moves its probability by that much (and the others' sum by no more): twice that, of sum p |v|.  The exponential and its argument: 2^-21.  The sum over n
+# keys: 4 sqrt(n) 2^-23.  Half a step of the output.  Kernels that take probabilities to the tensor core in the 16 bits of the cache (16-bit queries) lose half a step of that too.
+def close_attention(got, want, weight, reach, dim, keys, q_type, out_type, what):
+  tol = weight * (2 * 4 * dim ** 0.5 * 2.0 ** -23 * reach[..., None] + 2.0 ** -21 + 4 * keys ** 0.5 * 2.0 ** -23)
+  if q_type != "float32": tol = tol + weight * EPS[q_type] / 2
+  tol = tol + EPS[out_type] / 2 * (np.abs(want) + tol) + TINY[out_type]
+  bad = ~(np.abs(got - want) <= tol)
+  assert not bad.any(), f"{what}: {bad.sum()} of {bad.size}, worst {np.max(np.abs(got - want) / np.maximum(tol, 1e-300)):.2f} tolerances, first at {np.argwhere(bad)[0]}"
+
+
+def attend(seqs, h, hk, d, ps, qt, ct, ot=None, lay="head-major", seed=0, scale=0.0, pad=2, spread=1.0, poison=True, bounds=None, tables=None, stream=None):
+  """One call against the oracle.  poison: everything in the pools that belongs to no position of a sequence is NaN."""
+  from tinygrad_b200 import paged
+  ot = ot or qt
+  rng = np.random.default_rng(seed)
+  new, length = [n for n, _ in seqs], [l for _, l in seqs]
+  off, n = np.concatenate([[0], np.cumsum(new)]), sum(new)
+  t, n_pages = table(rng, length, ps)
+  strides, size = layout(lay, n_pages, hk, ps, d)
+  pools = []
+  for _ in "kv":
+    flat = np.full(size, np.nan if poison else 0.0, np.float32)
+    view = in_layout(flat, strides, n_pages, hk, ps, d)
+    for s, l in enumerate(length):
+      p = np.arange(l)
+      view[t[s][p // ps], :, p % ps] = rng.standard_normal((l, hk, d))
+    buf, val = put(flat, ct)
+    pools.append((buf, in_layout(val, strides, n_pages, hk, ps, d)))
+  q, qv = put(rng.standard_normal((n + pad, h, d)) * spread, qt)
+  out, _ = put(np.full((n + pad, h, d), 3.0), ot)
+  status()
+  cache = paged.PagedCache(n_pages, ps, hk, d, ct, k=pools[0][0], v=pools[1][0], strides=strides)
+  most_new, most_len = bounds or (max(new), max(length))
+  batch = paged.PagedBatch(i32(off), i32(length), i32(t), n_rows=n + pad, max_new=most_new, max_len=most_len)
+  want, weight, reach = ref.attention(qv[:n], pools[0][1], pools[1][1], off, length, t, ps, scale or d ** -0.5)
+  for again in range(2):      # (the second call finds the workspace as the first has left it)
+    paged.attention(cache, batch, q, out, h, qt, out_dtype=ot, scale=scale, stream=stream)
+    if stream is not None: stream.synchronize()
+    got = get(out, (n + pad, h, d), ot)
+    close_attention(got[:n], want, weight, reach, d, max(length), qt, ot, f"call {again}")
+    assert (got[n:] == 3).all(), "rows behind the last sequence are left as they were"
+  assert status() == 0
+  return got[:n]
+
+
+ATTEND = [   # seqs' (new, length), heads, KV heads, dim, page size, types of q / pages / out
+  ([(1, 1)], 4, 2, 64, 16, "float32", "float16", None),
+  ([(1, 513)], 32, 8, 128, 16, "float32", "float16", None),
+  ([(1, 2000), (1, 3), (1, 64), (1, 1025)], 28, 4, 128, 64, "float32", "float16", None),
+  ([(1, 700), (0, 50), (1, 701)], 8, 8, 128, 32, "float16", "float16", None),
+  ([(3, 300), (4, 4), (2, 129)], 7, 1, 64, 16, "bfloat16", "bfloat16", None),
+  ([(40, 40), (1, 100), (129, 260)], 4, 2, 128, 16, "float32", "float16", "float16"),
+  ([(70, 333)], 6, 3, 32, 5, "float32", "bfloat16", None),
+  ([(17, 17), (5, 90)], 3, 1, 16, 1, "float16", "bfloat16", "float32"),
+  ([(65, 200), (3, 1500)], 4, 1, 64, 100, "float32", "float32", None),
+  ([(1, 4097)], 4, 4, 128, 128, "float32", "float32", None),
+  ([(200, 700)], 8, 2, 128, 128, "float16", "float16", None),
+  ([(257, 257), (130, 1000), (1, 900)], 8, 2, 64, 32, "bfloat16", "bfloat16", None),
+  ([(129, 129)], 5, 5, 128, 8, "float16", "float16", None),
+  ([(300, 5000)], 4, 1, 128, 16, "float16", "float16", None),
+  ([(90, 4000)], 16, 1, 64, 256, "float16", "float16", "float32"),
+  ([(150, 150), (2, 60)], 7, 1, 128, 64, "bfloat16", "bfloat16", "float16"),
+]
+
+
+@pytest.mark.parametrize("lay", ["head-major", "slot-major", "loose"])
+@pytest.mark.parametrize("case", range(len(ATTEND)))
+def test_attention(case, lay):
+  need_gpu()
+  seqs, h, hk, d, ps, qt, ct, ot = ATTEND[case]
+  attend(seqs, h, hk, d, ps, qt, ct, ot, lay, seed=case)
+
+
+@pytest.mark.parametrize("qt,ct", [("float32", "float16"), ("float16", "float16"), ("bfloat16", "bfloat16"), ("float32", "bfloat16")])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("seqs", [[(1, 900), (1, 17)], [(200, 900), (9, 9)]], ids=["tokens", "chunks"])
+def test_attention_with_peaked_scores_and_a_scale(qt, ct, d, seqs):
+  """Scores some hundred apart: the running maximum moves, most probabilities vanish."""
+  need_gpu()
+  attend(seqs, 4, 2, d, 16, qt, ct, seed=d, spread=20.0)
+  attend(seqs, 4, 2, d, 16, qt, ct, seed=d, scale=0.03)
+
+
+@pytest.mark.parametrize("qt,ct", [("float32", "float16"), ("float16", "float16"), ("float32", "float32")])
+def test_rows_without_a_position(qt, ct):
+  """length below the number of new rows: the first of them stand before position 0, see nothing and get zeros."""
+  need_gpu()
+  got = attend([(5, 2), (3, 0), (150, 20), (1, 0)], 4, 2, 64, 16, qt, ct, seed=3)
+  assert not got[:3].any() and got[3].any() and not got[5:8].any() and not got[8:138].any() and got[138].any() and not got[158].any()
+
+
+@pytest.mark.parametrize("qt,ct", [("float32", "float16"), ("float16", "float16"), ("bfloat16", "bfloat16"), ("float32", "float32")])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new,length,at", [(4, 100, 98), (200, 400, 300), (130, 130, 1), (130, 140, 139)])
+def test_values_behind_a_rows_position_are_not_read_into_it(qt, ct, d, new, length, at):
+  """A later token's key and value are NaN or infinite: rows before it are what they were, rows from it on are not finite (NaN)."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(at)
+  h, hk, ps = 4, 2, 16
+  t, n_pages = table(rng, [length], ps)
+  outs = []
+  k, v, q = rng.standard_normal((n_pages, hk, ps, d)), rng.standard_normal((n_pages, hk, ps, d)), rng.standard_normal((new, h, d))
+  for bad in (None, (np.nan, np.nan), (0.5, np.nan), (0.5, np.inf)):
+    if bad is not None:
+      k[t[0, at // ps], :, at % ps], v[t[0, at // ps], :, at % ps, 5] = bad[0], bad[1]
+    cache = paged.PagedCache(n_pages, ps, hk, d, ct, k=put(k, ct)[0], v=put(v, ct)[0])
+    batch = paged.PagedBatch(i32([0, new]), i32([length]), i32(t), n_rows=new, max_new=new, max_len=length)
+    out = put(np.zeros((new, h, d)), qt)[0]
+    paged.attention(cache, batch, put(q, qt)[0], out, h, qt)
+    outs.append(get(out, (new, h, d), qt))
+  sees = np.arange(new) + length - new >= at
+  for bad in outs[1:]:
+    assert (bad[~sees] == outs[0][~sees]).all()
+    assert not np.isfinite(bad[sees][..., 5]).any()
+  assert np.isfinite(outs[2][sees][..., 6]).all() and np.isfinite(outs[3][sees][..., 6]).all()
+
+
+def test_attention_where_the_tables_are_wrong():
+  """Pages that do not exist read as zeros; what lies past a bound is not attended, or not computed; status 2 each time."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(8)
+  h, hk, d, ps, n_pages = 4, 2, 64, 16, 7
+  for qt, ct, new in (("float32", "float16", 1), ("float16", "float16", 40), ("float32", "float32", 3), ("float16", "float16", 200)):
+    length = 210
+    (k, kv), (v, vv), (q, qv) = (put(rng.standard_normal(s), t) for s, t in (((n_pages, hk, ps, d), ct), ((n_pages, hk, ps, d), ct), ((new, h, d), qt)))
+    t = rng.integers(0, n_pages, (1, 14)).astype(np.int32)      # (the same page twice is fine)
+    t[0, [2, 9]] = -1, n_pages
+    cache = paged.PagedCache(n_pages, ps, hk, d, ct, k=k, v=v)
+    out = put(np.full((new, h, d), 9.0), qt)[0]
+    status()
+    paged.attention(cache, paged.PagedBatch(i32([0, new]), i32([length]), i32(t), n_rows=new, max_new=new, max_len=length), q, out, h, qt)
+    want, weight, reach = ref.attention(qv, kv, vv, [0, new], [length], t, ps, d ** -0.5)
+    close_attention(get(out, (new, h, d), qt), want, weight, reach, d, length, qt, qt, "pages")
+    assert status() == 2
+    # a length past the bound: keys 0 .. max_len - 1, every row at its own position
+    t[0, [2, 9]] = 0
+    paged.attention(cache, paged.PagedBatch(i32([0, new]), i32([length]), i32(t), n_rows=new, max_new=new, max_len=150), q, out, h, qt)
+    got = get(out, (new, h, d), qt)
+    keep = [i for i in range(new) if length - new + i < 150]
+    want, weight, reach = ref.attention(qv, kv, vv, [0, new], [length], t, ps, d ** -0.5)
+    if keep: close_attention(got[keep], want[keep], weight[keep], reach[keep], d, length, qt, qt, "rows below the bound")
+    want, weight, reach = ref.attention(qv[-1:], kv, vv, [0, 1], [150], t, ps, d ** -0.5)
+    close_attention(got[-1:], want, weight, reach, d, length, qt, qt, "the last row")
+    assert status() == 2
+    if new > 1:      # more rows than the bound
+      out = put(np.full((new, h, d), 9.0), qt)[0]
+      paged.attention(cache, paged.PagedBatch(i32([0, new]), i32([length]), i32(t), n_rows=new, max_new=new - 1, max_len=length), q, out, h, qt)
+      got = get(out, (new, h, d), qt)
+      assert (got[-1] == 9).all() and not (got[-2] == 9).any() and status() == 2
+
+
+def test_attention_gives_the_same_bits_again():
+  need_gpu()
+  for args in (([(1, 3000), (1, 70)], 8, 2, 128, 16, "float32", "float16"), ([(300, 4000)], 8, 2, 128, 16, "float16", "float16"), ([(3, 2500)], 4, 2, 64, 16, "bfloat16", "bfloat16")):
+    a, b = attend(*args, seed=1), attend(*args, seed=1)
+    assert (a == b).all()
+
+
+def test_nothing_to_do():
+  need_gpu()
+  from tinygrad_b200 import paged
+  cache = paged.PagedCache(2, 16, 1, 64)
+  x, _ = put(np.ones((4, 3, 64)), "float32")
+  out, _ = put(np.full((4, 1, 64), 2.0), "float32")
+  for off, length in (([0, 0], [0]), ([0, 0, 0], [5, 0])):
+    batch = paged.PagedBatch(i32(off), i32(length), i32(np.zeros((len(length), 1))), n_rows=4, max_new=1, max_len=16)
+    paged.append(cache, batch, x, out, 1)
+    paged.attention(cache, batch, x, out, 1)
+  paged.attention(cache, paged.PagedBatch(i32([0]), i32(np.zeros(0)), i32(np.zeros((0, 1))), n_rows=0, max_new=0, max_len=0), x, out, 1)
+  paged.head_norm_rope(x, out, 0, 1, 0, 64)
+  assert (get(out, (4, 64), "float32") == 2).all() and status() == 0
+
+
+# ---- as a serving program uses them ----
+@pytest.mark.parametrize("xt,ct", [("float32", "float16"), ("float16", "float16"), ("bfloat16", "bfloat16")])
+def test_prompts_and_tokens_of_two_sequences(xt, ct):
+  """Two sequences: a prompt each in chunks of different sizes, then single tokens in a captured graph whose lengths and pages change on the device; every row against causal attention over the whole
+  sequence."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  from tinygrad_b200.runtime import DeviceBuffer, Graph, Stream
+  rng = np.random.default_rng(4)
+  h, hk, d, ps, total = 8, 2, 64, 16, (150, 61)
+  steps = [(40, 0), (90, 33), (1, 20)] + [(1, 1)] * 8
+  stream = Stream()
+  cache = paged.PagedCache(20, ps, hk, d, ct)
+  x = [rng.standard_normal((n, h + 2 * hk, d)) for n in total]
+  w = rng.uniform(0.5, 1.5, (2, d)).astype(np.float16)
+  rope = cos_sin(200, d)
+  rope_d, wq, wk = DeviceBuffer.from_numpy(rope), DeviceBuffer.from_numpy(w[0]), DeviceBuffer.from_numpy(w[1])
+  pages = rng.permutation(20).reshape(2, 10).astype(np.int32)
+  at, got, graph = [0, 0], [[], []], None
+  one = None
+  for new in steps:
+    rows = np.concatenate([x[s][at[s]:at[s] + n] for s, n in enumerate(new)])
+    at = [a + n for a, n in zip(at, new)]
+    off = np.array([0, new[0], sum(new)], np.int32)
+    if new == (1, 1):
+      if one is None:
+        one = [put(rows, xt)[0], put(rows[:, :h], xt)[0], put(rows[:, :h], xt)[0], i32(off), i32(at), i32(np.zeros((2, 10)))]
+        batch = paged.PagedBatch(*one[3:], n_rows=2, max_new=1, max_len=200)
+        batch.reserve(cache, h, xt)
+        graph = Graph(stream)
+        with graph:
+          paged.append(cache, batch, one[0], one[1], h, xt, rope=rope_d, q_norm=wq, k_norm=wk, norm_eps=1e-6, stream=stream)
+          paged.attention(cache, batch, one[1], one[2], h, xt, flags=1, stream=stream)
+      xb = rows.astype(xt) if xt != "bfloat16" else ref.bf16_bits(rows.astype(np.float32))
+      one[0].copy_from(xb), one[4].copy_from(np.array(at, np.int32)), one[5].copy_from(pages)
+      graph.launch()
+      stream.synchronize()
+      out = get(one[2], (2, h, d), xt)
+    else:
+      xb, q, o = put(rows, xt)[0], put(rows[:, :h], xt)[0], put(rows[:, :h], xt)[0]
+      batch = paged.PagedBatch(i32(off), i32(at), i32(pages), n_rows=sum(new), max_new=max(new), max_len=max(at))
+      paged.append(cache, batch, xb, q, h, xt, rope=rope_d, q_norm=wq, k_norm=wk, norm_eps=1e-6, stream=stream)
+      paged.attention(cache, batch, q, o, h, xt, stream=stream)
+      stream.synchronize()
+      out = get(o, (sum(new), h, d), xt)
+    got[0].append(out[:new[0]]), got[1].append(out[new[0]:])
+  k = get(cache.k, (20, hk, ps, d), ct), get(cache.v, (20, hk, ps, d), ct)
+  for s in range(2):
+    n = at[s]
+    xs = put(x[s][:n], xt)[1]
+    q = ref.rotate(ref.head_norm(xs[:, :h], w[0], 1e-6), rope[:n])
+    qd = put(q, xt)[1]                       # rounded once by append
+    want, weight, reach = ref.attention(qd, *k, [0, n], [n], pages[s:s + 1], ps, d ** -0.5)
+    # append's q may be rounded the other way where it is half way between two values: a step of q moves a score by EPS / 2 of its reach
+    slack = weight * 2 * EPS[xt] / 2 * reach[..., None]
+    tol_got = np.concatenate(got[s])
+    err = np.abs(tol_got - want)
+    tol = weight * (2 * 4 * d ** 0.5 * 2.0 ** -23 * reach[..., None] + 2.0 ** -21 + 4 * n ** 0.5 * 2.0 ** -23 + (EPS[xt] / 2 if xt != "float32" else 0)) + slack
+    assert (err <= tol + EPS[xt] / 2 * (np.abs(want) + tol) + TINY[xt]).all(), s
+  assert status() == 0
+
+
+def test_against_the_contiguous_cache():
+  """The same prompt through b200q_attn_prefill and through pages: both within their tolerance of each other."""
+  need_gpu()
+  from tinygrad_b200 import _lib, paged
+  from tinygrad_b200.runtime import DeviceBuffer
+  rng = np.random.default_rng(6)
+  h, hk, d, n, ctx, ps = 8, 2, 128, 90, 128, 16
+  x = rng.standard_normal((n, (h + 2 * hk) * d)).astype(np.float32)
+  rope = cos_sin(ctx, d)
+  xb, rb = DeviceBuffer.from_numpy(x), DeviceBuffer.from_numpy(rope)
+  k, v = (DeviceBuffer.empty((hk, ctx, d), np.float16, zero=True) for _ in "kv")
+  q, out = DeviceBuffer.empty((n, h * d), np.float32), DeviceBuffer.empty((n, h * d), np.float32)
+  _lib.check(_lib.load().b200q_attn_prefill(xb.ptr, k.ptr, v.ptr, _lib.F16, rb.ptr, 0, n, h, hk, d, d, ctx, q.ptr, out.ptr, _lib.F32, None))
+  want = out.numpy()
+  cache = paged.PagedCache(8, ps, hk, d)
+  pages = rng.permutation(8).astype(np.int32)[None]
+  batch = paged.PagedBatch(i32([0, n]), i32([n]), i32(pages), n_rows=n, max_new=n, max_len=n)
+  paged.append(cache, batch, xb, q, h, rope=rb)
+  paged.attention(cache, batch, q, out, h)
+  kp = cache.k.numpy((8, hk, ps, d), np.float16)[pages[0]].transpose(1, 0, 2, 3).reshape(hk, ctx, d)
+  # a c - b s in 32 bits with one of the products rounded or the other: two values within 2^-23 (|a| + |b|) of each other, which may lie on either side of a border between two
+  # fp16 values.  They are rounded to neighbours then: a step of the larger one apart, 2^-10 of it at most
+  kc = k.numpy()[:, :n].astype(np.float64)
+  assert (np.abs(kp[:, :n].astype(np.float64) - kc) <= EPS["float16"] * np.abs(kc) + 2 * TINY["float16"]).all()
+  np.testing.assert_allclose(out.numpy(), want, rtol=0, atol=2e-5)

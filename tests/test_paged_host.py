@@ -1,0 +1,127 @@
+"""What the paged-cache entry points refuse, without a device, and the host side of their classes."""
+import ctypes
+import numpy as np
+import pytest
+from tinygrad_b200 import _lib, build, paged
+from tinygrad_b200._lib import F32, F16, BF16
+
+
+@pytest.fixture(scope="module")
+def lib():
+  build.build_lib()
+  return _lib.load()
+
+
+P = 0x1000
+
+
+def cache(**kw):
+  c = _lib.PagedCacheDesc(P, P, F16, 10, 16, 2, 64, 2 * 16 * 64, 16 * 64, 64)
+  for k, v in kw.items(): setattr(c, k, v)
+  return c
+
+
+def batch(**kw):
+  b = _lib.PagedBatchDesc(P, P, P, 2, 4, 3, 2, 60)
+  for k, v in kw.items(): setattr(b, k, v)
+  return b
+
+
+def call(fn, *structs): return fn(*[None if s is None else ctypes.byref(s) for s in structs], 0, None)
+
+
+BAD_CACHE = [(dict(k=None), -1), (dict(v=None), -1), (dict(dtype=3), -1), (dict(n_pages=0), -1), (dict(page_size=0), -1), (dict(n_kv_heads=-1), -1), (dict(head_dim=96), -2), (dict(head_dim=0), -2),
+             (dict(row_stride=32), -2), (dict(head_stride=0), -2), (dict(page_stride=-2048), -2), (dict(row_stride=68), -3), (dict(k=P + 8), -3)]
+BAD_BATCH = [(dict(row_off=None), -1), (dict(length=None), -1), (dict(pages=None), -1), (dict(n_seqs=-1), -1), (dict(n_rows=-1), -1), (dict(table_stride=0), -1), (dict(max_new=0), -1), (dict(max_len=-1), -1),
+             (dict(length=P + 2), -3)]
+
+
+@pytest.mark.parametrize("change,code", [(("cache", c), e) for c, e in BAD_CACHE] + [(("batch", c), e) for c, e in BAD_BATCH])
+def test_caches_and_batches_that_are_refused(lib, change, code):
+  c, b = cache(**change[1] if change[0] == "cache" else {}), batch(**change[1] if change[0] == "batch" else {})
+  assert call(lib.b200q_paged_append, c, b, _lib.PagedAppendArgs(P, P, F32, F32, 0, 0, 4)) == code
+  assert call(lib.b200q_paged_attention, c, b, _lib.PagedAttnArgs(P, P, F32, F32, 0, 0, 4, 0.0, P, 1 << 30)) == code
+  assert lib.b200q_paged_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(b), 4) == 0
+
+
+@pytest.mark.parametrize("change,code", [(dict(x=None), -1), (dict(q=None), -1), (dict(x_dtype=5), -1), (dict(q_dtype=-1), -1), (dict(n_heads=0), -1), (dict(x_stride=8 * 64 - 1), -2), (dict(q_stride=255), -2),
+                                         (dict(rope=P, rope_dim=0, rope_len=8), -1), (dict(rope=P, rope_dim=32, rope_len=0), -1), (dict(rope=P, rope_dim=31, rope_len=8), -2), (dict(rope=P, rope_dim=66, rope_len=8), -2),
+                                         (dict(rope=P + 1, rope_dim=32, rope_len=8), -3), (dict(x=P + 2), -3), (dict(q=P + 3), -3), (dict(k_norm=P + 1), -3), (dict(q=2 * P, q_stride=512), -1),
+                                         (dict(q=2 * P, q_dtype=F16, x_stride=512, q_stride=512), -1), (dict(n_heads=1 << 28), -2)])
+def test_append_refuses(lib, change, code):
+  a = _lib.PagedAppendArgs(2 * P, P, F32, F32, 0, 0, 4)
+  for k, v in change.items(): setattr(a, k, v)
+  if change.get("q") == 2 * P and "x_stride" not in change: a.x_stride = 600      # in place with other strides
+  assert call(lib.b200q_paged_append, cache(), batch(), a) == code
+
+
+@pytest.mark.parametrize("change,code", [(dict(q=None), -1), (dict(out=None), -1), (dict(q_dtype=9), -1), (dict(out_dtype=9), -1), (dict(n_heads=3), -1), (dict(n_heads=0), -1), (dict(scale=-1.0), -1),
+                                         (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(q_stride=255), -2), (dict(out_stride=10), -2), (dict(q=P + 2), -3), (dict(out=P + 1), -3),
+                                         (dict(workspace=P + 16), -3), (dict(workspace=None), -6), (dict(workspace_bytes=100), -6)])
+def test_attention_refuses(lib, change, code):
+  a = _lib.PagedAttnArgs(P, P, F32, F32, 0, 0, 4, 0.0, P, 1 << 30)
+  for k, v in change.items(): setattr(a, k, v)
+  b = batch(max_len=100000, table_stride=7000)      # long enough to be split over CTAs
+  assert lib.b200q_paged_attention_workspace_bytes(ctypes.byref(cache()), ctypes.byref(b), 4) > 100
+  assert call(lib.b200q_paged_attention, cache(), b, a) == code
+
+
+@pytest.mark.parametrize("change,code", [(dict(x=None), -1), (dict(out=None), -1), (dict(n_rows=-1), -1), (dict(n_heads=-1), -1), (dict(n_heads=0, n_kv_heads=0), -1), (dict(x_dtype=7), -1), (dict(out_dtype=7), -1),
+                                         (dict(head_dim=48), -2), (dict(x_stride=100), -2), (dict(out_stride=100), -2), (dict(rope=P, rope_dim=64, rope_len=9), -1), (dict(rope=P, rope_dim=65, rope_len=9, positions=P), -2),
+                                         (dict(rope=P, rope_dim=64, rope_len=9, positions=P + 1), -3), (dict(x=P + 1), -3), (dict(q_norm=P + 1), -3), (dict(out=2 * P, out_stride=1000), -1),
+                                         (dict(out=2 * P, out_dtype=F16), -1)])
+def test_head_norm_rope_refuses(lib, change, code):
+  a = _lib.HeadNormArgs(2 * P, P, F32, F32, 0, 0, 5, 4, 2, 64)
+  for k, v in change.items(): setattr(a, k, v)
+  assert lib.b200q_head_norm_rope(ctypes.byref(a), 0, None) == code
+
+
+def test_nothing_to_do_is_fine(lib):
+  for b in (batch(n_seqs=0, row_off=None, length=None, pages=None), batch(n_rows=0)):
+    assert call(lib.b200q_paged_append, cache(), b, _lib.PagedAppendArgs(None, None, F32, F32, 0, 0, 4)) == 0
+    assert call(lib.b200q_paged_attention, cache(), b, _lib.PagedAttnArgs(None, None, F32, F32, 0, 0, 4)) == 0
+  assert lib.b200q_head_norm_rope(ctypes.byref(_lib.HeadNormArgs(None, None, F32, F32, 0, 0, 0, 4, 2, 64)), 0, None) == 0
+
+
+def test_structs_have_the_header_s_layout(tmp_path):
+  import pathlib, shutil, subprocess
+  cc = shutil.which("gcc") or shutil.which("cc")
+  if not cc: pytest.skip("no host C compiler")
+  hdr = pathlib.Path(__file__).resolve().parent.parent / "include" / "b200q.h"
+  structs = {"b200q_paged_cache": _lib.PagedCacheDesc, "b200q_paged_batch": _lib.PagedBatchDesc, "b200q_paged_append_args": _lib.PagedAppendArgs, "b200q_head_norm_args": _lib.HeadNormArgs,
+             "b200q_paged_attn_args": _lib.PagedAttnArgs}
+  lines = ["#include <stdio.h>", "#include <stddef.h>", f'#include "{hdr}"', "int main(void) {"]
+  for c, t in structs.items():
+    lines += [f'printf("{c} %zu\\n", sizeof({c}));'] + [f'printf("{c}.{f} %zu\\n", offsetof({c}, {f}));' for f, _ in t._fields_]
+  (tmp_path / "l.c").write_text("\n".join(lines + ["return 0;", "}"]))
+  subprocess.run([cc, "-o", str(tmp_path / "l"), str(tmp_path / "l.c")], check=True)
+  got = dict(l.split() for l in subprocess.run([str(tmp_path / "l")], check=True, capture_output=True, text=True).stdout.splitlines())
+  for c, t in structs.items():
+    assert int(got[c]) == ctypes.sizeof(t), c
+    for f, _ in t._fields_: assert int(got[f"{c}.{f}"]) == getattr(t, f).offset, f"{c}.{f}"
+
+
+class Fake:
+  """A buffer that is only asked for its address, size and type."""
+  def __init__(self, shape, dtype): self.shape, self.dtype, self.ptr, self.nbytes = tuple(shape), np.dtype(dtype), P, int(np.prod(shape)) * np.dtype(dtype).itemsize
+
+
+def test_python_side_refuses(lib):
+  i = lambda *s: Fake(s, np.int32)
+  with pytest.raises(ValueError, match="both pools"): paged.PagedCache(4, 16, 2, 64, k=Fake((4, 2, 16, 64), np.float16))
+  with pytest.raises(ValueError, match="element type"): paged.PagedCache(4, 16, 2, 64, "int8", k=P, v=P)
+  with pytest.raises(ValueError, match="at least 1"): paged.PagedCache(4, 0, 2, 64, k=P, v=P)
+  with pytest.raises(ValueError, match="k has"): paged.PagedCache(4, 16, 2, 64, k=Fake((4, 2, 16, 63), np.float16), v=P)
+  with pytest.raises(ValueError, match="shorter"): paged.PagedCache(4, 16, 2, 64, k=P, v=P, strides=(2048, 1024, 32))
+  with pytest.raises(ValueError, match="do not match"): paged.PagedBatch(i(2), i(2), i(2, 5), 2, 1, 9)
+  with pytest.raises(ValueError, match="do not match"): paged.PagedBatch(i(3), i(2), i(3, 5), 2, 1, 9)
+  with pytest.raises(ValueError, match="at least one"): paged.PagedBatch(i(3), i(2), i(2, 0), 2, 1, 9)
+  with pytest.raises(ValueError, match="bounds"): paged.PagedBatch(i(3), i(2), i(2, 5), 2, -1, 9)
+  with pytest.raises(TypeError, match="int32"): paged.PagedBatch(i(3), Fake((2,), np.int64), i(2, 5), 2, 1, 9)
+  c, b = paged.PagedCache(4, 16, 2, 64, k=P, v=P), paged.PagedBatch(i(3), i(2), i(2, 5), 2, 1, 9)
+  with pytest.raises(ValueError, match="x has"): paged.append(c, b, Fake((2, 7, 64), np.float32), P, 4)
+  with pytest.raises(ValueError, match="q has"): paged.append(c, b, P, Fake((1, 4, 64), np.float32), 4)
+  with pytest.raises(TypeError, match="float16"): paged.append(c, b, P, P, 4, q_norm=Fake((64,), np.float32))
+  with pytest.raises(ValueError, match="out has"): paged.attention(c, b, P, Fake((2, 4, 63), np.float32), 4)
+  with pytest.raises(ValueError, match="positions has"): paged.head_norm_rope(P, P, 5, 4, 2, 64, rope=Fake((9, 64), np.float32), positions=i(4))
+  with pytest.raises(_lib.B200QError): paged.attention(c, b, P, P, 3)

@@ -78,6 +78,32 @@ class Fp8LinearDesc(Structure):
               ("x_q", c_void_p), ("x_e8", c_void_p), ("off", c_void_p), ("parts", c_void_p), ("factor", c_void_p)]
 
 
+class PagedCacheDesc(Structure):
+  _fields_ = [("k", c_void_p), ("v", c_void_p), ("dtype", c_int), ("n_pages", c_int), ("page_size", c_int), ("n_kv_heads", c_int), ("head_dim", c_int),
+              ("page_stride", c_int64), ("head_stride", c_int64), ("row_stride", c_int64)]
+
+
+class PagedBatchDesc(Structure):
+  _fields_ = [("row_off", c_void_p), ("length", c_void_p), ("pages", c_void_p), ("n_seqs", c_int), ("table_stride", c_int), ("n_rows", c_int), ("max_new", c_int),
+              ("max_len", c_int)]
+
+
+class PagedAppendArgs(Structure):
+  _fields_ = [("x", c_void_p), ("q", c_void_p), ("x_dtype", c_int), ("q_dtype", c_int), ("x_stride", c_int64), ("q_stride", c_int64), ("n_heads", c_int),
+              ("norm_eps", c_float), ("q_norm", c_void_p), ("k_norm", c_void_p), ("rope", c_void_p), ("rope_dim", c_int), ("rope_len", c_int)]
+
+
+class HeadNormArgs(Structure):
+  _fields_ = [("x", c_void_p), ("out", c_void_p), ("x_dtype", c_int), ("out_dtype", c_int), ("x_stride", c_int64), ("out_stride", c_int64), ("n_rows", c_int),
+              ("n_heads", c_int), ("n_kv_heads", c_int), ("head_dim", c_int), ("norm_eps", c_float), ("q_norm", c_void_p), ("k_norm", c_void_p), ("rope", c_void_p),
+              ("rope_dim", c_int), ("rope_len", c_int), ("positions", c_void_p)]
+
+
+class PagedAttnArgs(Structure):
+  _fields_ = [("q", c_void_p), ("out", c_void_p), ("q_dtype", c_int), ("out_dtype", c_int), ("q_stride", c_int64), ("out_stride", c_int64), ("n_heads", c_int),
+              ("scale", c_float), ("workspace", c_void_p), ("workspace_bytes", c_size_t)]
+
+
 # name -> (restype, argtypes); every symbol include/b200q.h declares
 SIGNATURES = {
   "b200q_strerror": (c_char_p, [c_int]),
@@ -192,6 +218,10 @@ SIGNATURES = {
   "b200q_mx_status_read_clear": (c_int, [POINTER(c_int)]),
   "b200q_moe_layer": (c_int, [POINTER(MoeArgs), c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
   "b200q_row_gemv": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int, c_void_p]),
+  "b200q_paged_append": (c_int, [POINTER(PagedCacheDesc), POINTER(PagedBatchDesc), POINTER(PagedAppendArgs), c_int, c_void_p]),
+  "b200q_head_norm_rope": (c_int, [POINTER(HeadNormArgs), c_int, c_void_p]),
+  "b200q_paged_attention_workspace_bytes": (c_size_t, [POINTER(PagedCacheDesc), POINTER(PagedBatchDesc), c_int]),
+  "b200q_paged_attention": (c_int, [POINTER(PagedCacheDesc), POINTER(PagedBatchDesc), POINTER(PagedAttnArgs), c_int, c_void_p]),
   "b200q_moe_rows": (c_int, [POINTER(RowsArgs), POINTER(MoeBlock), c_int, c_int, c_void_p, c_int, c_void_p]),
   "b200q_grouped_mxfp8_gemm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),
   "b200q_grouped_mxfp8_gemm_f32": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p]),

@@ -63,6 +63,8 @@ int b200q_moe_router_one(const b200q_moe_args* m, const void* router, int router
 int b200q_decode_status_take(int* status);
 int b200q_decode_step_status_take(int* status);   // the same for the whole-step kernel (decode_step.cu)
 int b200q_peer_status_take(int* status);          // the same for the peer-memory collectives (peer.cu)
+int b200q_paged_status_take(int* status);         // the same for rows on their way into a paged cache (paged.cu) ...
+int b200q_paged_attn_status_take(int* status);    // ... and for attention over it (paged_attn.cu)
 int b200q_qgemm_stream_status_take(int* status);  // the same for the many-row GEMM (qgemm_stream.cu)
 int b200q_ep_status_take(int* status);            // the same for the expert-parallel exchange (ep.cu)
 // current device index, or -1 (with the CUDA error recorded) if it cannot be had or is past the tables

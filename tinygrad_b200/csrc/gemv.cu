@@ -25,6 +25,7 @@
 #include "actquant.cuh"
 #include "qgemv_core.cuh"
 #include "kquant_wide.cuh"
+#include <initializer_list>
 
 namespace {
 
@@ -664,6 +665,12 @@ extern "C" int b200q_status_read_clear(int* status) {
   const int rc3 = b200q_peer_status_take(&peer);
   if (rc3 != B200Q_OK) return rc3;
   if (peer && !*status) *status = peer;
+  for (auto take : {b200q_paged_status_take, b200q_paged_attn_status_take}) {
+    int paged = 0;
+    const int rc4 = take(&paged);
+    if (rc4 != B200Q_OK) return rc4;
+    if (paged && !*status) *status = paged;
+  }
   return B200Q_OK;
 }
 

@@ -1,0 +1,75 @@
+// What the paged-cache kernels share: argument checks, element types, where a row or a page is.
+#pragma once
+#include "common.cuh"
+#include <cuda_bf16.h>
+
+namespace {
+
+// ---- element types ----
+__host__ __device__ constexpr int type_size(int t) { return t == B200Q_F32 ? 4 : 2; }
+static inline bool type_known(int t) { return t == B200Q_F32 || t == B200Q_F16 || t == B200Q_BF16; }
+template <int T> struct Elem;
+template <> struct Elem<B200Q_F32> { typedef float type; };
+template <> struct Elem<B200Q_F16> { typedef __half type; };
+template <> struct Elem<B200Q_BF16> { typedef __nv_bfloat16 type; };
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ uint32_t pack2(float a, float b, int type) {      // two 16-bit values, rounded to nearest
+  if (type == B200Q_F16) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float load_as_f(const void* base, int type, int64_t i) {
+  return type == B200Q_F32 ? static_cast<const float*>(base)[i] : type == B200Q_F16 ? __half2float(static_cast<const __half*>(base)[i])
+                                                                                   : __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]);
+}
+__device__ __forceinline__ void store_as(void* base, int type, int64_t i, float v) {
+  if (type == B200Q_F32) static_cast<float*>(base)[i] = v;
+  else if (type == B200Q_F16) static_cast<__half*>(base)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(v);
+}
+
+// ---- tables ----
+struct PagedTables {
+  const int32_t *row_off, *length, *pages;
+  int n_seqs, table_stride, n_rows, max_new, max_len, n_pages, page_size;
+};
+
+// The sequence of a row, by a whole warp: the number of sequences that end at or before it.  One token of every sequence is the usual case: asked first.
+__device__ __forceinline__ int seq_of_row(const PagedTables& t, int row) {
+  const int lane = threadIdx.x & 31, guess = min(row, t.n_seqs - 1);
+  const int g0 = t.row_off[guess], g1 = t.row_off[guess + 1];
+  if (g0 <= row && row < g1) return guess;
+  int seq = 0;
+  for (int s0 = 0; s0 < t.n_seqs; s0 += 32) {
+    const bool before = s0 + lane < t.n_seqs && t.row_off[s0 + lane + 1] <= row;
+    const int c = __popc(__ballot_sync(0xffffffffu, before));
+    seq += c;
+    if (c < 32) break;
+  }
+  return min(seq, t.n_seqs - 1);
+}
+
+// ---- checks of what all entry points take ----
+static inline int check_cache(const b200q_paged_cache* c) {
+  if (!c || !c->k || !c->v || !type_known(c->dtype) || c->n_pages <= 0 || c->page_size <= 0 || c->n_kv_heads <= 0) return B200Q_ERR_BAD_ARG;
+  if (c->head_dim != 16 && c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128) return B200Q_ERR_BAD_SHAPE;
+  const int64_t unit = 16 / type_size(c->dtype);
+  if (c->page_stride < c->head_dim || c->head_stride < c->head_dim || c->row_stride < c->head_dim) return B200Q_ERR_BAD_SHAPE;
+  if (c->page_stride % unit || c->head_stride % unit || c->row_stride % unit || (((uintptr_t)c->k | (uintptr_t)c->v) & 15)) return B200Q_ERR_MISALIGNED;
+  return B200Q_OK;
+}
+static inline int check_batch(const b200q_paged_batch* b) {
+  if (!b || b->n_seqs < 0 || b->n_rows < 0 || b->max_new < 0 || b->max_len < 0) return B200Q_ERR_BAD_ARG;
+  if (b->n_seqs == 0 || b->n_rows == 0) return B200Q_OK;
+  if (!b->row_off || !b->length || !b->pages || b->table_stride <= 0 || b->max_new <= 0) return B200Q_ERR_BAD_ARG;
+  if (((uintptr_t)b->row_off | (uintptr_t)b->length | (uintptr_t)b->pages) & 3) return B200Q_ERR_MISALIGNED;
+  return B200Q_OK;
+}
+static inline PagedTables tables_of(const b200q_paged_cache* c, const b200q_paged_batch* b) {
+  return PagedTables{b->row_off, b->length, b->pages, b->n_seqs, b->table_stride, b->n_rows, b->max_new, b->max_len, c->n_pages, c->page_size};
+}
+
+}  // namespace

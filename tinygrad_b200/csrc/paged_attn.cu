@@ -1,0 +1,302 @@
+// Attention of a batch's new tokens over a paged KV cache (tinygrad/llm/model.py:187-195 with a cache of pages and sequences of different lengths).
+//   row (token i of n, query head h), position p = length - n + i:  out = sum_{j <= p} e^(s_j - m) v_j / sum_{j <= p} e^(s_j - m),  s_j = scale q . k_j,  m = max s_j,
+// in one pass over the keys with the running maximum and sums of the softmax (32-bit); KV head h / G serves the G query heads of its group.
+//
+// Work is dealt as (tile of rows, KV head, part of the keys).  A tile is R consecutive (token, head of the group) pairs of one sequence, token-major, so the group's heads share every key
+// that is loaded.  The keys are split over CTAs where the tiles alone do not fill the GPU: parts leave (m, sum, weighted sum) in the workspace and the one that is done
+// last adds them, in the order of the keys (results do not depend on timing), and puts its counter back.
+#include "paged.cuh"
+
+namespace {
+
+__device__ int g_paged_attn_status = 0;
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct AttnParams {
+  const void *q, *k, *v;
+  void* out;
+  int q_dtype, out_dtype;
+  int64_t q_stride, out_stride, page_stride, head_stride, row_stride;
+  int n_heads, n_kv, group;
+  float scale;               // times log2 e
+  int tiles_per_seq;         // 0: tiles are counted sequence by sequence
+  int n_split, split_len;
+  int* counters;
+  float* parts;
+  PagedTables t;
+};
+
+struct TilePlace { int seq, first_row, n, r0, length, keys; };       // r0: the tile's first (token, head) pair; keys: those its last row sees, at most
+
+// R pairs to a tile; by a whole warp.  n == 0: nothing to do.
+template <int R>
+__device__ __forceinline__ TilePlace place_of_tile(const AttnParams& p, int tile) {
+  const PagedTables& t = p.t;
+  const int lane = threadIdx.x & 31;
+  TilePlace w{0, 0, 0, 0, 0, 0};
+  auto rows = [&](int s) {
+    const int b = min(max(t.row_off[s], 0), t.n_rows), e = min(max(t.row_off[s + 1], b), t.n_rows);
+    return make_int2(b, e - b);
+  };
+  if (p.tiles_per_seq) {
+    w.seq = tile / p.tiles_per_seq;
+    w.r0 = (tile - w.seq * p.tiles_per_seq) * R;
+  } else {
+    int s = 0, before = 0;
+    bool found = false;
+    for (int s0 = 0; s0 < t.n_seqs && !found; s0 += 32) {
+      int mine = 0;
+      if (s0 + lane < t.n_seqs) mine = (int)(((int64_t)min(rows(s0 + lane).y, t.max_new) * p.group + R - 1) / R);
+      int sum = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += u; }
+      const unsigned here = __ballot_sync(0xffffffffu, tile < before + sum);
+      if (here) {
+        const int l = __ffs(here) - 1;
+        s = s0 + l;
+        before += __shfl_sync(0xffffffffu, sum - mine, l);
+        found = true;
+      } else before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (!found) return w;
+    w.seq = s;
+    w.r0 = (tile - before) * R;
+  }
+  const int2 r = rows(w.seq);
+  w.first_row = r.x;
+  w.length = t.length[w.seq];
+  const int n = min(r.y, t.max_new);
+  if (w.r0 >= (int64_t)n * p.group) return w;
+  w.n = n;
+  const int64_t cap = min((int64_t)min(w.length, t.max_len), (int64_t)t.table_stride * t.page_size);
+  if ((r.y > n || w.length > cap) && lane == 0) atomicExch(&g_paged_attn_status, 2);
+  const int last = min((w.r0 + R - 1) / p.group, n - 1);
+  w.length -= r.y;                                           // from here on: the position of the first new token
+  w.keys = max(0, (int)min(cap, (int64_t)w.length + last + 1));
+  return w;
+}
+
+// the offset of a key in the pages, or -1
+__device__ __forceinline__ int64_t key_at(const AttnParams& p, int seq, int key) {
+  const int index = key / p.t.page_size, page = p.t.pages[(int64_t)seq * p.t.table_stride + index];
+  if (page < 0 || page >= p.t.n_pages) { atomicExch(&g_paged_attn_status, 2); return -1; }
+  return page * p.page_stride + (int64_t)(key - index * p.t.page_size) * p.row_stride;
+}
+
+// ---- parts of the keys ----
+template <int R, int D> constexpr int PART = R * (D + 2);           // m [R], sum [R], weighted sum [R][D]
+
+// The tile's last part to be done adds all of them; by the whole CTA (THREADS).  m in log2.
+template <int R, int D, int THREADS>
+__device__ __forceinline__ void join_parts(const AttnParams& p, const TilePlace& w, int unit, int n_parts, int kvh, int* s_flag) {
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const int old = atomicAdd(p.counters + unit, 1);
+    *s_flag = old == n_parts - 1;
+    if (old == n_parts - 1) p.counters[unit] = 0;
+  }
+  __syncthreads();
+  if (!*s_flag) return;
+  __threadfence();
+  const float* base = p.parts + (int64_t)unit * p.n_split * PART<R, D>;
+  for (int i = threadIdx.x; i < R * D; i += THREADS) {
+    const int r = i / D, d = i - r * D;
+    const int64_t pair = w.r0 + r;
+    if (pair >= (int64_t)w.n * p.group) break;
+    float m = -INFINITY, sum = 0.f, o = 0.f;
+    for (int s = 0; s < n_parts; s++) m = fmaxf(m, __ldcg(base + (int64_t)s * PART<R, D> + r));
+    for (int s = 0; s < n_parts; s++) {
+      const float* b = base + (int64_t)s * PART<R, D>;
+      const float ls = __ldcg(b + R + r), f = ls == 0.f ? 0.f : exp2f(__ldcg(b + r) - m);      // (a part without keys has sum 0)
+      sum = fmaf(f, ls, sum);
+      o = fmaf(f, __ldcg(b + 2 * R + i), o);
+    }
+    const int token = pair / p.group, head = kvh * p.group + (int)(pair - (int64_t)token * p.group);
+    store_as(p.out, p.out_dtype, (w.first_row + token) * p.out_stride + (int64_t)head * D + d, sum == 0.f ? 0.f : o / sum);
+  }
+}
+
+// ---- any types: multiply-adds in 32 bits.  A warp takes every fourth block of 32 keys, a key a lane for the scores, D / 32 values a lane for the weighted sum. ----
+constexpr int S_R = 16, S_WARPS = 4, S_THREADS = S_WARPS * 32;
+template <int D, typename KV>
+__global__ void __launch_bounds__(S_THREADS) attn_simple_kernel(const AttnParams p) {
+  constexpr int R = S_R, NV = D >= 32 ? D / 32 : 1, LIVE = D >= 32 ? 32 : D;
+  __shared__ float s_q[R][D], s_p[S_WARPS][R][32], s_o[R][D], s_m[S_WARPS][R], s_l[S_WARPS][R];
+  __shared__ int s_flag;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y, split = blockIdx.z;
+  const TilePlace w = place_of_tile<R>(p, blockIdx.x);
+  if (w.n == 0) return;
+  const int n_parts = max(1, (w.keys + p.split_len - 1) / p.split_len), k_begin = split * p.split_len, k_end = min(w.keys, k_begin + p.split_len);
+  if (split >= n_parts) return;
+  const int64_t pairs = (int64_t)w.n * p.group;
+  for (int i = tid; i < R * D; i += S_THREADS) {
+    const int r = i / D, d = i - r * D, pair = w.r0 + r, token = pair / p.group;
+    s_q[r][d] = pair < pairs ? load_as_f(p.q, p.q_dtype, (w.first_row + token) * p.q_stride + (int64_t)(kvh * p.group + pair - token * p.group) * D + d) * p.scale : 0.f;
+    s_o[r][d] = 0.f;
+  }
+  __syncthreads();
+  float o[R][NV], m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    m[r] = -INFINITY; l[r] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; j++) o[r][j] = 0.f;
+  }
+  const KV* kp = static_cast<const KV*>(p.k) + kvh * p.head_stride;
+  const KV* vp = static_cast<const KV*>(p.v) + kvh * p.head_stride;
+  for (int k0 = k_begin + warp * 32; k0 < k_end; k0 += S_WARPS * 32) {
+    const int key = k0 + lane;
+    const int64_t at = key < k_end ? key_at(p, w.seq, key) : -1;
+    float s[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) s[r] = 0.f;
+    for (int d = 0; d < D; d += 4) {
+      float f[4] = {0.f, 0.f, 0.f, 0.f};
+      if (at >= 0) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) f[j] = to_f(kp[at + d + j]);
+      }
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const float4 q = *reinterpret_cast<const float4*>(&s_q[r][d]);
+        s[r] = fmaf(q.x, f[0], fmaf(q.y, f[1], fmaf(q.z, f[2], fmaf(q.w, f[3], s[r]))));
+      }
+    }
+    int first = w.length + w.r0 / p.group, h = w.r0 % p.group;        // the position and head of row r
+    const bool all = k0 + 31 < k_end && k0 + 31 <= first;             // every row sees every key of the block
+    __syncwarp();
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      if (key >= k_end || key > first) s[r] = -INFINITY;
+      if (++h == p.group) { h = 0; first++; }
+      const float mn = fmaxf(m[r], warp_max(s[r])), c = mn == -INFINITY ? 1.f : exp2f(m[r] - mn);
+      const float e = mn == -INFINITY && s[r] == -INFINITY ? 0.f : exp2f(s[r] - mn);
+      m[r] = mn;
+      l[r] = l[r] * c + warp_sum(e);
+#pragma unroll
+      for (int j = 0; j < NV; j++) o[r][j] *= c;
+      s_p[warp][r][lane] = s[r] == -INFINITY ? 0.f : e;
+    }
+    __syncwarp();
+    const int n = min(32, k_end - k0);
+    for (int j = 0; j < n; j++) {
+      const int64_t vat = __shfl_sync(0xffffffffu, at, j);
+      float f[NV];
+#pragma unroll
+      for (int i = 0; i < NV; i++) f[i] = vat >= 0 && lane < LIVE ? to_f(vp[vat + lane + i * 32]) : 0.f;
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const float e = s_p[warp][r][j];
+#pragma unroll
+        for (int i = 0; i < NV; i++) o[r][i] = all || e != 0.f ? fmaf(e, f[i], o[r][i]) : o[r][i];      // (a masked value may be anything)
+      }
+    }
+  }
+  // the warps' sums, in the order of the warps
+  if (lane == 0)
+#pragma unroll
+    for (int r = 0; r < R; r++) { s_m[warp][r] = m[r]; s_l[warp][r] = l[r]; }
+  __syncthreads();
+  float mt[R];
+#pragma unroll
+  for (int r = 0; r < R; r++) mt[r] = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+  for (int x = 0; x < S_WARPS; x++) {
+    if (x == warp && lane < LIVE)
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const float c = l[r] == 0.f ? 0.f : exp2f(m[r] - mt[r]);
+#pragma unroll
+        for (int i = 0; i < NV; i++) s_o[r][lane + i * 32] += o[r][i] * c;
+      }
+    __syncthreads();
+  }
+  const int unit = blockIdx.x * p.n_kv + kvh;
+  float* mine = p.parts + ((int64_t)unit * p.n_split + split) * PART<R, D>;
+  for (int i = tid; i < R * D; i += S_THREADS) {
+    const int r = i / D, d = i - r * D, pair = w.r0 + r, token = pair / p.group;
+    if (pair >= pairs) break;
+    float ml = -INFINITY, sum = 0.f;
+    for (int x = 0; x < S_WARPS; x++) ml = fmaxf(ml, s_m[x][r]);
+    for (int x = 0; x < S_WARPS; x++) sum += s_l[x][r] == 0.f ? 0.f : s_l[x][r] * exp2f(s_m[x][r] - ml);
+    if (n_parts == 1) {
+      store_as(p.out, p.out_dtype, (w.first_row + token) * p.out_stride + (int64_t)(kvh * p.group + pair - token * p.group) * D + d, sum == 0.f ? 0.f : s_o[r][d] / sum);
+    } else {
+      if (d == 0) { __stcg(mine + r, ml); __stcg(mine + R + r, sum); }
+      __stcg(mine + 2 * R + i, s_o[r][d]);
+    }
+  }
+  if (n_parts > 1) join_parts<R, D, S_THREADS>(p, w, unit, n_parts, kvh, &s_flag);
+}
+
+// ---- how the work is dealt ----
+struct Plan { int tiles, tiles_per_seq, n_split, split_len; };
+
+// Tiles of `rows` pairs: those of all sequences at their largest, or (ragged batches, if that is less) the pairs' tiles and a broken one for each sequence.  Keys are split until
+// there are about `want` CTAs, in parts of at least `least` keys.
+Plan make_plan(const b200q_paged_batch* b, int n_kv, int group, int rows, int want, int least) {
+  const int64_t per = ((int64_t)b->max_new * group + rows - 1) / rows, even = per * b->n_seqs, ragged = (int64_t)b->n_rows * group / rows + b->n_seqs;
+  Plan p{};
+  p.tiles_per_seq = even <= ragged ? (int)per : 0;
+  p.tiles = (int)(even <= ragged ? even : ragged);
+  const int64_t len = b->max_len > 0 ? b->max_len : 1, most = (len + least - 1) / least;
+  const int64_t parts = want / ((int64_t)p.tiles * n_kv);
+  const int64_t n = parts < 1 ? 1 : parts < most ? parts : most;
+  p.split_len = (int)((len + n - 1) / n + 31) / 32 * 32;
+  p.n_split = (int)((len + p.split_len - 1) / p.split_len);
+  return p;
+}
+
+size_t workspace_of(const Plan& p, int n_kv, int rows, int dim, size_t* counters) {
+  *counters = ((size_t)p.tiles * n_kv * 4 + 255) / 256 * 256;
+  return p.n_split == 1 ? 0 : *counters + (size_t)p.tiles * n_kv * p.n_split * rows * (dim + 2) * 4;
+}
+
+Plan simple_plan(const b200q_paged_batch* b, int n_kv, int group) { return make_plan(b, n_kv, group, S_R, 4 * 148, 256); }
+
+}  // namespace
+
+int b200q_paged_attn_status_take(int* status) {
+  int zero = 0;
+  B200Q_CHECK_CUDA(cudaMemcpyFromSymbol(status, g_paged_attn_status, sizeof(int)));
+  B200Q_CHECK_CUDA(cudaMemcpyToSymbol(g_paged_attn_status, &zero, sizeof(int)));
+  return B200Q_OK;
+}
+
+extern "C" size_t b200q_paged_attention_workspace_bytes(const b200q_paged_cache* cache, const b200q_paged_batch* batch, int n_heads) {
+  if (check_cache(cache) != B200Q_OK || check_batch(batch) != B200Q_OK || n_heads <= 0 || n_heads % cache->n_kv_heads || batch->n_seqs == 0 || batch->n_rows == 0) return 0;
+  size_t c;
+  return workspace_of(simple_plan(batch, cache->n_kv_heads, n_heads / cache->n_kv_heads), cache->n_kv_heads, S_R, cache->head_dim, &c);
+}
+
+template <int D>
+static void (*pick_simple(int kv_dtype))(const AttnParams) {
+  return kv_dtype == B200Q_F32 ? attn_simple_kernel<D, float> : kv_dtype == B200Q_F16 ? attn_simple_kernel<D, __half> : attn_simple_kernel<D, __nv_bfloat16>;
+}
+
+extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q_paged_batch* batch, const b200q_paged_attn_args* a, int flags, void* stream) {
+  int rc = check_cache(cache);
+  if (rc == B200Q_OK) rc = check_batch(batch);
+  if (rc != B200Q_OK) return rc;
+  if (!a || a->n_heads <= 0 || a->n_heads % cache->n_kv_heads || !type_known(a->q_dtype) || !type_known(a->out_dtype) || !(a->scale >= 0.f) || a->scale > 3.4e38f) return B200Q_ERR_BAD_ARG;
+  const int dim = cache->head_dim, n_kv = cache->n_kv_heads, group = a->n_heads / n_kv;
+  const int64_t row = (int64_t)a->n_heads * dim;
+  if ((a->q_stride && a->q_stride < row) || (a->out_stride && a->out_stride < row) || row > INT32_MAX || (int64_t)batch->max_new * group > INT32_MAX - 1024) return B200Q_ERR_BAD_SHAPE;
+  if (batch->n_seqs == 0 || batch->n_rows == 0) return B200Q_OK;
+  if (!a->q || !a->out) return B200Q_ERR_BAD_ARG;
+  if ((uintptr_t)a->q % type_size(a->q_dtype) || (uintptr_t)a->out % type_size(a->out_dtype) || (uintptr_t)a->workspace & 255) return B200Q_ERR_MISALIGNED;
+  const Plan plan = simple_plan(batch, n_kv, group);
+  if (plan.n_split > 65535 || n_kv > 65535) return B200Q_ERR_TOO_LARGE;
+  size_t counters;
+  const size_t need = workspace_of(plan, n_kv, S_R, dim, &counters);
+  if (need && (!a->workspace || a->workspace_bytes < need)) return B200Q_ERR_TOO_LARGE;
+  const AttnParams p{a->q, cache->k, cache->v, a->out, a->q_dtype, a->out_dtype, a->q_stride ? a->q_stride : row, a->out_stride ? a->out_stride : row, cache->page_stride,
+                     cache->head_stride, cache->row_stride, a->n_heads, n_kv, group, (a->scale > 0.f ? a->scale : 1.f / sqrtf((float)dim)) * LOG2E, plan.tiles_per_seq, plan.n_split,
+                     plan.split_len, (int*)a->workspace, (float*)((char*)a->workspace + counters), tables_of(cache, batch)};
+  auto kernel = dim == 16 ? pick_simple<16>(cache->dtype) : dim == 32 ? pick_simple<32>(cache->dtype) : dim == 64 ? pick_simple<64>(cache->dtype) : pick_simple<128>(cache->dtype);
+  B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles, n_kv, plan.n_split), dim3(S_THREADS), 0, (cudaStream_t)stream, (flags & B200Q_FLAG_PDL) != 0, p));
+  return B200Q_OK;
+}

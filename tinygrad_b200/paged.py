@@ -1,0 +1,146 @@
+"""A paged KV cache and what reads and writes it: for serving sequences of different lengths in one batch.
+
+`PagedCache` holds one block's keys and values in pages of `page_size` positions, `PagedBatch` the tables that say which rows (new tokens) and pages belong to
+which sequence; all of it lives on the device, so that a captured step follows the lengths.  `append` takes the projections of the new tokens into the pages (norms of the heads and
+rotation on the way), `attention` is the attention of the new tokens over the pages -- TransformerBlock._attention of tinygrad/llm/model.py:167-207 for a
+ragged batch --, `head_norm_rope` the norms and the rotation alone, for caches that are not paged.
+
+Buffers are DeviceBuffers, raw addresses or foreign tensors of the current device (`runtime.ptr_of`); bf16 values are uint16 in a DeviceBuffer.  Calls launch on `stream` and return at
+once; a batch's workspace serves one call at a time: streams and graphs that may run together need a PagedBatch each."""
+import ctypes
+import numpy as np
+from . import _lib
+from ._lib import check, F32, F16, BF16
+from .runtime import DeviceBuffer, ptr_of, stream_ptr, synchronize
+
+DTYPES = {"float32": F32, "float16": F16, "bfloat16": BF16}
+_NP = {F32: np.float32, F16: np.float16, BF16: np.uint16}
+_SIZE = {F32: 4, F16: 2, BF16: 2}
+
+
+def _dtype(d) -> int:
+  t = DTYPES.get(d, d)
+  if not isinstance(t, int) or t not in _SIZE: raise ValueError(f"unknown element type {d!r}: float32, float16 or bfloat16")
+  return t
+
+
+def _ptr(o) -> int:
+  try: return o.data_ptr()
+  except AttributeError: return ptr_of(o)
+
+
+def _nbytes(o):      # None: not known (a raw address)
+  if o is None or isinstance(o, int): return None
+  n = getattr(o, "nbytes", None)
+  return n if isinstance(n, int) else None
+
+
+def _holds(o, nbytes: int, what: str) -> None:
+  have = _nbytes(o)
+  if have is not None and have < nbytes: raise ValueError(f"{what} has {have} bytes, needs {nbytes}")
+
+
+def _int32(o, what: str):
+  d = str(getattr(o, "dtype", "int32"))
+  if not d.endswith("int32") or d.endswith("uint32"): raise TypeError(f"{what} is a table of int32, got {d}")
+  return o
+
+
+class PagedCache:
+  """One block's keys and values: pools `k` and `v` of n_pages pages (allocated here, zeroed, unless given).  strides: elements from page to page, KV head to KV head and slot to
+  slot; the default is [page][head][slot][head_dim]."""
+  def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype="float16", k=None, v=None, strides: tuple = None):
+    if min(n_pages, page_size, n_kv_heads, head_dim) <= 0: raise ValueError("pages, page size, heads and head size are at least 1")
+    if (k is None) != (v is None): raise ValueError("give both pools or neither")
+    self.n_pages, self.page_size, self.n_kv_heads, self.head_dim, self.dtype = n_pages, page_size, n_kv_heads, head_dim, _dtype(dtype)
+    page, head, row = self.strides = tuple(strides) if strides is not None else (n_kv_heads * page_size * head_dim, page_size * head_dim, head_dim)
+    if min(self.strides) < head_dim: raise ValueError(f"strides {self.strides} are shorter than a head")
+    last = (n_pages - 1) * page + (n_kv_heads - 1) * head + (page_size - 1) * row + head_dim
+    if k is None: k, v = (DeviceBuffer.empty((last,), _NP[self.dtype], zero=True) for _ in range(2))
+    _holds(k, last * _SIZE[self.dtype], "k"), _holds(v, last * _SIZE[self.dtype], "v")
+    self.k, self.v = k, v
+    self.desc = _lib.PagedCacheDesc(_ptr(k), _ptr(v), self.dtype, n_pages, page_size, n_kv_heads, head_dim, page, head, row)
+    self.ref, self._key = ctypes.byref(self.desc), (self.dtype, page_size, n_kv_heads, head_dim)
+
+
+class PagedBatch:
+  """Which rows and pages belong to which sequence.  row_off int32 [n_seqs + 1]: sequence s has the rows row_off[s] .. row_off[s + 1] - 1, its new tokens; length int32 [n_seqs]: its
+  tokens in all, the new ones among them; pages int32 [n_seqs, most pages of a sequence].  The tables are read when the work runs and may change between calls (or replays of a
+  graph); n_rows (rows of the row arrays), max_new and max_len (of any sequence) are bounds that hold for all of them."""
+  def __init__(self, row_off, length, pages, n_rows: int, max_new: int, max_len: int):
+    if min(n_rows, max_new, max_len) < 0: raise ValueError("bounds are not negative")
+    (n_seqs,), (seqs, table) = length.shape, pages.shape
+    if seqs != n_seqs or tuple(row_off.shape) != (n_seqs + 1,): raise ValueError(f"row_off {tuple(row_off.shape)}, length {tuple(length.shape)} and pages {tuple(pages.shape)} do not match")
+    if n_seqs and table < 1: raise ValueError("a sequence has at least one entry in the table of pages")
+    if hasattr(pages, "is_contiguous") and not (pages.is_contiguous() and row_off.is_contiguous() and length.is_contiguous()): raise ValueError("tables are contiguous")
+    self.row_off, self.length, self.pages = _int32(row_off, "row_off"), _int32(length, "length"), _int32(pages, "pages")
+    self.n_seqs, self.n_rows, self.max_new, self.max_len = n_seqs, n_rows, max_new, max_len
+    self.desc = _lib.PagedBatchDesc(_ptr(row_off), _ptr(length), _ptr(pages), n_seqs, table, n_rows, max_new, max_len)
+    self.ref = ctypes.byref(self.desc)
+    self._ws, self._need, self._old = None, {}, []
+
+  def reserve(self, cache: PagedCache, n_heads: int, q_dtype="float32") -> None:
+    """Allocates the workspace that `attention` needs for such a cache (done by its first call otherwise; a call under capture allocates nothing)."""
+    _dtype(q_dtype)
+    need = self._need.get((cache._key, n_heads))
+    if need is None: need = self._need[(cache._key, n_heads)] = _lib.load().b200q_paged_attention_workspace_bytes(cache.ref, self.ref, n_heads)
+    if need and (self._ws is None or self._ws.nbytes < need):
+      if self._ws is not None: self._old.append(self._ws)      # graphs may hold it
+      self._ws = DeviceBuffer(need, zero=True)
+      synchronize()
+
+
+def append(cache: PagedCache, batch: PagedBatch, x, q, n_heads: int, x_dtype="float32", q_dtype=None, rope=None, q_norm=None, k_norm=None, norm_eps: float = 0.0, x_stride: int = 0,
+           q_stride: int = 0, flags: int = 0, stream=None) -> None:
+  """x rows [q | k | v] (x_dtype, x_stride elements apart, 0: back to back) of the batch's new tokens: q rows normed and rotated to `q` (q_dtype, the same as x's unless given), k likewise and v to
+  the pages.  rope: fp32 [positions, rotated dimensions], cos || sin (`model.precompute_freqs_cis`), or None; q_norm / k_norm: fp16 [head_dim], the weights of an RMSNorm over each head, or None."""
+  xt = _dtype(x_dtype)
+  qt = xt if q_dtype is None else _dtype(q_dtype)
+  n, d = batch.n_rows, cache.head_dim
+  if n:
+    row, q_row = (n_heads + 2 * cache.n_kv_heads) * d, n_heads * d
+    _holds(x, ((n - 1) * (x_stride or row) + row) * _SIZE[xt], "x"), _holds(q, ((n - 1) * (q_stride or q_row) + q_row) * _SIZE[qt], "q")
+  _check_norm(q_norm, d), _check_norm(k_norm, d)
+  rope_len, rope_dim = rope.shape if rope is not None else (0, 0)
+  a = _lib.PagedAppendArgs(_ptr(x), _ptr(q), xt, qt, x_stride, q_stride, n_heads, norm_eps, _ptr(q_norm) if q_norm is not None else None, _ptr(k_norm) if k_norm is not None else None,
+                           _ptr(rope) if rope is not None else None, rope_dim, rope_len)
+  check(_lib.load().b200q_paged_append(cache.ref, batch.ref, ctypes.byref(a), flags, stream_ptr(stream)))
+
+
+def attention(cache: PagedCache, batch: PagedBatch, q, out, n_heads: int, q_dtype="float32", out_dtype=None, scale: float = 0.0, q_stride: int = 0, out_stride: int = 0, flags: int = 0,
+              stream=None) -> None:
+  """out[row][head] = softmax(scale q . k) v over the positions up to the row's own (scale 0: head_dim ** -0.5); out_dtype is q's unless given."""
+  qt = _dtype(q_dtype)
+  ot = qt if out_dtype is None else _dtype(out_dtype)
+  n = batch.n_rows
+  if n:
+    row = n_heads * cache.head_dim
+    _holds(q, ((n - 1) * (q_stride or row) + row) * _SIZE[qt], "q"), _holds(out, ((n - 1) * (out_stride or row) + row) * _SIZE[ot], "out")
+  batch.reserve(cache, n_heads)
+  ws = batch._ws
+  a = _lib.PagedAttnArgs(_ptr(q), _ptr(out), qt, ot, q_stride, out_stride, n_heads, scale, ws.ptr if ws is not None else None, ws.nbytes if ws is not None else 0)
+  check(_lib.load().b200q_paged_attention(cache.ref, batch.ref, ctypes.byref(a), flags, stream_ptr(stream)))
+
+
+def _check_norm(w, d: int) -> None:
+  if w is None: return
+  t = str(getattr(w, "dtype", "float16"))
+  if not t.endswith("float16") or t.endswith("bfloat16"): raise TypeError(f"norm weights are float16, got {t}")
+  _holds(w, 2 * d, "a norm weight")
+
+
+def head_norm_rope(x, out, n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, x_dtype="float32", out_dtype=None, q_norm=None, k_norm=None, norm_eps: float = 0.0, rope=None,
+                   positions=None, x_stride: int = 0, out_stride: int = 0, flags: int = 0, stream=None) -> None:
+  """The norms and the rotation of the first n_heads (queries) + n_kv_heads (keys) heads of every row, from x to out, which may be x (strides and types as they are, then).  positions: int32
+  [n_rows] with rope."""
+  xt = _dtype(x_dtype)
+  ot = xt if out_dtype is None else _dtype(out_dtype)
+  row = (n_heads + n_kv_heads) * head_dim
+  if n_rows > 0:
+    _holds(x, ((n_rows - 1) * (x_stride or row) + row) * _SIZE[xt], "x"), _holds(out, ((n_rows - 1) * (out_stride or row) + row) * _SIZE[ot], "out")
+    if positions is not None: _holds(_int32(positions, "positions"), 4 * n_rows, "positions")
+  _check_norm(q_norm, head_dim), _check_norm(k_norm, head_dim)
+  rope_len, rope_dim = rope.shape if rope is not None else (0, 0)
+  a = _lib.HeadNormArgs(_ptr(x), _ptr(out), xt, ot, x_stride, out_stride, n_rows, n_heads, n_kv_heads, head_dim, norm_eps, _ptr(q_norm) if q_norm is not None else None,
+                        _ptr(k_norm) if k_norm is not None else None, _ptr(rope) if rope is not None else None, rope_dim, rope_len, _ptr(positions) if positions is not None else None)
+  check(_lib.load().b200q_head_norm_rope(ctypes.byref(a), flags, stream_ptr(stream)))
