@@ -232,6 +232,10 @@ __global__ void __launch_bounds__(S_THREADS) attn_simple_kernel(const AttnParams
   if (n_parts > 1) join_parts<R, D, S_THREADS>(p, w, unit, n_parts, kvh, &s_flag);
 }
 
+}  // namespace
+#include "paged_attn_rows.cuh"
+namespace {
+
 // ---- how the work is dealt ----
 struct Plan { int tiles, tiles_per_seq, n_split, split_len; };
 
@@ -255,7 +259,21 @@ size_t workspace_of(const Plan& p, int n_kv, int rows, int dim, size_t* counters
   return p.n_split == 1 ? 0 : *counters + (size_t)p.tiles * n_kv * p.n_split * rows * (dim + 2) * 4;
 }
 
-Plan simple_plan(const b200q_paged_batch* b, int n_kv, int group) { return make_plan(b, n_kv, group, S_R, 4 * 148, 256); }
+// fp32 pages: the simple kernel
+Plan plan_of(const b200q_paged_cache* c, const b200q_paged_batch* b, int group) {
+  const int want = b->n_seqs > 1 ? 8 * 296 : 296;
+  return c->dtype == B200Q_F32 ? make_plan(b, c->n_kv_heads, group, S_R, 4 * 148, 256) : make_plan(b, c->n_kv_heads, group, 16, want, 128);
+}
+
+typedef void (*AttnKernel)(const AttnParams);
+template <int D>
+AttnKernel pick_simple() { return attn_simple_kernel<D, float>; }
+template <int D>
+AttnKernel pick_rows(int kv_dtype, int parts, int* smem) {
+  *smem = R_SMEM<D>;
+  if (kv_dtype == B200Q_F16) return parts == 1 ? attn_rows_kernel<D, 1, false> : attn_rows_kernel<D, 2, false>;
+  return parts == 1 ? attn_rows_kernel<D, 1, true> : attn_rows_kernel<D, 3, true>;
+}
 
 }  // namespace
 
@@ -269,12 +287,7 @@ int b200q_paged_attn_status_take(int* status) {
 extern "C" size_t b200q_paged_attention_workspace_bytes(const b200q_paged_cache* cache, const b200q_paged_batch* batch, int n_heads) {
   if (check_cache(cache) != B200Q_OK || check_batch(batch) != B200Q_OK || n_heads <= 0 || n_heads % cache->n_kv_heads || batch->n_seqs == 0 || batch->n_rows == 0) return 0;
   size_t c;
-  return workspace_of(simple_plan(batch, cache->n_kv_heads, n_heads / cache->n_kv_heads), cache->n_kv_heads, S_R, cache->head_dim, &c);
-}
-
-template <int D>
-static void (*pick_simple(int kv_dtype))(const AttnParams) {
-  return kv_dtype == B200Q_F32 ? attn_simple_kernel<D, float> : kv_dtype == B200Q_F16 ? attn_simple_kernel<D, __half> : attn_simple_kernel<D, __nv_bfloat16>;
+  return workspace_of(plan_of(cache, batch, n_heads / cache->n_kv_heads), cache->n_kv_heads, S_R, cache->head_dim, &c);
 }
 
 extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q_paged_batch* batch, const b200q_paged_attn_args* a, int flags, void* stream) {
@@ -288,7 +301,7 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
   if (batch->n_seqs == 0 || batch->n_rows == 0) return B200Q_OK;
   if (!a->q || !a->out) return B200Q_ERR_BAD_ARG;
   if ((uintptr_t)a->q % type_size(a->q_dtype) || (uintptr_t)a->out % type_size(a->out_dtype) || (uintptr_t)a->workspace & 255) return B200Q_ERR_MISALIGNED;
-  const Plan plan = simple_plan(batch, n_kv, group);
+  const Plan plan = plan_of(cache, batch, group);
   if (plan.n_split > 65535 || n_kv > 65535) return B200Q_ERR_TOO_LARGE;
   size_t counters;
   const size_t need = workspace_of(plan, n_kv, S_R, dim, &counters);
@@ -296,7 +309,23 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
   const AttnParams p{a->q, cache->k, cache->v, a->out, a->q_dtype, a->out_dtype, a->q_stride ? a->q_stride : row, a->out_stride ? a->out_stride : row, cache->page_stride,
                      cache->head_stride, cache->row_stride, a->n_heads, n_kv, group, (a->scale > 0.f ? a->scale : 1.f / sqrtf((float)dim)) * LOG2E, plan.tiles_per_seq, plan.n_split,
                      plan.split_len, (int*)a->workspace, (float*)((char*)a->workspace + counters), tables_of(cache, batch)};
-  auto kernel = dim == 16 ? pick_simple<16>(cache->dtype) : dim == 32 ? pick_simple<32>(cache->dtype) : dim == 64 ? pick_simple<64>(cache->dtype) : pick_simple<128>(cache->dtype);
-  B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles, n_kv, plan.n_split), dim3(S_THREADS), 0, (cudaStream_t)stream, (flags & B200Q_FLAG_PDL) != 0, p));
+  AttnKernel kernel;
+  int smem = 0, threads = S_THREADS;
+  if (cache->dtype == B200Q_F32) kernel = dim == 16 ? pick_simple<16>() : dim == 32 ? pick_simple<32>() : dim == 64 ? pick_simple<64>() : pick_simple<128>();
+  else {
+    const int parts = a->q_dtype == cache->dtype && a->out_dtype != B200Q_F32 ? 1 : 2;
+    threads = R_THREADS;
+    kernel = dim == 16 ? pick_rows<16>(cache->dtype, parts, &smem) : dim == 32 ? pick_rows<32>(cache->dtype, parts, &smem) : dim == 64 ? pick_rows<64>(cache->dtype, parts, &smem)
+                                                                                                                       : pick_rows<128>(cache->dtype, parts, &smem);
+    static PerDeviceFlag attr_set[2][2][4];
+    const int dev = b200q_current_device();
+    if (dev < 0) return B200Q_ERR_CUDA;
+    PerDeviceFlag& flag = attr_set[cache->dtype == B200Q_BF16][parts - 1][dim == 16 ? 0 : dim == 32 ? 1 : dim == 64 ? 2 : 3];
+    if (!flag.test(dev)) {
+      B200Q_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      flag.set(dev);
+    }
+  }
+  B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles, n_kv, plan.n_split), dim3(threads), (size_t)smem, (cudaStream_t)stream, (flags & B200Q_FLAG_PDL) != 0, p));
   return B200Q_OK;
 }
