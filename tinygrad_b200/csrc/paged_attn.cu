@@ -21,6 +21,7 @@ struct AttnParams {
   int n_heads, n_kv, group;
   float scale;               // times log2 e
   int tiles_per_seq;         // 0: tiles are counted sequence by sequence
+  int above, up_to;          // sequences with above < new tokens <= up_to (those with others are another kernel's)
   int n_split, split_len;
   int* counters;
   float* parts;
@@ -39,6 +40,7 @@ __device__ __forceinline__ TilePlace place_of_tile(const AttnParams& p, int tile
     const int b = min(max(t.row_off[s], 0), t.n_rows), e = min(max(t.row_off[s + 1], b), t.n_rows);
     return make_int2(b, e - b);
   };
+  auto ours = [&](int n) { n = min(n, t.max_new); return n > p.above && n <= p.up_to ? n : 0; };
   if (p.tiles_per_seq) {
     w.seq = tile / p.tiles_per_seq;
     w.r0 = (tile - w.seq * p.tiles_per_seq) * R;
@@ -47,7 +49,7 @@ __device__ __forceinline__ TilePlace place_of_tile(const AttnParams& p, int tile
     bool found = false;
     for (int s0 = 0; s0 < t.n_seqs && !found; s0 += 32) {
       int mine = 0;
-      if (s0 + lane < t.n_seqs) mine = (int)(((int64_t)min(rows(s0 + lane).y, t.max_new) * p.group + R - 1) / R);
+      if (s0 + lane < t.n_seqs) mine = (int)(((int64_t)ours(rows(s0 + lane).y) * p.group + R - 1) / R);
       int sum = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += u; }
@@ -66,7 +68,7 @@ __device__ __forceinline__ TilePlace place_of_tile(const AttnParams& p, int tile
   const int2 r = rows(w.seq);
   w.first_row = r.x;
   w.length = t.length[w.seq];
-  const int n = min(r.y, t.max_new);
+  const int n = ours(r.y);
   if (w.r0 >= (int64_t)n * p.group) return w;
   w.n = n;
   const int64_t cap = min((int64_t)min(w.length, t.max_len), (int64_t)t.table_stride * t.page_size);
@@ -234,45 +236,87 @@ __global__ void __launch_bounds__(S_THREADS) attn_simple_kernel(const AttnParams
 
 }  // namespace
 #include "paged_attn_rows.cuh"
+#include "paged_attn_tiles.cuh"
 namespace {
 
 // ---- how the work is dealt ----
-struct Plan { int tiles, tiles_per_seq, n_split, split_len; };
+struct Plan { int tiles, tiles_per_seq, n_split, split_len, above, up_to, rows; size_t at, counters, bytes; };      // at, counters, bytes: in the workspace
 
 // Tiles of `rows` pairs: those of all sequences at their largest, or (ragged batches, if that is less) the pairs' tiles and a broken one for each sequence.  Keys are split until
 // there are about `want` CTAs, in parts of at least `least` keys.
-Plan make_plan(const b200q_paged_batch* b, int n_kv, int group, int rows, int want, int least) {
-  const int64_t per = ((int64_t)b->max_new * group + rows - 1) / rows, even = per * b->n_seqs, ragged = (int64_t)b->n_rows * group / rows + b->n_seqs;
+Plan make_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group, int above, int up_to, int rows, int want, int least, int unit) {
+  const int n_kv = c->n_kv_heads, most_new = b->max_new < up_to ? b->max_new : up_to;
+  const int64_t per = ((int64_t)most_new * group + rows - 1) / rows, even = per * b->n_seqs, ragged = (int64_t)b->n_rows * group / rows + b->n_seqs;
   Plan p{};
+  p.above = above; p.up_to = up_to;
   p.tiles_per_seq = even <= ragged ? (int)per : 0;
   p.tiles = (int)(even <= ragged ? even : ragged);
   const int64_t len = b->max_len > 0 ? b->max_len : 1, most = (len + least - 1) / least;
   const int64_t parts = want / ((int64_t)p.tiles * n_kv);
   const int64_t n = parts < 1 ? 1 : parts < most ? parts : most;
-  p.split_len = (int)((len + n - 1) / n + 31) / 32 * 32;
+  p.split_len = (int)(((len + n - 1) / n + unit - 1) / unit * unit);
   p.n_split = (int)((len + p.split_len - 1) / p.split_len);
+  p.bytes = p.n_split == 1 ? 0 : ((size_t)p.tiles * n_kv * p.n_split * rows * (c->head_dim + 2) * 4 + 255) / 256 * 256;
   return p;
 }
 
-size_t workspace_of(const Plan& p, int n_kv, int rows, int dim, size_t* counters) {
-  *counters = ((size_t)p.tiles * n_kv * 4 + 255) / 256 * 256;
-  return p.n_split == 1 ? 0 : *counters + (size_t)p.tiles * n_kv * p.n_split * rows * (dim + 2) * 4;
-}
+// The workspace begins with the counters of the tiles that are split, MAX_UNITS for each kernel of a call: a fixed place, whatever calls share the workspace.  Tiles x KV heads are split only
+// where they are at most half of the CTAs that are wanted.
+constexpr int MAX_UNITS = 2048, MOST_CTAS = 8 * 296;
+constexpr size_t COUNTERS_BYTES = 2 * MAX_UNITS * sizeof(int);
+static_assert(MOST_CTAS / 2 <= MAX_UNITS, "counters");
 
-// fp32 pages: the simple kernel
-Plan plan_of(const b200q_paged_cache* c, const b200q_paged_batch* b, int group) {
-  const int want = b->n_seqs > 1 ? 8 * 296 : 296;
-  return c->dtype == B200Q_F32 ? make_plan(b, c->n_kv_heads, group, S_R, 4 * 148, 256) : make_plan(b, c->n_kv_heads, group, 16, want, 128);
+constexpr int FEW_PAIRS = 32;      // (token, head) pairs of a sequence that the rows kernel takes
+// The kernels of a call and their shares of it.  many: sequences of more than FEW_PAIRS pairs go to the tiles kernel.
+struct Deal { bool many; int n; Plan plan[2]; size_t bytes; };
+Deal deal_of(const b200q_paged_cache* c, const b200q_paged_batch* b, int group, bool tiles_take) {
+  Deal d{};
+  const int few = FEW_PAIRS / group > 1 ? FEW_PAIRS / group : 1;
+  d.many = tiles_take && b->max_new > few;
+  if (d.many) {
+    d.plan[0] = make_plan(c, b, group, few, INT32_MAX, T_R, 148, 512, T_KEYS);
+    d.n = 1;
+    if (b->n_seqs > 1) {
+      d.plan[1] = make_plan(c, b, group, 0, few, 16, MOST_CTAS, 128, 32);
+      d.n = 2;
+    } else d.plan[0].above = 0;
+  } else {
+    d.plan[0] = c->dtype == B200Q_F32 ? make_plan(c, b, group, 0, INT32_MAX, S_R, 4 * 148, 256, 32) : make_plan(c, b, group, 0, INT32_MAX, 16, b->n_seqs > 1 ? MOST_CTAS : 296, 128, 32);
+    d.n = 1;
+  }
+  const size_t parts = d.plan[0].bytes + d.plan[1].bytes;
+  d.bytes = parts ? COUNTERS_BYTES + parts : 0;
+  return d;
 }
+// The tiles kernel: 16-bit pages of whole boxes
+bool pages_for_tiles(const b200q_paged_cache* c) {
+  return c->dtype != B200Q_F32 && (c->head_dim == 64 || c->head_dim == 128) && c->page_size >= 8 && (c->page_size & (c->page_size - 1)) == 0 &&
+         c->page_stride < (1LL << 38) && c->head_stride < (1LL << 38) && c->row_stride < (1LL << 38);
+}
+int box_rows_of(const b200q_paged_cache* c) { return c->page_size < T_KEYS ? c->page_size : T_KEYS; }
 
 typedef void (*AttnKernel)(const AttnParams);
+typedef void (*TilesKernel)(const AttnParams, const CUtensorMap, const CUtensorMap, int);
 template <int D>
-AttnKernel pick_simple() { return attn_simple_kernel<D, float>; }
-template <int D>
-AttnKernel pick_rows(int kv_dtype, int parts, int* smem) {
-  *smem = R_SMEM<D>;
+AttnKernel pick_rows(int kv_dtype, int parts) {
+  if (kv_dtype == B200Q_F32) return attn_simple_kernel<D, float>;
   if (kv_dtype == B200Q_F16) return parts == 1 ? attn_rows_kernel<D, 1, false> : attn_rows_kernel<D, 2, false>;
   return parts == 1 ? attn_rows_kernel<D, 1, true> : attn_rows_kernel<D, 3, true>;
+}
+template <int D>
+TilesKernel pick_tiles(int kv_dtype, int parts, int* smem) {
+  *smem = parts == 1 ? T_SMEM<D, 1> : T_SMEM<D, 2>;
+  if (kv_dtype == B200Q_F16) return parts == 1 ? attn_tiles_kernel<D, 1, false> : attn_tiles_kernel<D, 2, false>;
+  return attn_tiles_kernel<D, 1, true>;
+}
+template <typename K>
+int allow_smem(K kernel, int smem, PerDeviceFlag& flag) {
+  const int dev = b200q_current_device();
+  if (dev < 0) return B200Q_ERR_CUDA;
+  if (flag.test(dev)) return B200Q_OK;
+  B200Q_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  flag.set(dev);
+  return B200Q_OK;
 }
 
 }  // namespace
@@ -286,8 +330,9 @@ int b200q_paged_attn_status_take(int* status) {
 
 extern "C" size_t b200q_paged_attention_workspace_bytes(const b200q_paged_cache* cache, const b200q_paged_batch* batch, int n_heads) {
   if (check_cache(cache) != B200Q_OK || check_batch(batch) != B200Q_OK || n_heads <= 0 || n_heads % cache->n_kv_heads || batch->n_seqs == 0 || batch->n_rows == 0) return 0;
-  size_t c;
-  return workspace_of(plan_of(cache, batch, n_heads / cache->n_kv_heads), cache->n_kv_heads, S_R, cache->head_dim, &c);
+  const int group = n_heads / cache->n_kv_heads;
+  const size_t a = deal_of(cache, batch, group, false).bytes, b = pages_for_tiles(cache) ? deal_of(cache, batch, group, true).bytes : 0;
+  return a > b ? a : b;
 }
 
 extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q_paged_batch* batch, const b200q_paged_attn_args* a, int flags, void* stream) {
@@ -301,31 +346,45 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
   if (batch->n_seqs == 0 || batch->n_rows == 0) return B200Q_OK;
   if (!a->q || !a->out) return B200Q_ERR_BAD_ARG;
   if ((uintptr_t)a->q % type_size(a->q_dtype) || (uintptr_t)a->out % type_size(a->out_dtype) || (uintptr_t)a->workspace & 255) return B200Q_ERR_MISALIGNED;
-  const Plan plan = plan_of(cache, batch, group);
-  if (plan.n_split > 65535 || n_kv > 65535) return B200Q_ERR_TOO_LARGE;
-  size_t counters;
-  const size_t need = workspace_of(plan, n_kv, S_R, dim, &counters);
-  if (need && (!a->workspace || a->workspace_bytes < need)) return B200Q_ERR_TOO_LARGE;
-  const AttnParams p{a->q, cache->k, cache->v, a->out, a->q_dtype, a->out_dtype, a->q_stride ? a->q_stride : row, a->out_stride ? a->out_stride : row, cache->page_stride,
-                     cache->head_stride, cache->row_stride, a->n_heads, n_kv, group, (a->scale > 0.f ? a->scale : 1.f / sqrtf((float)dim)) * LOG2E, plan.tiles_per_seq, plan.n_split,
-                     plan.split_len, (int*)a->workspace, (float*)((char*)a->workspace + counters), tables_of(cache, batch)};
-  AttnKernel kernel;
-  int smem = 0, threads = S_THREADS;
-  if (cache->dtype == B200Q_F32) kernel = dim == 16 ? pick_simple<16>() : dim == 32 ? pick_simple<32>() : dim == 64 ? pick_simple<64>() : pick_simple<128>();
-  else {
-    const int parts = a->q_dtype == cache->dtype && a->out_dtype != B200Q_F32 ? 1 : 2;
-    threads = R_THREADS;
-    kernel = dim == 16 ? pick_rows<16>(cache->dtype, parts, &smem) : dim == 32 ? pick_rows<32>(cache->dtype, parts, &smem) : dim == 64 ? pick_rows<64>(cache->dtype, parts, &smem)
-                                                                                                                       : pick_rows<128>(cache->dtype, parts, &smem);
-    static PerDeviceFlag attr_set[2][2][4];
-    const int dev = b200q_current_device();
-    if (dev < 0) return B200Q_ERR_CUDA;
-    PerDeviceFlag& flag = attr_set[cache->dtype == B200Q_BF16][parts - 1][dim == 16 ? 0 : dim == 32 ? 1 : dim == 64 ? 2 : 3];
-    if (!flag.test(dev)) {
-      B200Q_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-      flag.set(dev);
-    }
+  // one part of 16 bits where queries, keys and outputs have 16; two (bf16 keys: three, which the rows kernel has) where something is wider
+  const int parts = a->q_dtype == cache->dtype && a->out_dtype != B200Q_F32 ? 1 : 2;
+  alignas(64) CUtensorMap tm_k, tm_v;
+  bool tiles_take = pages_for_tiles(cache) && (parts == 1 || cache->dtype == B200Q_F16);
+  Deal deal = deal_of(cache, batch, group, tiles_take);
+  if (deal.many) {
+    memset(&tm_k, 0, sizeof(tm_k)); memset(&tm_v, 0, sizeof(tm_v));
+    rc = make_page_map(&tm_k, cache, cache->k, box_rows_of(cache));
+    if (rc == B200Q_OK) rc = make_page_map(&tm_v, cache, cache->v, box_rows_of(cache));
+    if (rc == B200Q_ERR_UNSUPPORTED) deal = deal_of(cache, batch, group, false);      // strides that no map can have
+    else if (rc != B200Q_OK) return rc;
   }
-  B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles, n_kv, plan.n_split), dim3(threads), (size_t)smem, (cudaStream_t)stream, (flags & B200Q_FLAG_PDL) != 0, p));
+  if (deal.bytes && (!a->workspace || a->workspace_bytes < deal.bytes)) return B200Q_ERR_TOO_LARGE;
+  for (int i = 0; i < deal.n; i++)
+    if (deal.plan[i].n_split > 65535 || n_kv > 65535 || (int64_t)deal.plan[i].tiles * n_kv > INT32_MAX) return B200Q_ERR_TOO_LARGE;
+  const cudaStream_t st = (cudaStream_t)stream;
+  for (int i = 0; i < deal.n; i++) {
+    const Plan& plan = deal.plan[i];
+    int* const counters = (int*)a->workspace + i * MAX_UNITS;
+    float* const parts_at = (float*)((char*)a->workspace + COUNTERS_BYTES + (i ? deal.plan[0].bytes : 0));
+    const AttnParams p{a->q, cache->k, cache->v, a->out, a->q_dtype, a->out_dtype, a->q_stride ? a->q_stride : row, a->out_stride ? a->out_stride : row, cache->page_stride,
+                       cache->head_stride, cache->row_stride, a->n_heads, n_kv, group, (a->scale > 0.f ? a->scale : 1.f / sqrtf((float)dim)) * LOG2E, plan.tiles_per_seq, plan.above, plan.up_to,
+                       plan.n_split, plan.split_len, counters, parts_at, tables_of(cache, batch)};
+    const bool pdl = i == 0 && (flags & B200Q_FLAG_PDL);
+    const int type = cache->dtype == B200Q_BF16;
+    if (deal.many && i == 0) {
+      int smem;
+      const TilesKernel kernel = dim == 64 ? pick_tiles<64>(cache->dtype, parts, &smem) : pick_tiles<128>(cache->dtype, parts, &smem);
+      static PerDeviceFlag allowed[2][2][2];
+      if ((rc = allow_smem(kernel, smem, allowed[type][parts - 1][dim == 128])) != B200Q_OK) return rc;
+      B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles * n_kv, plan.n_split), dim3(T_THREADS), (size_t)smem, st, pdl, p, tm_k, tm_v, box_rows_of(cache)));
+      continue;
+    }
+    const int d = dim == 16 ? 0 : dim == 32 ? 1 : dim == 64 ? 2 : 3;
+    const AttnKernel kernel = d == 0 ? pick_rows<16>(cache->dtype, parts) : d == 1 ? pick_rows<32>(cache->dtype, parts) : d == 2 ? pick_rows<64>(cache->dtype, parts) : pick_rows<128>(cache->dtype, parts);
+    const int smem = cache->dtype == B200Q_F32 ? 0 : d == 0 ? R_SMEM<16> : d == 1 ? R_SMEM<32> : d == 2 ? R_SMEM<64> : R_SMEM<128>;
+    static PerDeviceFlag allowed[2][2][4];
+    if (smem && (rc = allow_smem(kernel, smem, allowed[type][parts - 1][d])) != B200Q_OK) return rc;
+    B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles, n_kv, plan.n_split), dim3(smem ? R_THREADS : S_THREADS), (size_t)smem, st, pdl, p));
+  }
   return B200Q_OK;
 }

@@ -1,0 +1,548 @@
+// Attention over pages for many rows (prompts and chunks): paged_attn.cu includes this.
+//
+// Bound by the tensor core and, as much, by the exponentials: 256 rows x 128 keys are 2 x 256 x 128 x D multiply-adds (2048 cycles of the tensor core at D = 128) and 32768 powers (2048
+// cycles of the special-function units).  So a CTA has two tiles of 128 rows whose products and softmaxes take turns: while one's scores are turned into probabilities, the other's
+// products run.  Warps 0-3 and 4-7 are the tiles' softmax, a thread a row (scores are read from tensor memory as it holds them, no exchange between threads); one
+// thread issues the products, S = Q K^T from shared memory and O += P V with P from tensor memory, where it takes the place of the scores; one warp brings keys and values (TMA boxes of a page's
+// rows, 128-byte swizzle), two look after the values that a product must not see.  Tensor memory: S0 S1 O0 O1, 128 columns each.
+//
+// The running maximum moves only when it has grown by 2^8: until then probabilities are relative to an older one, which the quotient does not notice, and the weighted sums
+// in tensor memory stay as they are.
+//
+// Precision: N = 1, 16-bit queries and outputs: a probability loses half a step, as the output does.  N = 2, fp32 rows on fp16 keys: queries (under a power of two that keeps the row in range) and
+// probabilities are two halves each, and a tile's weighted sum starts from zero and is added in registers, because the tensor core cuts its sums where others round.
+#pragma once
+#include <cuda.h>
+#include <string.h>
+
+namespace {
+
+constexpr int T_ROWS = 128, T_R = 2 * T_ROWS, T_KEYS = 128, T_THREADS = 384, T_BASE = 7;      // probabilities up to 2^(7 + 8)
+template <int D> constexpr int T_TILE = T_KEYS * D * 2;                                     // bytes of 128 rows of 16-bit values
+template <int D, int N> constexpr int T_KS = D == 64 ? 3 : N == 1 ? 2 : 1;
+template <int D, int N> constexpr int T_VS = D == 64 ? 3 : N == 1 ? 3 : 2;
+template <int D, int N> constexpr int T_SMEM = (2 * N + T_KS<D, N> + T_VS<D, N>) * T_TILE<D> + 1024;
+
+struct SharedA {
+  uint64_t k_full[3], k_empty[3], v_full[3], v_clean[3], v_empty[3], s_full[2], p_full[2], q_full, o_full;
+  uint32_t tmem;
+  int abort, flag, bad_lo, bad_hi;
+};
+
+__device__ __forceinline__ uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void a_bar_init(uint64_t* b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s_addr(b)), "r"(n) : "memory"); }
+__device__ __forceinline__ void a_bar_arrive(uint64_t* b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s_addr(b)) : "memory"); }
+// Bounded wait: false once another role has given up, or when the time is over (then the others are told).
+__device__ __forceinline__ bool a_wait_on(uint32_t bar, uint32_t parity, uint32_t abort) {
+  for (int i = 0; i < (1 << 20); i++) {
+    uint32_t ok, gone;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity), "r"(2000) : "memory");
+    if (ok) return true;
+    asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(gone) : "r"(abort) : "memory");
+    if (gone) return false;
+  }
+  asm volatile("st.volatile.shared::cta.u32 [%0], 1;" ::"r"(abort) : "memory");
+  atomicExch(&g_paged_attn_status, 1);
+  return false;
+}
+__device__ __forceinline__ bool a_wait(SharedA& sh, uint64_t* b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(s_addr(b)), "r"(parity) : "memory");
+  return ok || a_wait_on(s_addr(b), parity, s_addr(&sh.abort));
+}
+__device__ __forceinline__ void a_commit(uint64_t* b) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s_addr(b)) : "memory"); }
+
+// Operands in the 128-byte-swizzle layout: sub-tiles of 64 values (128 bytes) a row, 8 rows = 1024 bytes.  Q and K are read along a row (rows 1024 bytes per 8 apart); V, whose reduction runs over
+// its rows, across them: then the distance between sub-tiles stands in the other field.
+__device__ __forceinline__ uint64_t desc_128(uint32_t addr, uint32_t other) {
+  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(other >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+template <bool BF, bool ACROSS> __host__ __device__ constexpr uint32_t idesc_of(int n) {
+  return 1u << 4 | (BF ? 1u << 7 | 1u << 10 : 0u) | (ACROSS ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(T_ROWS >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss_a(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void ld32(uint32_t a, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+                 "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
+                 "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31]) : "r"(a));
+}
+__device__ __forceinline__ void st32(uint32_t a, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+               ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+                 "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
+                 "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t a, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+               ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
+                 "r"(v[15]) : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ float pow2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ void st_s4(uint32_t a, uint4 v) { asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); }
+__device__ __forceinline__ uint4 ld_s4(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+// 64 values from element i on, as fp32 (all loads before the first use)
+__device__ __forceinline__ void load64(const void* base, int type, int64_t i, bool wide, float (&f)[64]) {
+  if (wide && type == B200Q_F32) {
+    float4 x[16];
+#pragma unroll
+    for (int c = 0; c < 16; c++) x[c] = reinterpret_cast<const float4*>(static_cast<const float*>(base) + i)[c];
+#pragma unroll
+    for (int c = 0; c < 16; c++) { f[c * 4] = x[c].x; f[c * 4 + 1] = x[c].y; f[c * 4 + 2] = x[c].z; f[c * 4 + 3] = x[c].w; }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 64; c++) f[c] = load_as_f(base, type, i + c);
+  }
+}
+
+struct RowOf { int64_t row, head; int last; bool live; };      // of a thread: its row of the arrays, its head, the position it sees up to
+
+// What rows that see keys [lo, hi] with values that are not finite get of them (their finite values are in the products already).
+template <int D, bool BF>
+__device__ __forceinline__ void add_not_finite(const AttnParams& p, int seq, int kvh, int lo, int hi, int d0, float* o) {
+  for (int key = lo; key <= hi; key++) {
+    const int64_t at = key_at(p, seq, key);
+    if (at < 0) continue;
+    const uint16_t* v = static_cast<const uint16_t*>(p.v) + kvh * p.head_stride + at + d0;
+    for (int d = 0; d < 32; d++) {
+      const uint32_t x = v[d];
+      if (finite_only<BF>(x) != x) o[d] += unpack2(x, BF).x;
+    }
+  }
+}
+
+template <int D, int N, bool BF>
+__global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, int box_rows) {
+  constexpr int SUBS = D / 64, TILE = T_TILE<D>, SUB = T_KEYS * 128, KS = T_KS<D, N>, VS = T_VS<D, N>, KK = D / 16;
+  extern __shared__ unsigned char raw[];
+  __shared__ SharedA sh;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int order = blockIdx.x / p.n_kv, kvh = blockIdx.x - order * p.n_kv, split = blockIdx.y;
+  const int tile_index = gridDim.x / p.n_kv - 1 - order;      // long ones first
+  const TilePlace w = place_of_tile<T_R>(p, tile_index);
+  if (w.n == 0) return;
+  const int n_parts = max(1, (w.keys + p.split_len - 1) / p.split_len), k_begin = split * p.split_len, k_end = min(w.keys, k_begin + p.split_len);
+  if (split >= n_parts) return;
+  const int tiles = max(0, (k_end - k_begin + T_KEYS - 1) / T_KEYS);
+  const int64_t pairs = (int64_t)w.n * p.group;
+  const bool two = w.r0 + T_ROWS < pairs;                      // the second tile of rows has some
+  const int first_last = w.length + w.r0 / p.group;            // what the first row sees
+  const uint32_t s_q = (s_addr(raw) + 1023) & ~1023u, s_k = s_q + 2 * N * TILE, s_v = s_k + KS * TILE;
+
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_addr(&sh.tmem)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (tid == 0) {
+    for (int i = 0; i < 3; i++) {
+      a_bar_init(&sh.k_full[i], 1); a_bar_init(&sh.k_empty[i], 1); a_bar_init(&sh.v_full[i], 1); a_bar_init(&sh.v_clean[i], 2); a_bar_init(&sh.v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; i++) { a_bar_init(&sh.s_full[i], 1); a_bar_init(&sh.p_full[i], 4); }
+    a_bar_init(&sh.q_full, 8); a_bar_init(&sh.o_full, 1);
+    sh.abort = sh.flag = 0; sh.bad_lo = INT32_MAX; sh.bad_hi = -1;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async();
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = sh.tmem;
+  const int unit = tile_index * p.n_kv + kvh;
+
+  // registers: 384 threads x 168 = 64512 at launch = 256 x 208 + 128 x 88
+  if (warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    // ---- softmax: a thread a row ----
+    const int t = warp >> 2, r = tid & 127;
+    RowOf me;
+    {
+      const int64_t pair = w.r0 + t * T_ROWS + r;
+      me.live = pair < pairs;
+      const int token = me.live ? (int)(pair / p.group) : 0;
+      me.row = w.first_row + token;
+      me.head = kvh * p.group + (me.live ? pair - (int64_t)token * p.group : 0);
+      me.last = me.live ? w.length + token : -1;
+    }
+    float qs = p.scale;
+    if (t == 0 || two) {
+      // its row of queries: N parts, chunks of 16 bytes in the swizzled places
+      const int64_t at = me.row * p.q_stride + me.head * D;
+      const uint32_t to = s_q + t * TILE + r * 128;
+      const int size = type_size(p.q_dtype);
+      const bool wide = (((uintptr_t)p.q | (uintptr_t)(p.q_stride * size)) & 15) == 0;
+      float up = 1.f;
+      if constexpr (N == 2) {
+        float amax = 0.f, down;
+#pragma unroll 1
+        for (int b = 0; me.live && b < D; b += 64) {
+          float f[64];
+          load64(p.q, p.q_dtype, at + b, wide, f);
+#pragma unroll
+          for (int i = 0; i < 64; i++) amax = fmaxf(amax, fabsf(f[i]));
+        }
+        pow2_scale(amax, up, down);
+        if (amax > 0.f) qs *= down;
+      }
+      qs = fmaxf(qs, 1.1754944e-38f);
+#pragma unroll 1
+      for (int b = 0; b < D; b += 64) {
+        uint4 v[N][8];
+        if (N == 1 && wide && me.live) {
+#pragma unroll
+          for (int c = 0; c < 8; c++) v[0][c] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at + b + c * 8);
+        } else {
+          float f[64];
+          if (me.live) load64(p.q, p.q_dtype, at + b, wide, f);
+#pragma unroll
+          for (int c = 0; c < 8; c++) {
+            uint32_t x[4][N];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const int i = c * 8 + j * 2;
+              parts_of<N, BF>(me.live ? f[i] * up : 0.f, me.live ? f[i + 1] * up : 0.f, x[j]);
+            }
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i][c] = make_uint4(x[0][i], x[1][i], x[2][i], x[3][i]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++)
+#pragma unroll
+          for (int c = 0; c < 8; c++) st_s4(to + i * 2 * TILE + (b / 64) * SUB + ((c ^ (r & 7)) << 4), v[i][c]);
+      }
+    }
+    fence_async();
+    __syncwarp();
+    if (lane == 0) a_bar_arrive(&sh.q_full);
+    float m = -INFINITY, l = 0.f;
+    [[maybe_unused]] float acc[N == 2 ? D : 1];
+    if constexpr (N == 2) {
+#pragma unroll
+      for (int d = 0; d < D; d++) acc[d] = 0.f;
+    }
+    const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * 128, to = ts + 256;
+    const int warp_first = __shfl_sync(0xffffffffu, me.last, 0);      // no row of the warp sees less (rows without a token see nothing, and are not stored)
+    bool ok = t == 0 || two;
+    float scaled = 1.f;      // N == 2: what the sum in registers is multiplied by before a tile's is added
+#pragma unroll 1
+    for (int j = 0; ok && j < tiles; j++) {
+      const int k0 = k_begin + j * T_KEYS;
+      ok = __all_sync(0xffffffffu, a_wait(sh, &sh.s_full[t], j & 1));
+      if (!ok) break;
+      fence_after();
+      const bool masked = k0 + T_KEYS - 1 > warp_first || k0 + T_KEYS > k_end;
+      const int lim = min(me.last, k_end - 1) - k0;
+      float top = -INFINITY;
+      if constexpr (N == 1) {
+        uint32_t s[128];
+#pragma unroll
+        for (int c = 0; c < 4; c++) ld32(ts + c * 32, s + c * 32);
+        wait_ld();
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 128; i++) s[i] = i <= lim ? s[i] : __float_as_uint(-INFINITY);
+        }
+        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 128; i++) tops[i & 3] = fmaxf(tops[i & 3], __uint_as_float(s[i]));
+        top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * qs;
+        const bool moves = j == 0 || top > m + 8.f;
+        if (__any_sync(0xffffffffu, moves)) {
+          const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : pow2(m - mn);
+          m = mn;
+          if (j > 0) {
+            l *= f;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; c++) {
+              uint32_t o[32];
+              ld32(to + c * 32, o);
+              wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              st32(to + c * 32, o);
+            }
+          }
+        }
+        const float sub = m == -INFINITY ? 0.f : T_BASE - m;
+        float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const float a = pow2(fmaf(__uint_as_float(s[c * 32 + 2 * i]), qs, sub)), b = pow2(fmaf(__uint_as_float(s[c * 32 + 2 * i + 1]), qs, sub));
+            sums[i & 3] += a + b;
+            pk[i] = pack2(a, b, BF ? B200Q_BF16 : B200Q_F16);
+          }
+          st16(ts + c * 32, pk);
+        }
+        l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+      } else {
+        // the tile before: its weighted sum is complete (the scores behind it in the tensor core's queue are)
+        if (j > 0) {
+#pragma unroll
+          for (int c = 0; c < D / 32; c++) {
+            uint32_t o[32];
+            ld32(to + c * 32, o);
+            wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; i++) acc[c * 32 + i] = fmaf(acc[c * 32 + i], scaled, __uint_as_float(o[i]));
+          }
+        }
+#pragma unroll 1
+        for (int c = 0; c < 4; c++) {
+          uint32_t s[32];
+          ld32(ts + c * 32, s);
+          wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; i++) top = fmaxf(top, masked && c * 32 + i > lim ? -INFINITY : __uint_as_float(s[i]));
+        }
+        top *= qs;
+        const float mn = fmaxf(m, top);
+        scaled = mn == -INFINITY ? 1.f : pow2(m - mn);
+        m = mn;
+        l *= scaled;
+        const float sub = m == -INFINITY ? 0.f : T_BASE + 7 - m;
+        float sum = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < 4; c++) {
+          uint32_t s[32], pk[32];
+          ld32(ts + c * 32, s);
+          wait_ld();
+          if (masked) {
+#pragma unroll
+            for (int i = 0; i < 32; i++) s[i] = c * 32 + i <= lim ? s[i] : __float_as_uint(-INFINITY);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const float a = pow2(fmaf(__uint_as_float(s[2 * i]), qs, sub)), b = pow2(fmaf(__uint_as_float(s[2 * i + 1]), qs, sub));
+            sum += a + b;
+            uint32_t x[N];
+            parts_of<N, BF>(a, b, x);
+#pragma unroll
+            for (int q = 0; q < N; q++) pk[q * 16 + i] = x[q];
+          }
+          st32(ts + c * 32, pk);
+        }
+        l += sum;
+      }
+      wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) a_bar_arrive(&sh.p_full[t]);
+    }
+    if (ok && tiles) ok = __all_sync(0xffffffffu, a_wait(sh, &sh.o_full, 0));
+    // ---- what comes out ----
+    if (ok) {
+      fence_after();
+      const int bad_lo = *(volatile int*)&sh.bad_lo, bad_hi = min(*(volatile int*)&sh.bad_hi, me.last);
+      float* part = p.parts + ((int64_t)unit * p.n_split + split) * PART<T_R, D>;
+      const int pr = t * T_ROWS + r;
+      if (n_parts > 1 && me.live) { __stcg(part + pr, m); __stcg(part + T_R + pr, l); }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int64_t at = me.row * p.out_stride + me.head * D;
+      const bool wide = (((uintptr_t)p.out | (uintptr_t)(p.out_stride * (p.out_dtype == B200Q_F32 ? 4 : 2))) & 15) == 0;
+#pragma unroll
+      for (int c = 0; c < D / 32; c++) {
+        uint32_t x[32];
+        float o[32];
+        if (tiles) { ld32(to + c * 32, x); wait_ld(); }
+#pragma unroll
+        for (int i = 0; i < 32; i++) {
+          const float f = tiles ? __uint_as_float(x[i]) : 0.f;
+          if constexpr (N == 2) o[i] = fmaf(acc[c * 32 + i], scaled, f);
+          else o[i] = f;
+        }
+        if (bad_lo <= bad_hi && me.live) {
+          float y[32];
+#pragma unroll
+          for (int i = 0; i < 32; i++) y[i] = o[i];
+          add_not_finite<D, BF>(p, w.seq, kvh, bad_lo, bad_hi, c * 32, y);
+#pragma unroll
+          for (int i = 0; i < 32; i++) o[i] = y[i];
+        }
+        if (!me.live) continue;
+        if (n_parts > 1) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) __stcg(reinterpret_cast<float4*>(part + 2 * T_R + pr * D + c * 32 + i), make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
+          continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i++) o[i] = l == 0.f ? 0.f : o[i] * inv;
+        if (!wide) {
+#pragma unroll
+          for (int i = 0; i < 32; i++) store_as(p.out, p.out_dtype, at + c * 32 + i, o[i]);
+        } else if (p.out_dtype == B200Q_F32) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at + c * 32 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint32_t y[4];
+#pragma unroll
+            for (int q = 0; q < 4; q++) y[q] = pack2(o[i + 2 * q], o[i + 2 * q + 1], p.out_dtype);
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at + c * 32 + i) = make_uint4(y[0], y[1], y[2], y[3]);
+          }
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 8) {
+    // ---- products ----
+    if (elect_one()) {
+      constexpr uint32_t ID_S = idesc_of<BF, false>(T_KEYS), ID_O = idesc_of<BF, true>(D);
+      auto scores = [&](int t, int ks) {
+#pragma unroll
+        for (int i = N - 1; i >= 0; i--)
+#pragma unroll
+          for (int kk = 0; kk < KK; kk++) {
+            const uint32_t o = (kk / 4) * SUB + (kk % 4) * 32;
+            mma_ss_a(tmem + t * 128, desc_128(s_q + (i * 2 + t) * TILE + o, 16), desc_128(s_k + ks * TILE + o, 16), ID_S, i < N - 1 || kk > 0);
+          }
+        a_commit(&sh.s_full[t]);
+      };
+      bool ok = tiles > 0 && a_wait(sh, &sh.q_full, 0) && a_wait(sh, &sh.k_full[0], 0);
+      if (ok) {
+        fence_after();
+        scores(0, 0);
+        if (two) scores(1, 0);
+        a_commit(&sh.k_empty[0]);
+      }
+      for (int j = 0; ok && j < tiles; j++) {
+        const int vs = j % VS, kn = (j + 1) % KS;
+        ok = a_wait(sh, &sh.v_clean[vs], (j / VS) & 1);
+        for (int t = 0; ok && t < 1 + two; t++) {
+          ok = a_wait(sh, &sh.p_full[t], j & 1);
+          if (!ok) break;
+          fence_after();
+#pragma unroll
+          for (int i = N - 1; i >= 0; i--)
+#pragma unroll
+            for (int kk = 0; kk < T_KEYS / 16; kk++)
+              mma_ts_a(tmem + 256 + t * 128, tmem + t * 128 + (kk / 2) * 32 + i * 16 + (kk & 1) * 8, desc_128(s_v + vs * TILE + kk * 2048, SUB), ID_O,
+                       i < N - 1 || kk > 0 || (N == 1 && j > 0));
+          if (t == two) a_commit(&sh.v_empty[vs]);
+          if (j + 1 < tiles) {
+            if (t == 0) { ok = a_wait(sh, &sh.k_full[kn], ((j + 1) / KS) & 1); if (!ok) break; fence_after(); }
+            scores(t, kn);
+            if (t == two) a_commit(&sh.k_empty[kn]);
+          }
+        }
+      }
+      a_commit(&sh.o_full);
+      if (!ok) a_wait_on(s_addr(&sh.o_full), 0, s_addr(&sh.flag));      // products in flight are done before tensor memory goes back (flag is 0 here)
+    }
+  } else if (warp == 9) {
+    // ---- keys and values: a lane a box ----
+    const int per_tile = T_KEYS / box_rows, ps = p.t.page_size, sub = lane % SUBS, pg = lane / SUBS;
+    const int32_t* row_pages = p.t.pages + (int64_t)w.seq * p.t.table_stride;
+    bool ok = true;
+    int issued[2] = {0, 0};
+    for (int j = 0; ok && j < tiles; j++) {
+      const int k0 = k_begin + j * T_KEYS, n_pages = min(per_tile, (k_end - k0 + box_rows - 1) / box_rows);
+      const bool mine = pg < n_pages;
+      int page = 0;
+      if (mine) {
+        page = row_pages[(k0 + pg * box_rows) / ps];
+        if (page < 0 || page >= p.t.n_pages) { page = p.t.n_pages; atomicExch(&g_paged_attn_status, 2); }      // (outside the map: the box is filled with zeros)
+      }
+      const int slot = (k0 + pg * box_rows) % ps;
+#pragma unroll
+      for (int v = 0; v < 2; v++) {
+        const int st = v ? j % VS : j % KS, use = v ? j / VS : j / KS;
+        uint64_t* full = v ? &sh.v_full[st] : &sh.k_full[st];
+        if (use > 0) ok = ok && a_wait(sh, v ? &sh.v_empty[st] : &sh.k_empty[st], (use - 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(s_addr(full)), "r"(n_pages * SUBS * box_rows * 128) : "memory");
+        __syncwarp();
+        if (mine)
+          asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                       ::"r"((v ? s_v : s_k) + st * TILE + sub * SUB + pg * box_rows * 128), "l"(v ? &tm_v : &tm_k), "r"(s_addr(full)), "r"(sub * 64), "r"(slot), "r"(kvh), "r"(page) : "memory");
+        __syncwarp();
+        issued[v] = j + 1;
+      }
+    }
+    if (!ok) {      // copies in flight end before the shared memory does
+      for (int x = max(0, issued[0] - KS); x < issued[0]; x++) a_wait_on(s_addr(&sh.k_full[x % KS]), (x / KS) & 1, s_addr(&sh.flag));
+      for (int x = max(0, issued[1] - VS); x < issued[1]; x++) a_wait_on(s_addr(&sh.v_full[x % VS]), (x / VS) & 1, s_addr(&sh.flag));
+    }
+  } else {
+    // ---- values that a product must not see: rows behind the last key, and what is not finite in rows that not every query sees (0 times it is not 0) ----
+    const int half = warp - 10;
+    bool ok = true;
+    for (int j = 0; ok && j < tiles; j++) {
+      const int st = j % VS, k0 = k_begin + j * T_KEYS;
+      ok = __all_sync(0xffffffffu, a_wait(sh, &sh.v_full[st], (j / VS) & 1));
+      if (!ok) break;
+      const int from = max(0, min(first_last + 1, k_end) - k0);      // the first row that somebody does not see
+      if (from < T_KEYS) {
+        bool changed = false;
+        for (int i = from * 8 + half * 32 + lane; i < T_KEYS * 8; i += 64) {
+          const int key = k0 + i / 8;
+#pragma unroll
+          for (int s = 0; s < SUBS; s++) {
+            const uint32_t a = s_v + st * TILE + s * SUB + i * 16;
+            if (key >= k_end) { st_s4(a, make_uint4(0, 0, 0, 0)); changed = true; continue; }
+            const uint4 x = ld_s4(a), y = make_uint4(finite_only<BF>(x.x), finite_only<BF>(x.y), finite_only<BF>(x.z), finite_only<BF>(x.w));
+            if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
+              st_s4(a, y);
+              changed = true;
+              atomicMin(&sh.bad_lo, key); atomicMax(&sh.bad_hi, key);
+            }
+          }
+        }
+        if (changed) fence_async();
+      }
+      __syncwarp();
+      if (lane == 0) a_bar_arrive(&sh.v_clean[st]);
+    }
+    }
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (n_parts > 1 && !*(volatile int*)&sh.abort) join_parts<T_R, D, T_THREADS>(p, w, unit, n_parts, kvh, &sh.flag);
+}
+
+// The map of a pool: [page][KV head][slot][value], boxes of 64 values x box_rows slots in the 128-byte-swizzle layout.
+int make_page_map(CUtensorMap* tm, const b200q_paged_cache* c, const void* pool, int box_rows) {
+  typedef CUresult (*encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<encode_fn> known{nullptr};
+  encode_fn fn = known.load(std::memory_order_acquire);
+  if (!fn) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    B200Q_CHECK_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q));
+    if (!f || q != cudaDriverEntryPointSuccess) return B200Q_ERR_UNSUPPORTED;
+    known.store(fn = (encode_fn)f, std::memory_order_release);
+  }
+  const cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->page_size, (cuuint64_t)c->n_kv_heads, (cuuint64_t)c->n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)c->row_stride * 2, (cuuint64_t)c->head_stride * 2, (cuuint64_t)c->page_stride * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, ones[4] = {1, 1, 1, 1};
+  const CUresult r = fn(tm, c->dtype == B200Q_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(pool), dims, strides, box, ones,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B200Q_OK : B200Q_ERR_UNSUPPORTED;
+}
+
+}  // namespace
