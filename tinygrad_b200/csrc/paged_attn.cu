@@ -6,6 +6,7 @@
 // that is loaded.  The keys are split over CTAs where the tiles alone do not fill the GPU: parts leave (m, sum, weighted sum) in the workspace and the one that is done
 // last adds them, in the order of the keys (results do not depend on timing), and puts its counter back.
 #include "paged.cuh"
+#include <algorithm>
 
 namespace {
 
@@ -89,9 +90,10 @@ __device__ __forceinline__ int64_t key_at(const AttnParams& p, int seq, int key)
 // ---- parts of the keys ----
 template <int R, int D> constexpr int PART = R * (D + 2);           // m [R], sum [R], weighted sum [R][D]
 
-// The tile's last part to be done adds all of them; by the whole CTA (THREADS).  m in log2.
+// The tile's last part to be done adds all of them; by the whole CTA (THREADS).  m in log2.  First every part's share of each row, a warp a row and a lane a part, then four values a thread over
+// all parts: loads that do not wait for one another (one value after the other, the two loops took 16 of 20 us of a call on 513 positions).  factors: shared, R x n_parts.
 template <int R, int D, int THREADS>
-__device__ __forceinline__ void join_parts(const AttnParams& p, const TilePlace& w, int unit, int n_parts, int kvh, int* s_flag) {
+__device__ __forceinline__ void join_parts(const AttnParams& p, const TilePlace& w, int unit, int n_parts, int kvh, int* s_flag, float* factors) {
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -103,20 +105,36 @@ __device__ __forceinline__ void join_parts(const AttnParams& p, const TilePlace&
   if (!*s_flag) return;
   __threadfence();
   const float* base = p.parts + (int64_t)unit * p.n_split * PART<R, D>;
-  for (int i = threadIdx.x; i < R * D; i += THREADS) {
-    const int r = i / D, d = i - r * D;
-    const int64_t pair = w.r0 + r;
-    if (pair >= (int64_t)w.n * p.group) break;
-    float m = -INFINITY, sum = 0.f, o = 0.f;
-    for (int s = 0; s < n_parts; s++) m = fmaxf(m, __ldcg(base + (int64_t)s * PART<R, D> + r));
-    for (int s = 0; s < n_parts; s++) {
-      const float* b = base + (int64_t)s * PART<R, D>;
-      const float ls = __ldcg(b + R + r), f = ls == 0.f ? 0.f : exp2f(__ldcg(b + r) - m);      // (a part without keys has sum 0)
+  const int lane = threadIdx.x & 31, live = (int)min((int64_t)R, (int64_t)w.n * p.group - w.r0);
+  for (int r = threadIdx.x >> 5; r < live; r += THREADS / 32) {
+    float m = -INFINITY, sum = 0.f;
+    for (int s = lane; s < n_parts; s += 32) m = fmaxf(m, __ldcg(base + (int64_t)s * PART<R, D> + r));
+    m = warp_max(m);
+    for (int s = lane; s < n_parts; s += 32) {
+      const float* b = base + (int64_t)s * PART<R, D> + r;
+      const float ls = __ldcg(b + R), f = ls == 0.f ? 0.f : exp2f(__ldcg(b) - m);      // (a part without keys has sum 0)
+      factors[s * R + r] = f;
       sum = fmaf(f, ls, sum);
-      o = fmaf(f, __ldcg(b + 2 * R + i), o);
     }
-    const int token = pair / p.group, head = kvh * p.group + (int)(pair - (int64_t)token * p.group);
-    store_as(p.out, p.out_dtype, (w.first_row + token) * p.out_stride + (int64_t)head * D + d, sum == 0.f ? 0.f : o / sum);
+    sum = warp_sum(sum);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (int s = lane; s < n_parts; s += 32) factors[s * R + r] *= inv;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < live * (D / 4); i += THREADS) {
+    const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+    const float* b = base + 2 * R + r * D + d;
+    float o[4] = {};
+#pragma unroll 8
+    for (int s = 0; s < n_parts; s++) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(b + (int64_t)s * PART<R, D>));
+      const float f = factors[s * R + r];
+      o[0] = fmaf(f, v.x, o[0]); o[1] = fmaf(f, v.y, o[1]); o[2] = fmaf(f, v.z, o[2]); o[3] = fmaf(f, v.w, o[3]);
+    }
+    const int pair = w.r0 + r, token = pair / p.group;
+    const int64_t at = (w.first_row + token) * p.out_stride + (int64_t)(kvh * p.group + pair - token * p.group) * D + d;
+#pragma unroll
+    for (int j = 0; j < 4; j++) store_as(p.out, p.out_dtype, at + j, o[j]);
   }
 }
 
@@ -127,6 +145,7 @@ __global__ void __launch_bounds__(S_THREADS) attn_simple_kernel(const AttnParams
   constexpr int R = S_R, NV = D >= 32 ? D / 32 : 1, LIVE = D >= 32 ? 32 : D;
   __shared__ float s_q[R][D], s_p[S_WARPS][R][32], s_o[R][D], s_m[S_WARPS][R], s_l[S_WARPS][R];
   __shared__ int s_flag;
+  extern __shared__ float s_f[];      // shares of the parts
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y, split = blockIdx.z;
@@ -231,7 +250,7 @@ __global__ void __launch_bounds__(S_THREADS) attn_simple_kernel(const AttnParams
       __stcg(mine + 2 * R + i, s_o[r][d]);
     }
   }
-  if (n_parts > 1) join_parts<R, D, S_THREADS>(p, w, unit, n_parts, kvh, &s_flag);
+  if (n_parts > 1) join_parts<R, D, S_THREADS>(p, w, unit, n_parts, kvh, &s_flag, s_f);
 }
 
 }  // namespace
@@ -240,11 +259,12 @@ __global__ void __launch_bounds__(S_THREADS) attn_simple_kernel(const AttnParams
 namespace {
 
 // ---- how the work is dealt ----
+constexpr int MAX_PARTS = 296;      // of a tile's keys: their shares of 16 rows take 19 KB of shared memory (of 256 rows, 64 parts at most, 64 KB)
 struct Plan { int tiles, tiles_per_seq, n_split, split_len, above, up_to, rows; size_t at, counters, bytes; };      // at, counters, bytes: in the workspace
 
 // Tiles of `rows` pairs: those of all sequences at their largest, or (ragged batches, if that is less) the pairs' tiles and a broken one for each sequence.  Keys are split until
 // there are about `want` CTAs, in parts of at least `least` keys.
-Plan make_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group, int above, int up_to, int rows, int want, int least, int unit) {
+Plan make_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group, int above, int up_to, int rows, int want, int least, int unit, int most_parts) {
   const int n_kv = c->n_kv_heads, most_new = b->max_new < up_to ? b->max_new : up_to;
   const int64_t per = ((int64_t)most_new * group + rows - 1) / rows, even = per * b->n_seqs, ragged = (int64_t)b->n_rows * group / rows + b->n_seqs;
   Plan p{};
@@ -253,9 +273,9 @@ Plan make_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group
   p.tiles = (int)(even <= ragged ? even : ragged);
   const int64_t len = b->max_len > 0 ? b->max_len : 1, most = (len + least - 1) / least;
   const int64_t parts = want / ((int64_t)p.tiles * n_kv);
-  const int64_t n = parts < 1 ? 1 : parts < most ? parts : most;
+  const int64_t n = std::min(std::max(std::min(parts, most), (int64_t)1), (int64_t)most_parts);
   p.split_len = (int)(((len + n - 1) / n + unit - 1) / unit * unit);
-  p.n_split = (int)((len + p.split_len - 1) / p.split_len);
+  p.n_split = (int)((len + p.split_len - 1) / p.split_len);      // at most want
   p.bytes = p.n_split == 1 ? 0 : ((size_t)p.tiles * n_kv * p.n_split * rows * (c->head_dim + 2) * 4 + 255) / 256 * 256;
   return p;
 }
@@ -274,14 +294,14 @@ Deal deal_of(const b200q_paged_cache* c, const b200q_paged_batch* b, int group, 
   const int few = FEW_PAIRS / group > 1 ? FEW_PAIRS / group : 1;
   d.many = tiles_take && b->max_new > few;
   if (d.many) {
-    d.plan[0] = make_plan(c, b, group, few, INT32_MAX, T_R, 148, 512, T_KEYS);
+    d.plan[0] = make_plan(c, b, group, few, INT32_MAX, T_R, 148, 512, T_KEYS, 64);
     d.n = 1;
     if (b->n_seqs > 1) {
-      d.plan[1] = make_plan(c, b, group, 0, few, 16, MOST_CTAS, 128, 32);
+      d.plan[1] = make_plan(c, b, group, 0, few, 16, MOST_CTAS, 128, 32, MAX_PARTS);
       d.n = 2;
     } else d.plan[0].above = 0;
   } else {
-    d.plan[0] = c->dtype == B200Q_F32 ? make_plan(c, b, group, 0, INT32_MAX, S_R, 4 * 148, 256, 32) : make_plan(c, b, group, 0, INT32_MAX, 16, b->n_seqs > 1 ? MOST_CTAS : 296, 128, 32);
+    d.plan[0] = c->dtype == B200Q_F32 ? make_plan(c, b, group, 0, INT32_MAX, S_R, 4 * 148, 256, 32, MAX_PARTS) : make_plan(c, b, group, 0, INT32_MAX, 16, b->n_seqs > 1 ? MOST_CTAS : 296, 128, 32, MAX_PARTS);
     d.n = 1;
   }
   const size_t parts = d.plan[0].bytes + d.plan[1].bytes;
@@ -381,10 +401,11 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
     }
     const int d = dim == 16 ? 0 : dim == 32 ? 1 : dim == 64 ? 2 : 3;
     const AttnKernel kernel = d == 0 ? pick_rows<16>(cache->dtype, parts) : d == 1 ? pick_rows<32>(cache->dtype, parts) : d == 2 ? pick_rows<64>(cache->dtype, parts) : pick_rows<128>(cache->dtype, parts);
-    const int smem = cache->dtype == B200Q_F32 ? 0 : d == 0 ? R_SMEM<16> : d == 1 ? R_SMEM<32> : d == 2 ? R_SMEM<64> : R_SMEM<128>;
+    const bool simple = cache->dtype == B200Q_F32;
+    const int smem = simple ? plan.n_split * S_R * 4 : d == 0 ? R_SMEM<16> : d == 1 ? R_SMEM<32> : d == 2 ? R_SMEM<64> : R_SMEM<128>;
     static PerDeviceFlag allowed[2][2][4];
-    if (smem && (rc = allow_smem(kernel, smem, allowed[type][parts - 1][d])) != B200Q_OK) return rc;
-    B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles, n_kv, plan.n_split), dim3(smem ? R_THREADS : S_THREADS), (size_t)smem, st, pdl, p));
+    if (!simple && (rc = allow_smem(kernel, smem, allowed[type][parts - 1][d])) != B200Q_OK) return rc;
+    B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles, n_kv, plan.n_split), dim3(simple ? S_THREADS : R_THREADS), (size_t)smem, st, pdl, p));
   }
   return B200Q_OK;
 }

@@ -72,21 +72,26 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3, kvh = blockIdx.y, split = blockIdx.z;
+  const int ps = p.t.page_size, k_begin = split * p.split_len;
+  const bool whole = ps % KB == 0;                      // a block lies in one page
+  auto block_key = [&](int it) { return k_begin + (warp + it * RW) * KB; };
+  // pages of this and the next 32 blocks; asked for before it is known how many of them there are, together with what says so
+  auto page_id = [&](int seq, int it) {
+    const int index = block_key(it) / ps;
+    return whole && index < p.t.table_stride ? p.t.pages[(int64_t)seq * p.t.table_stride + index] : -1;
+  };
+  int ids = p.tiles_per_seq ? page_id(blockIdx.x / p.tiles_per_seq, lane) : 0;
   const TilePlace w = place_of_tile<R>(p, blockIdx.x);
   if (w.n == 0) return;
-  const int n_parts = max(1, (w.keys + p.split_len - 1) / p.split_len), k_begin = split * p.split_len, k_end = min(w.keys, k_begin + p.split_len);
+  const int n_parts = max(1, (w.keys + p.split_len - 1) / p.split_len), k_end = min(w.keys, k_begin + p.split_len);
   if (split >= n_parts) return;
-  const int64_t pairs = (int64_t)w.n * p.group;
-  const int ps = p.t.page_size;
-  const bool whole = ps % KB == 0;                      // a block lies in one page
+  if (!p.tiles_per_seq) ids = page_id(w.seq, lane);
+  const int pairs = w.n * p.group;
   const int blocks = max(0, (k_end - k_begin + KB - 1) / KB), mine = (blocks - warp + RW - 1) / RW;      // this warp's: warp, warp + RW, ...
-  const int32_t* row_pages = p.t.pages + (int64_t)w.seq * p.t.table_stride;
   const uint16_t* kp = static_cast<const uint16_t*>(p.k) + kvh * p.head_stride;
   const uint16_t* vp = static_cast<const uint16_t*>(p.v) + kvh * p.head_stride;
   const uint32_t base = (uint32_t)__cvta_generic_to_shared(ring) + warp * (ST * 2 * BLOCK);
-  auto block_key = [&](int it) { return k_begin + (warp + it * RW) * KB; };
-  auto page_id = [&](int it) { return whole && it < mine ? row_pages[block_key(it) / ps] : 0; };
-  int ids = page_id(lane), ids_next = page_id(32 + lane);        // pages of this and the next 32 blocks
+  int ids_next = mine > 32 ? page_id(w.seq, 32 + lane) : 0;
   auto issue = [&](int it) {
     if (it < mine) {
       const int key0 = block_key(it);
@@ -95,7 +100,7 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
       bool there0 = true;
       if (whole) {
         const int page = __shfl_sync(0xffffffffu, ids, it & 31);
-        if ((it & 31) == 31) { ids = ids_next; ids_next = page_id(it + 33 + lane); }
+        if ((it & 31) == 31) { ids = ids_next; ids_next = mine > it + 33 ? page_id(w.seq, it + 33 + lane) : 0; }
         there0 = page >= 0 && page < p.t.n_pages;
         if (!there0 && lane == 0) atomicExch(&g_paged_attn_status, 2);
         at0 = there0 ? page * p.page_stride + (int64_t)(key0 % ps) * p.row_stride : 0;
@@ -114,29 +119,55 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+
+  // the queries, as the instruction's A operand: rows g and g + 8.  All loads first (one that waits for the one before it is 5 us a CTA), then the first blocks, then the parts.
+  float2 f[2][2 * KK];
+  int last[2];                                           // the position a row may see up to
+  {
+    int64_t at[2];
+    bool live[2];
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int pair = w.r0 + g + e * 8, token = pair / p.group;
+      live[e] = pair < pairs;
+      last[e] = live[e] ? w.length + token : -1;
+      at[e] = live[e] ? (w.first_row + token) * p.q_stride + (int64_t)(kvh * p.group + pair - token * p.group) * D + tq * 2 : 0;
+    }
+    const int size = type_size(p.q_dtype);
+    const bool paired = (((uintptr_t)p.q | (uintptr_t)(p.q_stride * size)) & (2 * size - 1)) == 0;
+    if (p.q_dtype == B200Q_F32 && paired) {
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int j = 0; j < 2 * KK; j++) f[e][j] = live[e] ? *reinterpret_cast<const float2*>(static_cast<const float*>(p.q) + at[e] + j * 8) : make_float2(0.f, 0.f);
+    } else if (paired) {
+      uint32_t x[2][2 * KK];
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int j = 0; j < 2 * KK; j++) x[e][j] = live[e] ? *reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.q) + at[e] + j * 8) : 0u;
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int j = 0; j < 2 * KK; j++) f[e][j] = unpack2(x[e][j], p.q_dtype == B200Q_BF16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int j = 0; j < 2 * KK; j++) f[e][j] = live[e] ? load2_as_f(p.q, p.q_dtype, at[e] + j * 8) : make_float2(0.f, 0.f);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < ST - 1; i++) issue(i);
-
-  // the queries, as the instruction's A operand: rows g and g + 8
   uint32_t qa[N][KK][4];
   float qs[2];
-  int last[2];                                           // the position a row may see up to
 #pragma unroll
   for (int e = 0; e < 2; e++) {
-    const int64_t pair = w.r0 + g + e * 8;
-    const bool live = pair < pairs;
-    const int token = live ? (int)(pair / p.group) : 0;
-    const int64_t at = (w.first_row + token) * p.q_stride + (int64_t)(kvh * p.group + (live ? pair - (int64_t)token * p.group : 0)) * D + tq * 2;
-    last[e] = live ? w.length + token : -1;
-    float2 f[2 * KK];
-    float amax = 0.f;
-#pragma unroll
-    for (int j = 0; j < 2 * KK; j++) {
-      f[j] = live ? load2_as_f(p.q, p.q_dtype, at + j * 8) : make_float2(0.f, 0.f);
-      amax = fmaxf(amax, fmaxf(fabsf(f[j].x), fabsf(f[j].y)));
-    }
     float up = 1.f, down = 1.f;
     if (N == 2) {
+      float amax = 0.f;
+#pragma unroll
+      for (int j = 0; j < 2 * KK; j++) amax = fmaxf(amax, fmaxf(fabsf(f[e][j].x), fabsf(f[e][j].y)));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       pow2_scale(amax, up, down);
@@ -145,7 +176,7 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
 #pragma unroll
     for (int j = 0; j < 2 * KK; j++) {
       uint32_t v[N];
-      parts_of<N, BF>(f[j].x * up, f[j].y * up, v);
+      parts_of<N, BF>(f[e][j].x * up, f[e][j].y * up, v);
 #pragma unroll
       for (int i = 0; i < N; i++) qa[i][j / 2][(j & 1) * 2 + e] = v[i];
     }
@@ -280,7 +311,7 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
   float* const part = p.parts + ((int64_t)unit * p.n_split + split) * PART<R, D>;
   for (int i = tid; i < R * D / 4; i += R_THREADS) {
     const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-    const int64_t pair = w.r0 + r;
+    const int pair = w.r0 + r;
     if (pair >= pairs) break;
     float ml = -INFINITY, sum = 0.f, v[4] = {};
 #pragma unroll
@@ -293,8 +324,8 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
       v[0] += f.x; v[1] += f.y; v[2] += f.z; v[3] += f.w;
     }
     if (n_parts == 1) {
-      const int token = (int)(pair / p.group);
-      const int64_t at = (w.first_row + token) * p.out_stride + (int64_t)(kvh * p.group + (pair - (int64_t)token * p.group)) * D + d;
+      const int token = pair / p.group;
+      const int64_t at = (w.first_row + token) * p.out_stride + (int64_t)(kvh * p.group + pair - token * p.group) * D + d;
 #pragma unroll
       for (int j = 0; j < 4; j++) store_as(p.out, p.out_dtype, at + j, sum == 0.f ? 0.f : v[j] / sum);
     } else {
@@ -302,7 +333,7 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
       __stcg(reinterpret_cast<float4*>(part + 2 * R + r * D + d), make_float4(v[0], v[1], v[2], v[3]));
     }
   }
-  if (n_parts > 1) join_parts<R, D, R_THREADS>(p, w, unit, n_parts, kvh, &s_flag);
+  if (n_parts > 1) join_parts<R, D, R_THREADS>(p, w, unit, n_parts, kvh, &s_flag, s_o);
 }
 
 }  // namespace

@@ -521,7 +521,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
   __syncthreads();
   fence_after();
   if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
-  if (n_parts > 1 && !*(volatile int*)&sh.abort) join_parts<T_R, D, T_THREADS>(p, w, unit, n_parts, kvh, &sh.flag);
+  if (n_parts > 1 && !*(volatile int*)&sh.abort) join_parts<T_R, D, T_THREADS>(p, w, unit, n_parts, kvh, &sh.flag, reinterpret_cast<float*>(raw));
 }
 
 // The map of a pool: [page][KV head][slot][value], boxes of 64 values x box_rows slots in the 128-byte-swizzle layout.
