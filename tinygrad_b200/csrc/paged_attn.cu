@@ -31,53 +31,56 @@ struct AttnParams {
 
 struct TilePlace { int seq, first_row, n, r0, length, keys; };       // r0: the tile's first (token, head) pair; keys: those its last row sees, at most
 
+// A sequence's rows, those of them that this kernel has, its positions that may be attended, the position of its first new token
+struct SeqPlace { int first_row, n, cap, start; };
+__device__ __forceinline__ SeqPlace place_of_seq(const AttnParams& p, int s) {
+  const PagedTables& t = p.t;
+  const int b0 = t.row_off[s], e0 = t.row_off[s + 1], length = t.length[s];
+  const int b = min(max(b0, 0), t.n_rows), e = min(max(e0, b), t.n_rows), n = min(e - b, t.max_new);
+  const int64_t room = (int64_t)t.table_stride * t.page_size;
+  return SeqPlace{b, n > p.above && n <= p.up_to ? n : 0, (int)min((int64_t)min(max(length, 0), t.max_len), room), length - (e - b)};
+}
+__device__ __forceinline__ void check_place(const AttnParams& p, int s, const SeqPlace& q) {      // what the tables promise and the bounds do not hold
+  if (min(max(p.t.row_off[s + 1], q.first_row), p.t.n_rows) - q.first_row > q.n || p.t.length[s] > q.cap) atomicExch(&g_paged_attn_status, 2);
+}
+template <int R>
+__device__ __forceinline__ TilePlace tile_of_seq(const AttnParams& p, int s, const SeqPlace& q, int tile) {
+  TilePlace w{s, q.first_row, q.n, tile * R, q.start, 0};
+  const int last = min((w.r0 + R - 1) / p.group, q.n - 1);
+  w.keys = max(0, min(q.cap, q.start + last + 1));
+  return w;
+}
+
 // R pairs to a tile; by a whole warp.  n == 0: nothing to do.
 template <int R>
 __device__ __forceinline__ TilePlace place_of_tile(const AttnParams& p, int tile) {
   const PagedTables& t = p.t;
   const int lane = threadIdx.x & 31;
-  TilePlace w{0, 0, 0, 0, 0, 0};
-  auto rows = [&](int s) {
-    const int b = min(max(t.row_off[s], 0), t.n_rows), e = min(max(t.row_off[s + 1], b), t.n_rows);
-    return make_int2(b, e - b);
-  };
-  auto ours = [&](int n) { n = min(n, t.max_new); return n > p.above && n <= p.up_to ? n : 0; };
+  int s = 0;
   if (p.tiles_per_seq) {
-    w.seq = tile / p.tiles_per_seq;
-    w.r0 = (tile - w.seq * p.tiles_per_seq) * R;
+    s = tile / p.tiles_per_seq;
+    tile -= s * p.tiles_per_seq;
   } else {
-    int s = 0, before = 0;
     bool found = false;
     for (int s0 = 0; s0 < t.n_seqs && !found; s0 += 32) {
-      int mine = 0;
-      if (s0 + lane < t.n_seqs) mine = (int)(((int64_t)ours(rows(s0 + lane).y) * p.group + R - 1) / R);
+      const int mine = s0 + lane < t.n_seqs ? (place_of_seq(p, s0 + lane).n * p.group + R - 1) / R : 0;
       int sum = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) { const int u = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += u; }
-      const unsigned here = __ballot_sync(0xffffffffu, tile < before + sum);
+      const unsigned here = __ballot_sync(0xffffffffu, tile < sum);
       if (here) {
         const int l = __ffs(here) - 1;
         s = s0 + l;
-        before += __shfl_sync(0xffffffffu, sum - mine, l);
+        tile -= __shfl_sync(0xffffffffu, sum - mine, l);
         found = true;
-      } else before += __shfl_sync(0xffffffffu, sum, 31);
+      } else tile -= __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (!found) return w;
-    w.seq = s;
-    w.r0 = (tile - before) * R;
+    if (!found) return TilePlace{};
   }
-  const int2 r = rows(w.seq);
-  w.first_row = r.x;
-  w.length = t.length[w.seq];
-  const int n = ours(r.y);
-  if (w.r0 >= (int64_t)n * p.group) return w;
-  w.n = n;
-  const int64_t cap = min((int64_t)min(w.length, t.max_len), (int64_t)t.table_stride * t.page_size);
-  if ((r.y > n || w.length > cap) && lane == 0) atomicExch(&g_paged_attn_status, 2);
-  const int last = min((w.r0 + R - 1) / p.group, n - 1);
-  w.length -= r.y;                                           // from here on: the position of the first new token
-  w.keys = max(0, (int)min(cap, (int64_t)w.length + last + 1));
-  return w;
+  const SeqPlace q = place_of_seq(p, s);
+  if (tile * R >= q.n * p.group) return TilePlace{};
+  if (lane == 0 && tile == 0) check_place(p, s, q);
+  return tile_of_seq<R>(p, s, q, tile);
 }
 
 // the offset of a key in the pages, or -1
@@ -92,26 +95,26 @@ template <int R, int D> constexpr int PART = R * (D + 2);           // m [R], su
 
 // The tile's last part to be done adds all of them; by the whole CTA (THREADS).  m in log2.  First every part's share of each row, a warp a row and a lane a part, then four values a thread over
 // all parts: loads that do not wait for one another (one value after the other, the two loops took 16 of 20 us of a call on 513 positions).  factors: shared, R x n_parts.
-template <int R, int D, int THREADS>
-__device__ __forceinline__ void join_parts(const AttnParams& p, const TilePlace& w, int unit, int n_parts, int kvh, int* s_flag, float* factors) {
+// part_at(s): where part s is.
+template <int R, int D, int THREADS, typename At>
+__device__ __forceinline__ void join_parts(const AttnParams& p, const TilePlace& w, int* counter, int n_parts, int kvh, int* s_flag, float* factors, At part_at) {
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) {
-    const int old = atomicAdd(p.counters + unit, 1);
+    const int old = atomicAdd(counter, 1);
     *s_flag = old == n_parts - 1;
-    if (old == n_parts - 1) p.counters[unit] = 0;
+    if (old == n_parts - 1) *counter = 0;
   }
   __syncthreads();
   if (!*s_flag) return;
   __threadfence();
-  const float* base = p.parts + (int64_t)unit * p.n_split * PART<R, D>;
   const int lane = threadIdx.x & 31, live = (int)min((int64_t)R, (int64_t)w.n * p.group - w.r0);
   for (int r = threadIdx.x >> 5; r < live; r += THREADS / 32) {
     float m = -INFINITY, sum = 0.f;
-    for (int s = lane; s < n_parts; s += 32) m = fmaxf(m, __ldcg(base + (int64_t)s * PART<R, D> + r));
+    for (int s = lane; s < n_parts; s += 32) m = fmaxf(m, __ldcg(part_at(s) + r));
     m = warp_max(m);
     for (int s = lane; s < n_parts; s += 32) {
-      const float* b = base + (int64_t)s * PART<R, D> + r;
+      const float* b = part_at(s) + r;
       const float ls = __ldcg(b + R), f = ls == 0.f ? 0.f : exp2f(__ldcg(b) - m);      // (a part without keys has sum 0)
       factors[s * R + r] = f;
       sum = fmaf(f, ls, sum);
@@ -123,11 +126,10 @@ __device__ __forceinline__ void join_parts(const AttnParams& p, const TilePlace&
   __syncthreads();
   for (int i = threadIdx.x; i < live * (D / 4); i += THREADS) {
     const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-    const float* b = base + 2 * R + r * D + d;
     float o[4] = {};
 #pragma unroll 8
     for (int s = 0; s < n_parts; s++) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(b + (int64_t)s * PART<R, D>));
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(part_at(s) + 2 * R + r * D + d));
       const float f = factors[s * R + r];
       o[0] = fmaf(f, v.x, o[0]); o[1] = fmaf(f, v.y, o[1]); o[2] = fmaf(f, v.z, o[2]); o[3] = fmaf(f, v.w, o[3]);
     }
@@ -250,7 +252,8 @@ __global__ void __launch_bounds__(S_THREADS) attn_simple_kernel(const AttnParams
       __stcg(mine + 2 * R + i, s_o[r][d]);
     }
   }
-  if (n_parts > 1) join_parts<R, D, S_THREADS>(p, w, unit, n_parts, kvh, &s_flag, s_f);
+  const float* first = p.parts + (int64_t)unit * p.n_split * PART<R, D>;
+  if (n_parts > 1) join_parts<R, D, S_THREADS>(p, w, p.counters + unit, n_parts, kvh, &s_flag, s_f, [&](int s) { return first + (int64_t)s * PART<R, D>; });
 }
 
 }  // namespace
@@ -260,7 +263,7 @@ namespace {
 
 // ---- how the work is dealt ----
 constexpr int MAX_PARTS = 296;      // of a tile's keys: their shares of 16 rows take 19 KB of shared memory (of 256 rows, 64 parts at most, 64 KB)
-struct Plan { int tiles, tiles_per_seq, n_split, split_len, above, up_to, rows; size_t at, counters, bytes; };      // at, counters, bytes: in the workspace
+struct Plan { int tiles, tiles_per_seq, n_split, split_len, above, up_to, ctas; int64_t rounds; size_t bytes; };      // bytes: of the parts in the workspace
 
 // Tiles of `rows` pairs: those of all sequences at their largest, or (ragged batches, if that is less) the pairs' tiles and a broken one for each sequence.  Keys are split until
 // there are about `want` CTAs, in parts of at least `least` keys.
@@ -282,9 +285,18 @@ Plan make_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group
 
 // The workspace begins with the counters of the tiles that are split, MAX_UNITS for each kernel of a call: a fixed place, whatever calls share the workspace.  Tiles x KV heads are split only
 // where they are at most half of the CTAs that are wanted.
-constexpr int MAX_UNITS = 2048, MOST_CTAS = 8 * 296;
+constexpr int MAX_UNITS = 2048, ROWS_CTAS = 296, MOST_CTAS = 4 * 148;
 constexpr size_t COUNTERS_BYTES = 2 * MAX_UNITS * sizeof(int);
-static_assert(MOST_CTAS / 2 <= MAX_UNITS, "counters");
+static_assert(MOST_CTAS / 2 <= MAX_UNITS && ROWS_CTAS <= MAX_UNITS, "counters");
+
+// The rows kernel: as many CTAs as run at once, or as there is work for; parts of every CTA
+Plan rows_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group, int above, int up_to) {
+  Plan p = make_plan(c, b, group, above, up_to, 16, 1, 1, ROUND, 1);
+  p.rounds = (int64_t)p.tiles * c->n_kv_heads * std::max<int64_t>(1, ((int64_t)b->max_len + ROUND - 1) / ROUND);
+  p.ctas = (int)std::min((p.rounds + R_LEAST - 1) / R_LEAST, (int64_t)ROWS_CTAS);
+  p.bytes = (size_t)p.ctas * 2 * 16 * (c->head_dim + 2) * 4;
+  return p;
+}
 
 constexpr int FEW_PAIRS = 32;      // (token, head) pairs of a sequence that the rows kernel takes
 // The kernels of a call and their shares of it.  many: sequences of more than FEW_PAIRS pairs go to the tiles kernel.
@@ -297,31 +309,38 @@ Deal deal_of(const b200q_paged_cache* c, const b200q_paged_batch* b, int group, 
     d.plan[0] = make_plan(c, b, group, few, INT32_MAX, T_R, 148, 512, T_KEYS, 64);
     d.n = 1;
     if (b->n_seqs > 1) {
-      d.plan[1] = make_plan(c, b, group, 0, few, 16, MOST_CTAS, 128, 32, MAX_PARTS);
+      d.plan[1] = rows_plan(c, b, group, 0, few);
       d.n = 2;
     } else d.plan[0].above = 0;
   } else {
-    d.plan[0] = c->dtype == B200Q_F32 ? make_plan(c, b, group, 0, INT32_MAX, S_R, 4 * 148, 256, 32, MAX_PARTS) : make_plan(c, b, group, 0, INT32_MAX, 16, b->n_seqs > 1 ? MOST_CTAS : 296, 128, 32, MAX_PARTS);
+    d.plan[0] = c->dtype == B200Q_F32 ? make_plan(c, b, group, 0, INT32_MAX, S_R, MOST_CTAS, 256, 32, MAX_PARTS) : rows_plan(c, b, group, 0, INT32_MAX);
     d.n = 1;
   }
   const size_t parts = d.plan[0].bytes + d.plan[1].bytes;
   d.bytes = parts ? COUNTERS_BYTES + parts : 0;
   return d;
 }
-// The tiles kernel: 16-bit pages of whole boxes
-bool pages_for_tiles(const b200q_paged_cache* c) {
-  return c->dtype != B200Q_F32 && (c->head_dim == 64 || c->head_dim == 128) && c->page_size >= 8 && (c->page_size & (c->page_size - 1)) == 0 &&
-         c->page_stride < (1LL << 38) && c->head_stride < (1LL << 38) && c->row_stride < (1LL << 38);
+// TMA boxes of pages: 64 values x 16 positions (rows kernel), x a page's positions up to 128 (tiles kernel, whose tiles of 128 positions are whole boxes)
+bool pages_have_boxes(const b200q_paged_cache* c) {
+  return c->dtype != B200Q_F32 && c->head_dim >= 64 && c->page_size % KB == 0 && c->page_stride < (1LL << 38) && c->head_stride < (1LL << 38) && c->row_stride < (1LL << 38);
 }
+bool pages_for_tiles(const b200q_paged_cache* c) { return pages_have_boxes(c) && (c->page_size & (c->page_size - 1)) == 0; }
 int box_rows_of(const b200q_paged_cache* c) { return c->page_size < T_KEYS ? c->page_size : T_KEYS; }
 
-typedef void (*AttnKernel)(const AttnParams);
+typedef void (*SimpleKernel)(const AttnParams);
+typedef void (*RowsKernel)(const AttnParams, const CUtensorMap, const CUtensorMap);
+constexpr int R_RING_OF[4] = {R_RING<16>, R_RING<32>, R_RING<64>, R_RING<128>};
 typedef void (*TilesKernel)(const AttnParams, const CUtensorMap, const CUtensorMap, int);
-template <int D>
-AttnKernel pick_rows(int kv_dtype, int parts) {
-  if (kv_dtype == B200Q_F32) return attn_simple_kernel<D, float>;
-  if (kv_dtype == B200Q_F16) return parts == 1 ? attn_rows_kernel<D, 1, false> : attn_rows_kernel<D, 2, false>;
-  return parts == 1 ? attn_rows_kernel<D, 1, true> : attn_rows_kernel<D, 3, true>;
+SimpleKernel pick_simple(int dim) { return dim == 16 ? attn_simple_kernel<16, float> : dim == 32 ? attn_simple_kernel<32, float> : dim == 64 ? attn_simple_kernel<64, float> : attn_simple_kernel<128, float>; }
+template <int D, bool BOXES>
+RowsKernel pick_rows_of(int kv_dtype, int parts) {
+  if (kv_dtype == B200Q_F16) return parts == 1 ? attn_rows_kernel<D, 1, false, BOXES> : attn_rows_kernel<D, 2, false, BOXES>;
+  return parts == 1 ? attn_rows_kernel<D, 1, true, BOXES> : attn_rows_kernel<D, 3, true, BOXES>;
+}
+RowsKernel pick_rows(int dim, int kv_dtype, int parts, bool boxes) {
+  if (dim == 128) return boxes ? pick_rows_of<128, true>(kv_dtype, parts) : pick_rows_of<128, false>(kv_dtype, parts);
+  if (dim == 64) return boxes ? pick_rows_of<64, true>(kv_dtype, parts) : pick_rows_of<64, false>(kv_dtype, parts);
+  return dim == 32 ? pick_rows_of<32, false>(kv_dtype, parts) : pick_rows_of<16, false>(kv_dtype, parts);
 }
 template <int D>
 TilesKernel pick_tiles(int kv_dtype, int parts, int* smem) {
@@ -368,19 +387,20 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
   if ((uintptr_t)a->q % type_size(a->q_dtype) || (uintptr_t)a->out % type_size(a->out_dtype) || (uintptr_t)a->workspace & 255) return B200Q_ERR_MISALIGNED;
   // one part of 16 bits where queries, keys and outputs have 16; two (bf16 keys: three, which the rows kernel has) where something is wider
   const int parts = a->q_dtype == cache->dtype && a->out_dtype != B200Q_F32 ? 1 : 2;
-  alignas(64) CUtensorMap tm_k, tm_v;
-  bool tiles_take = pages_for_tiles(cache) && (parts == 1 || cache->dtype == B200Q_F16);
-  Deal deal = deal_of(cache, batch, group, tiles_take);
-  if (deal.many) {
-    memset(&tm_k, 0, sizeof(tm_k)); memset(&tm_v, 0, sizeof(tm_v));
-    rc = make_page_map(&tm_k, cache, cache->k, box_rows_of(cache));
-    if (rc == B200Q_OK) rc = make_page_map(&tm_v, cache, cache->v, box_rows_of(cache));
-    if (rc == B200Q_ERR_UNSUPPORTED) deal = deal_of(cache, batch, group, false);      // strides that no map can have
+  alignas(64) CUtensorMap boxes[4];      // of the rows kernel and the tiles kernel, k and v each
+  memset(boxes, 0, sizeof(boxes));
+  bool have_boxes = pages_have_boxes(cache);
+  Deal deal = deal_of(cache, batch, group, pages_for_tiles(cache) && (parts == 1 || cache->dtype == B200Q_F16));
+  if (a->workspace_bytes < deal.bytes || (deal.bytes && !a->workspace)) return B200Q_ERR_TOO_LARGE;
+  for (int i = 0; i < 4 && have_boxes; i++) {
+    if (i < 2 ? deal.many && deal.n == 1 : !deal.many) continue;
+    rc = make_page_map(boxes + i, cache, i & 1 ? cache->v : cache->k, i < 2 ? KB : box_rows_of(cache));
+    if (rc == B200Q_ERR_UNSUPPORTED) { have_boxes = false; deal = deal_of(cache, batch, group, false); }      // strides that no map can have; b200q_paged_attention_workspace_bytes knows both deals
     else if (rc != B200Q_OK) return rc;
   }
-  if (deal.bytes && (!a->workspace || a->workspace_bytes < deal.bytes)) return B200Q_ERR_TOO_LARGE;
+  if (a->workspace_bytes < deal.bytes) return B200Q_ERR_TOO_LARGE;
   for (int i = 0; i < deal.n; i++)
-    if (deal.plan[i].n_split > 65535 || n_kv > 65535 || (int64_t)deal.plan[i].tiles * n_kv > INT32_MAX) return B200Q_ERR_TOO_LARGE;
+    if (deal.plan[i].rounds > INT32_MAX || deal.plan[i].n_split > 65535 || n_kv > 65535 || (int64_t)deal.plan[i].tiles * n_kv > INT32_MAX) return B200Q_ERR_TOO_LARGE;
   const cudaStream_t st = (cudaStream_t)stream;
   for (int i = 0; i < deal.n; i++) {
     const Plan& plan = deal.plan[i];
@@ -396,16 +416,18 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
       const TilesKernel kernel = dim == 64 ? pick_tiles<64>(cache->dtype, parts, &smem) : pick_tiles<128>(cache->dtype, parts, &smem);
       static PerDeviceFlag allowed[2][2][2];
       if ((rc = allow_smem(kernel, smem, allowed[type][parts - 1][dim == 128])) != B200Q_OK) return rc;
-      B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles * n_kv, plan.n_split), dim3(T_THREADS), (size_t)smem, st, pdl, p, tm_k, tm_v, box_rows_of(cache)));
+      B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles * n_kv, plan.n_split), dim3(T_THREADS), (size_t)smem, st, pdl, p, boxes[2], boxes[3], box_rows_of(cache)));
       continue;
     }
-    const int d = dim == 16 ? 0 : dim == 32 ? 1 : dim == 64 ? 2 : 3;
-    const AttnKernel kernel = d == 0 ? pick_rows<16>(cache->dtype, parts) : d == 1 ? pick_rows<32>(cache->dtype, parts) : d == 2 ? pick_rows<64>(cache->dtype, parts) : pick_rows<128>(cache->dtype, parts);
-    const bool simple = cache->dtype == B200Q_F32;
-    const int smem = simple ? plan.n_split * S_R * 4 : d == 0 ? R_SMEM<16> : d == 1 ? R_SMEM<32> : d == 2 ? R_SMEM<64> : R_SMEM<128>;
-    static PerDeviceFlag allowed[2][2][4];
-    if (!simple && (rc = allow_smem(kernel, smem, allowed[type][parts - 1][d])) != B200Q_OK) return rc;
-    B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles, n_kv, plan.n_split), dim3(simple ? S_THREADS : R_THREADS), (size_t)smem, st, pdl, p));
+    if (cache->dtype == B200Q_F32) {
+      B200Q_CHECK_CUDA(launch_k(pick_simple(dim), dim3(plan.tiles, n_kv, plan.n_split), dim3(S_THREADS), (size_t)(plan.n_split * S_R * 4), st, pdl, p));
+      continue;
+    }
+    const int d = dim == 16 ? 0 : dim == 32 ? 1 : dim == 64 ? 2 : 3, smem = R_RING_OF[d] + (parts == 1 ? 1 : type ? 3 : 2) * 16 * dim * 2 + 1024;
+    const RowsKernel kernel = pick_rows(dim, cache->dtype, parts, have_boxes);
+    static PerDeviceFlag allowed[2][2][2][4];
+    if ((rc = allow_smem(kernel, smem, allowed[have_boxes][type][parts - 1][d])) != B200Q_OK) return rc;
+    B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.ctas), dim3(R_THREADS), (size_t)smem, st, pdl, p, boxes[0], boxes[1]));
   }
   return B200Q_OK;
 }

@@ -12,8 +12,6 @@
 // Precision: N = 1, 16-bit queries and outputs: a probability loses half a step, as the output does.  N = 2, fp32 rows on fp16 keys: queries (under a power of two that keeps the row in range) and
 // probabilities are two halves each, and a tile's weighted sum starts from zero and is added in registers, because the tensor core cuts its sums where others round.
 #pragma once
-#include <cuda.h>
-#include <string.h>
 
 namespace {
 
@@ -29,27 +27,7 @@ struct SharedA {
   int abort, flag, bad_lo, bad_hi;
 };
 
-__device__ __forceinline__ uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void a_bar_init(uint64_t* b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s_addr(b)), "r"(n) : "memory"); }
-__device__ __forceinline__ void a_bar_arrive(uint64_t* b) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s_addr(b)) : "memory"); }
-// Bounded wait: false once another role has given up, or when the time is over (then the others are told).
-__device__ __forceinline__ bool a_wait_on(uint32_t bar, uint32_t parity, uint32_t abort) {
-  for (int i = 0; i < (1 << 20); i++) {
-    uint32_t ok, gone;
-    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity), "r"(2000) : "memory");
-    if (ok) return true;
-    asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(gone) : "r"(abort) : "memory");
-    if (gone) return false;
-  }
-  asm volatile("st.volatile.shared::cta.u32 [%0], 1;" ::"r"(abort) : "memory");
-  atomicExch(&g_paged_attn_status, 1);
-  return false;
-}
-__device__ __forceinline__ bool a_wait(SharedA& sh, uint64_t* b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(s_addr(b)), "r"(parity) : "memory");
-  return ok || a_wait_on(s_addr(b), parity, s_addr(&sh.abort));
-}
+__device__ __forceinline__ bool a_wait(SharedA& sh, uint64_t* b, uint32_t parity) { return bar_ready(b, parity) || a_wait_on(s_addr(b), parity, s_addr(&sh.abort)); }
 __device__ __forceinline__ void a_commit(uint64_t* b) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s_addr(b)) : "memory"); }
 
 // Operands in the 128-byte-swizzle layout: sub-tiles of 64 values (128 bytes) a row, 8 rows = 1024 bytes.  Q and K are read along a row (rows 1024 bytes per 8 apart); V, whose reduction runs over
@@ -87,9 +65,6 @@ __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ float pow2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ void st_s4(uint32_t a, uint4 v) { asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory"); }
 __device__ __forceinline__ uint4 ld_s4(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
@@ -521,28 +496,10 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
   __syncthreads();
   fence_after();
   if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
-  if (n_parts > 1 && !*(volatile int*)&sh.abort) join_parts<T_R, D, T_THREADS>(p, w, unit, n_parts, kvh, &sh.flag, reinterpret_cast<float*>(raw));
-}
-
-// The map of a pool: [page][KV head][slot][value], boxes of 64 values x box_rows slots in the 128-byte-swizzle layout.
-int make_page_map(CUtensorMap* tm, const b200q_paged_cache* c, const void* pool, int box_rows) {
-  typedef CUresult (*encode_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static std::atomic<encode_fn> known{nullptr};
-  encode_fn fn = known.load(std::memory_order_acquire);
-  if (!fn) {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    B200Q_CHECK_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q));
-    if (!f || q != cudaDriverEntryPointSuccess) return B200Q_ERR_UNSUPPORTED;
-    known.store(fn = (encode_fn)f, std::memory_order_release);
+  if (n_parts > 1 && !*(volatile int*)&sh.abort) {
+    const float* first = p.parts + (int64_t)unit * p.n_split * PART<T_R, D>;
+    join_parts<T_R, D, T_THREADS>(p, w, p.counters + unit, n_parts, kvh, &sh.flag, reinterpret_cast<float*>(raw), [&](int s) { return first + (int64_t)s * PART<T_R, D>; });
   }
-  const cuuint64_t dims[4] = {(cuuint64_t)c->head_dim, (cuuint64_t)c->page_size, (cuuint64_t)c->n_kv_heads, (cuuint64_t)c->n_pages};
-  const cuuint64_t strides[3] = {(cuuint64_t)c->row_stride * 2, (cuuint64_t)c->head_stride * 2, (cuuint64_t)c->page_stride * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, ones[4] = {1, 1, 1, 1};
-  const CUresult r = fn(tm, c->dtype == B200Q_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(pool), dims, strides, box, ones,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? B200Q_OK : B200Q_ERR_UNSUPPORTED;
 }
 
 }  // namespace
