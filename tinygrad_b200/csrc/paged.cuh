@@ -31,6 +31,17 @@ __device__ __forceinline__ void store_as(void* base, int type, int64_t i, float 
   else static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(v);
 }
 
+// Division of values below 2^31 by a number that the host knows: n / d = (high word of n * mul + n) >> shift (a division proper is forty dependent instructions)
+struct Divisor {
+  uint32_t d, mul, shift;
+  __device__ __forceinline__ int div(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
+};
+static inline Divisor divisor_of(int d) {
+  uint32_t shift = 0;
+  while ((1u << shift) < (uint32_t)d) shift++;      // d <= 2^shift < 2 d; mul = 2^32 (2^shift - d) / d + 1
+  return Divisor{(uint32_t)d, (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1), shift};
+}
+
 // ---- tables ----
 struct PagedTables {
   const int32_t *row_off, *length, *pages;

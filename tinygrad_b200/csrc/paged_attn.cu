@@ -21,9 +21,10 @@ struct AttnParams {
   int64_t q_stride, out_stride, page_stride, head_stride, row_stride;
   int n_heads, n_kv, group;
   float scale;               // times log2 e
+  Divisor by_group, by_kv, by_page;
   int tiles_per_seq;         // 0: tiles are counted sequence by sequence
   int above, up_to;          // sequences with above < new tokens <= up_to (those with others are another kernel's)
-  int n_split, split_len;
+  int n_split, split_len, n_sm;
   int* counters;
   float* parts;
   PagedTables t;
@@ -46,7 +47,7 @@ __device__ __forceinline__ void check_place(const AttnParams& p, int s, const Se
 template <int R>
 __device__ __forceinline__ TilePlace tile_of_seq(const AttnParams& p, int s, const SeqPlace& q, int tile) {
   TilePlace w{s, q.first_row, q.n, tile * R, q.start, 0};
-  const int last = min((w.r0 + R - 1) / p.group, q.n - 1);
+  const int last = min(p.by_group.div(w.r0 + R - 1), q.n - 1);
   w.keys = max(0, min(q.cap, q.start + last + 1));
   return w;
 }
@@ -93,47 +94,64 @@ __device__ __forceinline__ int64_t key_at(const AttnParams& p, int seq, int key)
 // ---- parts of the keys ----
 template <int R, int D> constexpr int PART = R * (D + 2);           // m [R], sum [R], weighted sum [R][D]
 
-// The tile's last part to be done adds all of them; by the whole CTA (THREADS).  m in log2.  First every part's share of each row, a warp a row and a lane a part, then four values a thread over
-// all parts: loads that do not wait for one another (one value after the other, the two loops took 16 of 20 us of a call on 513 positions).  factors: shared, R x n_parts.
-// part_at(s): where part s is.
+// The tile's last part to be done adds all of them; by the whole CTA (THREADS).  m in log2.  One thread's count releases what all have stored before the barrier.  Then the first AHEAD parts of every
+// thread's values are asked for, every part's share of each row is computed meanwhile (a warp a row, a lane a part), and the values are added.  factors: shared, R x n_parts.
+// part_at(s): where part s is.  (One value after the other, 513 positions took 16 us more; with a fence in every thread and the values behind the shares 2 us more.)
 template <int R, int D, int THREADS, typename At>
 __device__ __forceinline__ void join_parts(const AttnParams& p, const TilePlace& w, int* counter, int n_parts, int kvh, int* s_flag, float* factors, At part_at) {
-  __threadfence();
+  constexpr int AHEAD = 4;
   __syncthreads();
   if (threadIdx.x == 0) {
-    const int old = atomicAdd(counter, 1);
+    int old;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(counter) : "memory");
     *s_flag = old == n_parts - 1;
     if (old == n_parts - 1) *counter = 0;
   }
   __syncthreads();
   if (!*s_flag) return;
-  __threadfence();
-  const int lane = threadIdx.x & 31, live = (int)min((int64_t)R, (int64_t)w.n * p.group - w.r0);
+  const int lane = threadIdx.x & 31, live = min(R, w.n * p.group - w.r0);
+  float4 ahead[AHEAD];
+  auto value = [&](int i, int s) { return __ldcg(reinterpret_cast<const float4*>(part_at(s) + 2 * R + i * 4)); };
+  if ((int)threadIdx.x < live * (D / 4)) {
+#pragma unroll
+    for (int s = 0; s < AHEAD; s++) ahead[s] = value(threadIdx.x, min(s, n_parts - 1));
+  }
   for (int r = threadIdx.x >> 5; r < live; r += THREADS / 32) {
-    float m = -INFINITY, sum = 0.f;
-    for (int s = lane; s < n_parts; s += 32) m = fmaxf(m, __ldcg(part_at(s) + r));
+    float m = -INFINITY, sum = 0.f, m0 = -INFINITY, l0 = 0.f;
+    if (lane < n_parts) { m0 = __ldcg(part_at(lane) + r); l0 = __ldcg(part_at(lane) + R + r); }
+    m = m0;
+    for (int s = lane + 32; s < n_parts; s += 32) m = fmaxf(m, __ldcg(part_at(s) + r));
     m = warp_max(m);
-    for (int s = lane; s < n_parts; s += 32) {
-      const float* b = part_at(s) + r;
-      const float ls = __ldcg(b + R), f = ls == 0.f ? 0.f : exp2f(__ldcg(b) - m);      // (a part without keys has sum 0)
+    const float f0 = l0 == 0.f ? 0.f : exp2f(m0 - m);      // (a part without keys has sum 0)
+    sum = f0 * l0;
+    for (int s = lane + 32; s < n_parts; s += 32) {
+      const float ls = __ldcg(part_at(s) + R + r), f = ls == 0.f ? 0.f : exp2f(__ldcg(part_at(s) + r) - m);
       factors[s * R + r] = f;
       sum = fmaf(f, ls, sum);
     }
     sum = warp_sum(sum);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    for (int s = lane; s < n_parts; s += 32) factors[s * R + r] *= inv;
+    if (lane < n_parts) factors[lane * R + r] = f0 * inv;
+    for (int s = lane + 32; s < n_parts; s += 32) factors[s * R + r] *= inv;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < live * (D / 4); i += THREADS) {
     const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
     float o[4] = {};
-#pragma unroll 8
-    for (int s = 0; s < n_parts; s++) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(part_at(s) + 2 * R + r * D + d));
+    auto add = [&](float4 v, int s) {
       const float f = factors[s * R + r];
       o[0] = fmaf(f, v.x, o[0]); o[1] = fmaf(f, v.y, o[1]); o[2] = fmaf(f, v.z, o[2]); o[3] = fmaf(f, v.w, o[3]);
+    };
+    int s0 = 0;
+    if (i == (int)threadIdx.x) {
+#pragma unroll
+      for (int s = 0; s < AHEAD; s++)
+        if (s < n_parts) add(ahead[s], s);
+      s0 = AHEAD;
     }
-    const int pair = w.r0 + r, token = pair / p.group;
+#pragma unroll 8
+    for (int s = s0; s < n_parts; s++) add(value(i, s), s);
+    const int pair = w.r0 + r, token = p.by_group.div(pair);
     const int64_t at = (w.first_row + token) * p.out_stride + (int64_t)(kvh * p.group + pair - token * p.group) * D + d;
 #pragma unroll
     for (int j = 0; j < 4; j++) store_as(p.out, p.out_dtype, at + j, o[j]);
@@ -285,15 +303,15 @@ Plan make_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group
 
 // The workspace begins with the counters of the tiles that are split, MAX_UNITS for each kernel of a call: a fixed place, whatever calls share the workspace.  Tiles x KV heads are split only
 // where they are at most half of the CTAs that are wanted.
-constexpr int MAX_UNITS = 2048, ROWS_CTAS = 296, MOST_CTAS = 4 * 148;
+constexpr int N_SM = 148, MAX_UNITS = 2048, ROWS_CTAS = 2 * N_SM, MOST_CTAS = 4 * N_SM;      // of a B200
 constexpr size_t COUNTERS_BYTES = 2 * MAX_UNITS * sizeof(int);
 static_assert(MOST_CTAS / 2 <= MAX_UNITS && ROWS_CTAS <= MAX_UNITS, "counters");
 
 // The rows kernel: as many CTAs as run at once, or as there is work for; parts of every CTA
 Plan rows_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group, int above, int up_to) {
   Plan p = make_plan(c, b, group, above, up_to, 16, 1, 1, ROUND, 1);
-  p.rounds = (int64_t)p.tiles * c->n_kv_heads * std::max<int64_t>(1, ((int64_t)b->max_len + ROUND - 1) / ROUND);
-  p.ctas = (int)std::min((p.rounds + R_LEAST - 1) / R_LEAST, (int64_t)ROWS_CTAS);
+  p.rounds = (int64_t)p.tiles * c->n_kv_heads * (std::max<int64_t>(1, ((int64_t)b->max_len + ROUND - 1) / ROUND) + R_EXTRA);
+  p.ctas = (int)std::min(p.rounds, (int64_t)ROWS_CTAS);
   p.bytes = (size_t)p.ctas * 2 * 16 * (c->head_dim + 2) * 4;
   return p;
 }
@@ -407,8 +425,8 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
     int* const counters = (int*)a->workspace + i * MAX_UNITS;
     float* const parts_at = (float*)((char*)a->workspace + COUNTERS_BYTES + (i ? deal.plan[0].bytes : 0));
     const AttnParams p{a->q, cache->k, cache->v, a->out, a->q_dtype, a->out_dtype, a->q_stride ? a->q_stride : row, a->out_stride ? a->out_stride : row, cache->page_stride,
-                       cache->head_stride, cache->row_stride, a->n_heads, n_kv, group, (a->scale > 0.f ? a->scale : 1.f / sqrtf((float)dim)) * LOG2E, plan.tiles_per_seq, plan.above, plan.up_to,
-                       plan.n_split, plan.split_len, counters, parts_at, tables_of(cache, batch)};
+                       cache->head_stride, cache->row_stride, a->n_heads, n_kv, group, (a->scale > 0.f ? a->scale : 1.f / sqrtf((float)dim)) * LOG2E, divisor_of(group), divisor_of(n_kv), divisor_of(cache->page_size), plan.tiles_per_seq, plan.above, plan.up_to,
+                       plan.n_split, plan.split_len, N_SM, counters, parts_at, tables_of(cache, batch)};
     const bool pdl = i == 0 && (flags & B200Q_FLAG_PDL);
     const int type = cache->dtype == B200Q_BF16;
     if (deal.many && i == 0) {

@@ -23,7 +23,8 @@ constexpr int RW = 4, R_THREADS = RW * 32, KB = 16;
 template <int D> constexpr int R_BLOCK = KB * D * 2;                                      // bytes of a block's keys (or values)
 template <int D> constexpr int R_STAGES = D == 128 ? 3 : D == 64 ? 6 : 8;
 template <int D> constexpr int R_RING = RW * R_STAGES<D> * 2 * R_BLOCK<D> > RW * 16 * D * 4 ? RW * R_STAGES<D> * 2 * R_BLOCK<D> : RW * 16 * D * 4;
-constexpr int ROUND = RW * KB, R_LEAST = 2;                // positions of a round; rounds that a CTA has at least
+constexpr int ROUND = RW * KB, R_LEAST = 4;                // positions of a round; rounds that a CTA has at least, where there are enough for an SM each
+constexpr uint32_t R_LONG = 12, R_EXTRA = 4;           // rounds of a share from which the beginning and end of a unit count as R_EXTRA rounds
 
 __device__ __forceinline__ uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void a_bar_init(uint64_t* b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s_addr(b)), "r"(n) : "memory"); }
@@ -129,42 +130,50 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
   const bool whole = BOXES || ps % KB == 0;              // a block lies in one page
 
   // ---- this CTA's share ----
-  auto units_of = [&](const SeqPlace& q) { return (uint32_t)((q.n * p.group + R - 1) / R * p.n_kv); };
+  auto units_of = [&](const SeqPlace& q) { return (uint32_t)((unsigned)(q.n * p.group + R - 1) / R * p.n_kv); };
   auto rounds_of = [&](const SeqPlace& q) { return (uint32_t)max(1, (q.cap + ROUND - 1) / ROUND); };      // (without keys: somebody writes the zeros)
-  auto work_of = [&](int s) {
-    if (s >= p.t.n_seqs) return 0u;
-    const SeqPlace q = place_of_seq(p, s);
-    if (blockIdx.x == 0 && warp == 0 && q.n) check_place(p, s, q);
-    return units_of(q) * rounds_of(q);
-  };
-  auto sum_up = [&](uint32_t v) {
+  struct Work { uint32_t units, rounds; };
+  auto sums_of = [&](int s) {                            // of this lane's sequence and those of the lanes before it
+    Work v{0, 0};
+    if (s < p.t.n_seqs) {
+      const SeqPlace q = place_of_seq(p, s);
+      if (blockIdx.x == 0 && warp == 0 && q.n) check_place(p, s, q);
+      v.units = units_of(q);
+      v.rounds = v.units * rounds_of(q);
+    }
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const uint32_t u = __shfl_up_sync(0xffffffffu, v, o); if (lane >= o) v += u; }
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t u = __shfl_up_sync(0xffffffffu, v.units, o), r = __shfl_up_sync(0xffffffffu, v.rounds, o);
+      if (lane >= o) { v.units += u; v.rounds += r; }
+    }
     return v;
   };
-  uint32_t total = 0, sums = 0;
+  Work sums{}, all{};
   for (int s0 = 0; s0 < p.t.n_seqs; s0 += 32) {
-    sums = sum_up(work_of(s0 + lane));
-    total += __shfl_sync(0xffffffffu, sums, 31);
+    sums = sums_of(s0 + lane);
+    all.units += __shfl_sync(0xffffffffu, sums.units, 31);
+    all.rounds += __shfl_sync(0xffffffffu, sums.rounds, 31);
   }
-  // shares of `share` rounds, one more for the first `more` CTAs
-  const uint32_t ctas = min(gridDim.x, (total + R_LEAST - 1) / R_LEAST), c = blockIdx.x;
+  // A unit costs its rounds and, where shares are long, what it takes to begin and end one.  A share that would begin or end in that part does so where the unit begins.
+  const uint32_t ctas = min(gridDim.x, max(min(all.rounds, (uint32_t)p.n_sm), all.rounds / R_LEAST)), c = blockIdx.x;
   if (c >= ctas) return;
-  const uint32_t share = total / ctas, more = total - share * ctas, x_end = (c + 1) * share + min(c + 1, more);
+  const uint32_t extra = all.rounds / ctas >= R_LONG ? R_EXTRA : 0, total = all.rounds + extra * all.units;
+  const uint32_t share = total / ctas, more = total - share * ctas, x_end = (c + 1) * share + min(c + 1, more);      // one more for the first `more` CTAs
   uint32_t x = c * share + min(c, more);
   auto cta_of = [&](uint32_t y) { return y < more * (share + 1) ? y / (share + 1) : more + (y - more * (share + 1)) / share; };
   int seq = 0;
   uint32_t seq_begin = 0;
   for (int s0 = 0; s0 < p.t.n_seqs; s0 += 32) {
-    if (p.t.n_seqs > 32) sums = sum_up(work_of(s0 + lane));
-    const unsigned here = __ballot_sync(0xffffffffu, x < seq_begin + sums);
+    if (p.t.n_seqs > 32) sums = sums_of(s0 + lane);
+    const uint32_t upto = sums.rounds + extra * sums.units;
+    const unsigned here = __ballot_sync(0xffffffffu, x < seq_begin + upto);
     if (here) {
       const int l = __ffs(here) - 1;
       seq = s0 + l;
-      if (l) seq_begin += __shfl_sync(0xffffffffu, sums, l - 1);
+      if (l) seq_begin += __shfl_sync(0xffffffffu, upto, l - 1);
       break;
     }
-    seq_begin += __shfl_sync(0xffffffffu, sums, 31);
+    seq_begin += __shfl_sync(0xffffffffu, upto, 31);
   }
   SeqPlace sp = place_of_seq(p, seq);
   uint32_t n_issued = 0, n_used = 0;                     // this warp's blocks so far: stage and phase
@@ -172,18 +181,22 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
 #pragma unroll 1
   while (x < x_end) {
     // ---- the next unit of it ----
-    while (x >= seq_begin + units_of(sp) * rounds_of(sp)) {
-      seq_begin += units_of(sp) * rounds_of(sp);
+    uint32_t cost = rounds_of(sp) + extra;
+    while (x >= seq_begin + units_of(sp) * cost) {
+      seq_begin += units_of(sp) * cost;
       if (++seq >= p.t.n_seqs) return;                     // (sums of tables that contradict themselves)
       sp = place_of_seq(p, seq);
+      cost = rounds_of(sp) + extra;
     }
-    const uint32_t rounds = rounds_of(sp), in_seq = (x - seq_begin) / rounds, unit_begin = seq_begin + in_seq * rounds, unit_end = unit_begin + rounds, end = min(unit_end, x_end);
-    const int tile = in_seq / p.n_kv, kvh = in_seq - tile * p.n_kv;
+    const uint32_t in_seq = (x - seq_begin) / cost, unit_begin = seq_begin + in_seq * cost, unit_end = unit_begin + cost, end = min(unit_end, x_end);
+    const uint32_t from = x - unit_begin <= extra ? 0 : x - unit_begin - extra, to_round = end - unit_begin <= extra ? 0 : end - unit_begin - extra;
+    if (to_round == 0) return;                             // the share ends in what it takes to begin: the next CTA begins there
+    const int tile = p.by_kv.div(in_seq), kvh = in_seq - tile * p.n_kv;
     const TilePlace w = tile_of_seq<R>(p, seq, sp, tile);
-    const int k_begin = (x - unit_begin) * ROUND, k_end = min((uint32_t)w.keys, (end - unit_begin) * ROUND), pairs = w.n * p.group;      // (rounds x 64 < 2^31 + 64)
+    const int k_begin = from * ROUND, k_end = min((uint32_t)w.keys, to_round * ROUND), pairs = w.n * p.group;      // (rounds x 64 < 2^31 + 64)
     const int blocks = max(0, (k_end - k_begin + KB - 1) / KB), mine = (blocks - warp + RW - 1) / RW;      // this warp's: warp, warp + RW, ...
     auto block_key = [&](int it) { return k_begin + (warp + it * RW) * KB; };
-    auto page_id = [&](int it) { return whole && it < mine ? p.t.pages[(int64_t)seq * p.t.table_stride + block_key(it) / ps] : -1; };
+    auto page_id = [&](int it) { return whole && it < mine ? p.t.pages[(int64_t)seq * p.t.table_stride + p.by_page.div(block_key(it))] : -1; };
     int ids = page_id(lane), ids_next = mine > 32 ? page_id(32 + lane) : 0;      // pages of this and the next 32 blocks
 
     // the queries, four rows a warp: all loads, then (behind the first blocks' copies) a power of two that keeps a row in fp16's range (N == 2) and their parts
@@ -193,7 +206,7 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
       bool live[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        const int pair = w.r0 + warp * 4 + i, token = pair / p.group;
+        const int pair = w.r0 + warp * 4 + i, token = p.by_group.div(pair);
         live[i] = pair < pairs && lane < D / 2;
         at[i] = (w.first_row + token) * p.q_stride + (kvh * p.group + pair - token * p.group) * D + lane * 2;
       }
@@ -241,12 +254,12 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
           if (lane < D / 32) {      // a lane a box: keys' sub-blocks, values' sub-blocks
             const int sub = lane % (D / 64);
             asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-                         ::"r"(to + lane * (KB * 128)), "l"(lane < D / 64 ? &tm_k : &tm_v), "r"(bar), "r"(sub * 64), "r"(key0 % ps), "r"(kvh), "r"(page) : "memory");
+                         ::"r"(to + lane * (KB * 128)), "l"(lane < D / 64 ? &tm_k : &tm_v), "r"(bar), "r"(sub * 64), "r"(key0 - p.by_page.div(key0) * ps), "r"(kvh), "r"(page) : "memory");
           }
         } else {
           const uint16_t* kp = static_cast<const uint16_t*>(p.k) + kvh * p.head_stride;
           const uint16_t* vp = static_cast<const uint16_t*>(p.v) + kvh * p.head_stride;
-          const int64_t at0 = page >= 0 ? page * p.page_stride + (int64_t)(key0 % ps) * p.row_stride : 0;
+          const int64_t at0 = page >= 0 ? page * p.page_stride + (int64_t)(key0 - p.by_page.div(key0) * ps) * p.row_stride : 0;
 #pragma unroll
           for (int i = 0; i < (KB * CH + 31) / 32; i++) {
             const int ch = lane + i * 32, r = ch / CH, col = ch % CH;
@@ -270,7 +283,7 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
     float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < D / 8; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    const int first_last = w.length + w.r0 / p.group;      // what the tile's first row sees: blocks up to it are seen by all
+    const int first_last = w.length + p.by_group.div(w.r0);      // what the tile's first row sees: blocks up to it are seen by all
 #pragma unroll 1
     for (int it = 1 - ST; it < max(mine, 1); it++) {       // (one copy of the loop's code: what a short call waits for is instructions)
       if (it == 0) {
@@ -307,7 +320,7 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           const int pair = w.r0 + g + e * 8;
-          last[e] = pair < pairs ? w.length + pair / p.group : -1;
+          last[e] = pair < pairs ? w.length + p.by_group.div(pair) : -1;
           qs[e] = s_scale[g + e * 8];
         }
         if (mine <= 0) break;
@@ -450,9 +463,9 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
       for (int n = 0; n < D / 8; n++) *reinterpret_cast<float2*>(s_o + (warp * R + r) * D + n * 8 + tq * 2) = make_float2(l[e] == 0.f ? 0.f : o[n][e * 2] * cw, l[e] == 0.f ? 0.f : o[n][e * 2 + 1] * cw);
     }
     __syncthreads();
-    const int c_first = cta_of(unit_begin), n_parts = cta_of(unit_end - 1) - c_first + 1;
+    const int c_first = cta_of(unit_begin + extra), n_parts = cta_of(unit_end - 1) - c_first + 1;
     auto place = [&](int cta, bool first) { return p.parts + (cta * 2 + first) * PART<R, D>; };
-    float* const part = place(c, x == unit_begin);
+    float* const part = place(c, from == 0);
 #pragma unroll 1
     for (int i = tid; i < R * D / 4; i += R_THREADS) {
       const int r = i / (D / 4), d = (i - r * (D / 4)) * 4, pair = w.r0 + r;
@@ -468,7 +481,7 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
         v[0] += y.x; v[1] += y.y; v[2] += y.z; v[3] += y.w;
       }
       if (n_parts == 1) {
-        const int token = pair / p.group;
+        const int token = p.by_group.div(pair);
         const int64_t at = (w.first_row + token) * p.out_stride + (kvh * p.group + pair - token * p.group) * D + d;
 #pragma unroll
         for (int j = 0; j < 4; j++) store_as(p.out, p.out_dtype, at + j, sum == 0.f ? 0.f : v[j] / sum);

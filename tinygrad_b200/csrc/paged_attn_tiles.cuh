@@ -22,7 +22,7 @@ template <int D, int N> constexpr int T_VS = D == 64 ? 3 : N == 1 ? 3 : 2;
 template <int D, int N> constexpr int T_SMEM = (2 * N + T_KS<D, N> + T_VS<D, N>) * T_TILE<D> + 1024;
 
 struct SharedA {
-  uint64_t k_full[3], k_empty[3], v_full[3], v_clean[3], v_empty[3], s_full[2], p_full[2], q_full, o_full;
+  uint64_t k_full[3], k_empty[3], v_full[3], v_clean[3], v_empty[3], s_full[2], p_full[2][2], q_full, o_full;
   uint32_t tmem;
   int abort, flag, bad_lo, bad_hi;
 };
@@ -85,6 +85,35 @@ __device__ __forceinline__ void load64(const void* base, int type, int64_t i, bo
   }
 }
 
+template <bool V> struct Switch { static constexpr bool value = V; };
+// two fp32 values at a time
+__device__ __forceinline__ uint64_t pair_of(float a, float b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ float2 floats_of(uint64_t r) { float2 f; asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(r)); return f; }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }      // NaN if one is
+// 2^x of two values without the special-function units: x = n + f, n the nearest integer, 2^f by a polynomial fitted to it on [-1/2, 1/2] (least largest relative error: degree 3 2^-13.7, for
+// probabilities that bf16 rounds by 2^-9; degree 4 2^-18.5, fp16 2^-12), n added to the exponent.  Below 2^-126: 2^-126.
+template <bool BF>
+__device__ __forceinline__ uint64_t pow2_poly(uint64_t x) {
+  const float2 c = floats_of(x);
+  x = pair_of(fmaxf(c.x, -126.f), fmaxf(c.y, -126.f));
+  const uint64_t t = add2(x, pair_of(12582912.f, 12582912.f)), n = add2(t, pair_of(-12582912.f, -12582912.f)), f = fma2(n, pair_of(-1.f, -1.f), x);      // 1.5 x 2^23: t ends in n
+  uint64_t y;
+  if constexpr (BF) {
+    y = fma2(pair_of(0.055171665f, 0.055171665f), f, pair_of(0.24261113f, 0.24261113f));
+    y = fma2(y, f, pair_of(0.69326097f, 0.69326097f));
+    y = fma2(y, f, pair_of(0.99992806f, 0.99992806f));
+  } else {
+    y = fma2(pair_of(0.009570101f, 0.009570101f), f, pair_of(0.05591786f, 0.05591786f));
+    y = fma2(y, f, pair_of(0.24024744f, 0.24024744f));
+    y = fma2(y, f, pair_of(0.6931218f, 0.6931218f));
+    y = fma2(y, f, pair_of(0.9999993f, 0.9999993f));
+  }
+  const float2 tn = floats_of(t), yf = floats_of(y);
+  return pair_of(__uint_as_float(__float_as_uint(yf.x) + (__float_as_uint(tn.x) << 23)), __uint_as_float(__float_as_uint(yf.y) + (__float_as_uint(tn.y) << 23)));
+}
+
 struct RowOf { int64_t row, head; int last; bool live; };      // of a thread: its row of the arrays, its head, the position it sees up to
 
 // What rows that see keys [lo, hi] with values that are not finite get of them (their finite values are in the products already).
@@ -109,16 +138,16 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int order = blockIdx.x / p.n_kv, kvh = blockIdx.x - order * p.n_kv, split = blockIdx.y;
-  const int tile_index = gridDim.x / p.n_kv - 1 - order;      // long ones first
+  const int order = p.by_kv.div(blockIdx.x), kvh = blockIdx.x - order * p.n_kv, split = blockIdx.y;
+  const int tile_index = p.by_kv.div(gridDim.x) - 1 - order;      // long ones first
   const TilePlace w = place_of_tile<T_R>(p, tile_index);
   if (w.n == 0) return;
   const int n_parts = max(1, (w.keys + p.split_len - 1) / p.split_len), k_begin = split * p.split_len, k_end = min(w.keys, k_begin + p.split_len);
   if (split >= n_parts) return;
   const int tiles = max(0, (k_end - k_begin + T_KEYS - 1) / T_KEYS);
-  const int64_t pairs = (int64_t)w.n * p.group;
+  const int pairs = w.n * p.group;
   const bool two = w.r0 + T_ROWS < pairs;                      // the second tile of rows has some
-  const int first_last = w.length + w.r0 / p.group;            // what the first row sees
+  const int first_last = w.length + p.by_group.div(w.r0);            // what the first row sees
   const uint32_t s_q = (s_addr(raw) + 1023) & ~1023u, s_k = s_q + 2 * N * TILE, s_v = s_k + KS * TILE;
 
   if (warp == 8) {
@@ -129,7 +158,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
     for (int i = 0; i < 3; i++) {
       a_bar_init(&sh.k_full[i], 1); a_bar_init(&sh.k_empty[i], 1); a_bar_init(&sh.v_full[i], 1); a_bar_init(&sh.v_clean[i], 2); a_bar_init(&sh.v_empty[i], 1);
     }
-    for (int i = 0; i < 2; i++) { a_bar_init(&sh.s_full[i], 1); a_bar_init(&sh.p_full[i], 4); }
+    for (int i = 0; i < 2; i++) { a_bar_init(&sh.s_full[i], 1); a_bar_init(&sh.p_full[i][0], 4); a_bar_init(&sh.p_full[i][1], 4); }
     a_bar_init(&sh.q_full, 8); a_bar_init(&sh.o_full, 1);
     sh.abort = sh.flag = 0; sh.bad_lo = INT32_MAX; sh.bad_hi = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -148,11 +177,11 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
     const int t = warp >> 2, r = tid & 127;
     RowOf me;
     {
-      const int64_t pair = w.r0 + t * T_ROWS + r;
+      const int pair = w.r0 + t * T_ROWS + r;
       me.live = pair < pairs;
-      const int token = me.live ? (int)(pair / p.group) : 0;
+      const int token = me.live ? p.by_group.div(pair) : 0;
       me.row = w.first_row + token;
-      me.head = kvh * p.group + (me.live ? pair - (int64_t)token * p.group : 0);
+      me.head = kvh * p.group + (me.live ? pair - token * p.group : 0);
       me.last = me.live ? w.length + token : -1;
     }
     float qs = p.scale;
@@ -226,18 +255,24 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
       const int lim = min(me.last, k_end - 1) - k0;
       float top = -INFINITY;
       if constexpr (N == 1) {
-        uint32_t s[128];
+        float s[128];
 #pragma unroll
-        for (int c = 0; c < 4; c++) ld32(ts + c * 32, s + c * 32);
+        for (int c = 0; c < 4; c++) ld32(ts + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
         wait_ld();
         if (masked) {
 #pragma unroll
-          for (int i = 0; i < 128; i++) s[i] = i <= lim ? s[i] : __float_as_uint(-INFINITY);
+          for (int i = 0; i < 128; i++) s[i] = i <= lim ? s[i] : -INFINITY;
         }
-        float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float tops[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-        for (int i = 0; i < 128; i++) tops[i & 3] = fmaxf(tops[i & 3], __uint_as_float(s[i]));
-        top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) * qs;
+        for (int i = 4; i < 124; i += 8) {
+#pragma unroll
+          for (int q = 0; q < 4; q++) tops[q] = max3(tops[q], s[i + q], s[i + 4 + q]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; q++) tops[q] = max3(tops[q], s[124 + q], s[124 + q]);
+        top = max3(tops[0], tops[1], max3(tops[2], tops[3], tops[3])) * qs;
+        if (!(top < INFINITY)) { l = __uint_as_float(0x7FC00000u); top = m; }      // a score that is infinite or NaN: the row is NaN, whatever takes its exponentials
         const bool moves = j == 0 || top > m + 8.f;
         if (__any_sync(0xffffffffu, moves)) {
           const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : pow2(m - mn);
@@ -256,19 +291,33 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
           }
         }
         const float sub = m == -INFINITY ? 0.f : T_BASE - m;
-        float sums[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t qs2 = pair_of(qs, qs), sub2 = pair_of(sub, sub);
+        uint64_t sums[2] = {0, 0};
+        auto powers = [&](auto some) {
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-          uint32_t pk[16];
+          for (int c = 0; c < 4; c++) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const float a = pow2(fmaf(__uint_as_float(s[c * 32 + 2 * i]), qs, sub)), b = pow2(fmaf(__uint_as_float(s[c * 32 + 2 * i + 1]), qs, sub));
-            sums[i & 3] += a + b;
-            pk[i] = pack2(a, b, BF ? B200Q_BF16 : B200Q_F16);
+            for (int i = 0; i < 16; i++) {
+              uint64_t x = fma2(pair_of(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), qs2, sub2);
+              if (some.value && i % 4 == 3) x = pow2_poly<BF>(x);
+              else { const float2 y = floats_of(x); x = pair_of(pow2(y.x), pow2(y.y)); }
+              sums[i & 1] = add2(sums[i & 1], x);
+              const float2 y = floats_of(x);
+              pk[i] = pack2(y.x, y.y, BF ? B200Q_BF16 : B200Q_F16);
+            }
+            st16(ts + c * 32, pk);
+            if (c & 1) {      // half of the tile's probabilities: the product begins with them
+              wait_st();
+              fence_before();
+              __syncwarp();
+              if (lane == 0) a_bar_arrive(&sh.p_full[t][c / 2]);
+            }
           }
-          st16(ts + c * 32, pk);
-        }
-        l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        };
+        if (masked) powers(Switch<false>{}); else powers(Switch<true>{});
+        const float2 y0 = floats_of(sums[0]), y1 = floats_of(sums[1]);
+        l += (y0.x + y0.y) + (y1.x + y1.y);
       } else {
         // the tile before: its weighted sum is complete (the scores behind it in the tensor core's queue are)
         if (j > 0) {
@@ -317,11 +366,11 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
           st32(ts + c * 32, pk);
         }
         l += sum;
+        wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) { a_bar_arrive(&sh.p_full[t][0]); a_bar_arrive(&sh.p_full[t][1]); }
       }
-      wait_st();
-      fence_before();
-      __syncwarp();
-      if (lane == 0) a_bar_arrive(&sh.p_full[t]);
     }
     if (ok && tiles) ok = __all_sync(0xffffffffu, a_wait(sh, &sh.o_full, 0));
     // ---- what comes out ----
@@ -405,15 +454,22 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
         const int vs = j % VS, kn = (j + 1) % KS;
         ok = a_wait(sh, &sh.v_clean[vs], (j / VS) & 1);
         for (int t = 0; ok && t < 1 + two; t++) {
-          ok = a_wait(sh, &sh.p_full[t], j & 1);
+          // N == 1: the probabilities come in two halves; N == 2: the parts one after the other, small ones first
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            ok = ok && a_wait(sh, &sh.p_full[t][h], j & 1);
+            if (!ok) break;
+            fence_after();
+            if (N == 2 && h == 1) break;
+#pragma unroll
+            for (int i = N - 1; i >= 0; i--)
+#pragma unroll
+              for (int k = 0; k < (N == 1 ? 4 : 8); k++) {
+                const int kk = N == 1 ? h * 4 + k : k;
+                mma_ts_a(tmem + 256 + t * 128, tmem + t * 128 + (kk / 2) * 32 + i * 16 + (kk & 1) * 8, desc_128(s_v + vs * TILE + kk * 2048, SUB), ID_O, i < N - 1 || kk > 0 || (N == 1 && j > 0));
+              }
+          }
           if (!ok) break;
-          fence_after();
-#pragma unroll
-          for (int i = N - 1; i >= 0; i--)
-#pragma unroll
-            for (int kk = 0; kk < T_KEYS / 16; kk++)
-              mma_ts_a(tmem + 256 + t * 128, tmem + t * 128 + (kk / 2) * 32 + i * 16 + (kk & 1) * 8, desc_128(s_v + vs * TILE + kk * 2048, SUB), ID_O,
-                       i < N - 1 || kk > 0 || (N == 1 && j > 0));
           if (t == two) a_commit(&sh.v_empty[vs]);
           if (j + 1 < tiles) {
             if (t == 0) { ok = a_wait(sh, &sh.k_full[kn], ((j + 1) / KS) & 1); if (!ok) break; fence_after(); }
@@ -436,10 +492,10 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
       const bool mine = pg < n_pages;
       int page = 0;
       if (mine) {
-        page = row_pages[(k0 + pg * box_rows) / ps];
+        page = row_pages[p.by_page.div(k0 + pg * box_rows)];
         if (page < 0 || page >= p.t.n_pages) { page = p.t.n_pages; atomicExch(&g_paged_attn_status, 2); }      // (outside the map: the box is filled with zeros)
       }
-      const int slot = (k0 + pg * box_rows) % ps;
+      const int slot = k0 + pg * box_rows - p.by_page.div(k0 + pg * box_rows) * ps;
 #pragma unroll
       for (int v = 0; v < 2; v++) {
         const int st = v ? j % VS : j % KS, use = v ? j / VS : j / KS;
