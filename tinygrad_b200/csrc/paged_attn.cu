@@ -324,7 +324,7 @@ Deal deal_of(const b200q_paged_cache* c, const b200q_paged_batch* b, int group, 
   const int few = FEW_PAIRS / group > 1 ? FEW_PAIRS / group : 1;
   d.many = tiles_take && b->max_new > few;
   if (d.many) {
-    d.plan[0] = make_plan(c, b, group, few, INT32_MAX, T_R, 148, 512, T_KEYS, 64);
+    d.plan[0] = make_plan(c, b, group, few, INT32_MAX, T_R, N_SM, 512, T_KEYS, T_PARTS);
     d.n = 1;
     if (b->n_seqs > 1) {
       d.plan[1] = rows_plan(c, b, group, 0, few);
@@ -435,6 +435,7 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
       static PerDeviceFlag allowed[2][2][2];
       if ((rc = allow_smem(kernel, smem, allowed[type][parts - 1][dim == 128])) != B200Q_OK) return rc;
       B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles * n_kv, plan.n_split), dim3(T_THREADS), (size_t)smem, st, pdl, p, boxes[2], boxes[3], box_rows_of(cache)));
+      if (plan.n_split > 1) B200Q_CHECK_CUDA(launch_k(dim == 64 ? join_tiles_kernel<64> : join_tiles_kernel<128>, dim3(plan.tiles * n_kv, T_R / J_ROWS), dim3(J_THREADS), 0, st, true, p));
       continue;
     }
     if (cache->dtype == B200Q_F32) {

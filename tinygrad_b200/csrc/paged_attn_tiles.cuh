@@ -15,7 +15,7 @@
 
 namespace {
 
-constexpr int T_ROWS = 128, T_R = 2 * T_ROWS, T_KEYS = 128, T_THREADS = 384, T_BASE = 7;      // probabilities up to 2^(7 + 8)
+constexpr int T_ROWS = 128, T_R = 2 * T_ROWS, T_KEYS = 128, T_THREADS = 384, T_BASE = 7, T_PARTS = 8;      // probabilities up to 2^(7 + 8)
 template <int D> constexpr int T_TILE = T_KEYS * D * 2;                                     // bytes of 128 rows of 16-bit values
 template <int D, int N> constexpr int T_KS = D == 64 ? 3 : N == 1 ? 2 : 1;
 template <int D, int N> constexpr int T_VS = D == 64 ? 3 : N == 1 ? 3 : 2;
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
   }
   if (tid == 0) {
     for (int i = 0; i < 3; i++) {
-      a_bar_init(&sh.k_full[i], 1); a_bar_init(&sh.k_empty[i], 1); a_bar_init(&sh.v_full[i], 1); a_bar_init(&sh.v_clean[i], 2); a_bar_init(&sh.v_empty[i], 1);
+      a_bar_init(&sh.k_full[i], 1); a_bar_init(&sh.k_empty[i], 1); a_bar_init(&sh.v_full[i], 1); a_bar_init(&sh.v_clean[i], 1); a_bar_init(&sh.v_empty[i], 1);
     }
     for (int i = 0; i < 2; i++) { a_bar_init(&sh.s_full[i], 1); a_bar_init(&sh.p_full[i][0], 4); a_bar_init(&sh.p_full[i][1], 4); }
     a_bar_init(&sh.q_full, 8); a_bar_init(&sh.o_full, 1);
@@ -481,63 +481,64 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
       a_commit(&sh.o_full);
       if (!ok) a_wait_on(s_addr(&sh.o_full), 0, s_addr(&sh.flag));      // products in flight are done before tensor memory goes back (flag is 0 here)
     }
-  } else if (warp == 9) {
-    // ---- keys and values: a lane a box ----
-    const int per_tile = T_KEYS / box_rows, ps = p.t.page_size, sub = lane % SUBS, pg = lane / SUBS;
+  } else if (warp < 11) {
+    // ---- keys (one warp), values (another): a lane a box ----
+    const bool v = warp == 10;
+    const int stages = v ? VS : KS, per_tile = T_KEYS / box_rows, ps = p.t.page_size, sub = lane % SUBS, pg = lane / SUBS;
+    const uint32_t to = (v ? s_v : s_k) + sub * SUB + pg * box_rows * 128;
+    uint64_t* const full = v ? sh.v_full : sh.k_full;
+    uint64_t* const empty = v ? sh.v_empty : sh.k_empty;
     const int32_t* row_pages = p.t.pages + (int64_t)w.seq * p.t.table_stride;
+    auto page_of = [&](int j) {
+      const int key = k_begin + j * T_KEYS + pg * box_rows;
+      return j < tiles && key < k_end && pg < per_tile ? row_pages[p.by_page.div(key)] : -1;
+    };
     bool ok = true;
-    int issued[2] = {0, 0};
-    for (int j = 0; ok && j < tiles; j++) {
-      const int k0 = k_begin + j * T_KEYS, n_pages = min(per_tile, (k_end - k0 + box_rows - 1) / box_rows);
+    int st = 0, use = 0, j = 0, next = page_of(0);
+    for (; j < tiles; j++) {
+      const int k0 = k_begin + j * T_KEYS, n_pages = min(per_tile, (k_end - k0 + box_rows - 1) / box_rows), slot = k0 + pg * box_rows - p.by_page.div(k0 + pg * box_rows) * ps;
       const bool mine = pg < n_pages;
-      int page = 0;
-      if (mine) {
-        page = row_pages[p.by_page.div(k0 + pg * box_rows)];
-        if (page < 0 || page >= p.t.n_pages) { page = p.t.n_pages; atomicExch(&g_paged_attn_status, 2); }      // (outside the map: the box is filled with zeros)
-      }
-      const int slot = k0 + pg * box_rows - p.by_page.div(k0 + pg * box_rows) * ps;
-#pragma unroll
-      for (int v = 0; v < 2; v++) {
-        const int st = v ? j % VS : j % KS, use = v ? j / VS : j / KS;
-        uint64_t* full = v ? &sh.v_full[st] : &sh.k_full[st];
-        if (use > 0) ok = ok && a_wait(sh, v ? &sh.v_empty[st] : &sh.k_empty[st], (use - 1) & 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(s_addr(full)), "r"(n_pages * SUBS * box_rows * 128) : "memory");
-        __syncwarp();
-        if (mine)
-          asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-                       ::"r"((v ? s_v : s_k) + st * TILE + sub * SUB + pg * box_rows * 128), "l"(v ? &tm_v : &tm_k), "r"(s_addr(full)), "r"(sub * 64), "r"(slot), "r"(kvh), "r"(page) : "memory");
-        __syncwarp();
-        issued[v] = j + 1;
-      }
+      int page = next;
+      next = page_of(j + 1);
+      if (mine && (page < 0 || page >= p.t.n_pages)) { page = p.t.n_pages; atomicExch(&g_paged_attn_status, 2); }      // (outside the map: the box is filled with zeros)
+      if (use > 0) ok = a_wait(sh, &empty[st], (use - 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      if (lane == 0) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(s_addr(&full[st])), "r"(n_pages * SUBS * box_rows * 128) : "memory");
+      __syncwarp();
+      if (mine)
+        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                     ::"r"(to + st * TILE), "l"(v ? &tm_v : &tm_k), "r"(s_addr(&full[st])), "r"(sub * 64), "r"(slot), "r"(kvh), "r"(page) : "memory");
+      __syncwarp();
+      if (++st == stages) { st = 0; use++; }
     }
-    if (!ok) {      // copies in flight end before the shared memory does
-      for (int x = max(0, issued[0] - KS); x < issued[0]; x++) a_wait_on(s_addr(&sh.k_full[x % KS]), (x / KS) & 1, s_addr(&sh.flag));
-      for (int x = max(0, issued[1] - VS); x < issued[1]; x++) a_wait_on(s_addr(&sh.v_full[x % VS]), (x / VS) & 1, s_addr(&sh.flag));
-    }
+    if (!ok)        // copies in flight end before the shared memory does
+      for (int x = max(0, j - stages); x < j; x++) a_wait_on(s_addr(&full[x % stages]), (x / stages) & 1, s_addr(&sh.flag));
   } else {
     // ---- values that a product must not see: rows behind the last key, and what is not finite in rows that not every query sees (0 times it is not 0) ----
-    const int half = warp - 10;
     bool ok = true;
-    for (int j = 0; ok && j < tiles; j++) {
-      const int st = j % VS, k0 = k_begin + j * T_KEYS;
-      ok = __all_sync(0xffffffffu, a_wait(sh, &sh.v_full[st], (j / VS) & 1));
+    int st = 0, use = 0;
+    for (int j = 0; j < tiles; j++) {
+      const int k0 = k_begin + j * T_KEYS;
+      ok = __all_sync(0xffffffffu, a_wait(sh, &sh.v_full[st], use & 1));
       if (!ok) break;
       const int from = max(0, min(first_last + 1, k_end) - k0);      // the first row that somebody does not see
       if (from < T_KEYS) {
         bool changed = false;
-        for (int i = from * 8 + half * 32 + lane; i < T_KEYS * 8; i += 64) {
+#pragma unroll 4
+        for (int i = from * 8 + lane; i < T_KEYS * 8; i += 32) {
           const int key = k0 + i / 8;
 #pragma unroll
           for (int s = 0; s < SUBS; s++) {
             const uint32_t a = s_v + st * TILE + s * SUB + i * 16;
-            if (key >= k_end) { st_s4(a, make_uint4(0, 0, 0, 0)); changed = true; continue; }
-            const uint4 x = ld_s4(a), y = make_uint4(finite_only<BF>(x.x), finite_only<BF>(x.y), finite_only<BF>(x.z), finite_only<BF>(x.w));
+            const uint4 x = ld_s4(a);
+            uint4 y = make_uint4(finite_only<BF>(x.x), finite_only<BF>(x.y), finite_only<BF>(x.z), finite_only<BF>(x.w));
+            const bool behind = key >= k_end;
+            if (behind) y = make_uint4(0, 0, 0, 0);
             if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
               st_s4(a, y);
               changed = true;
-              atomicMin(&sh.bad_lo, key); atomicMax(&sh.bad_hi, key);
+              if (!behind) { atomicMin(&sh.bad_lo, key); atomicMax(&sh.bad_hi, key); }
             }
           }
         }
@@ -545,6 +546,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
       }
       __syncwarp();
       if (lane == 0) a_bar_arrive(&sh.v_clean[st]);
+      if (++st == VS) { st = 0; use++; }
     }
     }
   }
@@ -552,9 +554,43 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
   __syncthreads();
   fence_after();
   if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
-  if (n_parts > 1 && !*(volatile int*)&sh.abort) {
-    const float* first = p.parts + (int64_t)unit * p.n_split * PART<T_R, D>;
-    join_parts<T_R, D, T_THREADS>(p, w, p.counters + unit, n_parts, kvh, &sh.flag, reinterpret_cast<float*>(raw), [&](int s) { return first + (int64_t)s * PART<T_R, D>; });
+}
+
+// The parts of tiles whose keys are split, added in the order of the keys: a CTA 32 rows of a (tile, KV head).
+constexpr int J_ROWS = 32, J_THREADS = 256;
+template <int D>
+__global__ void __launch_bounds__(J_THREADS) join_tiles_kernel(const AttnParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int order = p.by_kv.div(blockIdx.x), kvh = blockIdx.x - order * p.n_kv, tile_index = p.by_kv.div(gridDim.x) - 1 - order;
+  const TilePlace w = place_of_tile<T_R>(p, tile_index);
+  const int n_parts = (w.keys + p.split_len - 1) / p.split_len, end = min(T_R, w.n * p.group - w.r0);
+  if (w.n == 0 || n_parts <= 1) return;
+  const float* first = p.parts + (int64_t)(tile_index * p.n_kv + kvh) * p.n_split * PART<T_R, D>;
+  for (int i = threadIdx.x; i < J_ROWS * (D / 4); i += J_THREADS) {
+    const int r = blockIdx.y * J_ROWS + i / (D / 4), d = i % (D / 4) * 4, pair = w.r0 + r, token = p.by_group.div(pair);
+    if (r >= end) return;
+    float ms[T_PARTS], ls[T_PARTS], m = -INFINITY, sum = 0.f, o[4] = {};
+    float4 v[T_PARTS];
+#pragma unroll
+    for (int q = 0; q < T_PARTS; q++) {
+      const float* b = first + (int64_t)min(q, n_parts - 1) * PART<T_R, D>;
+      ms[q] = __ldcg(b + r);
+      ls[q] = __ldcg(b + T_R + r);
+      v[q] = __ldcg(reinterpret_cast<const float4*>(b + 2 * T_R + r * D + d));
+    }
+#pragma unroll
+    for (int q = 0; q < T_PARTS; q++) m = fmaxf(m, ms[q]);
+#pragma unroll
+    for (int q = 0; q < T_PARTS; q++) {
+      if (q >= n_parts) break;
+      const float f = ls[q] == 0.f ? 0.f : pow2(ms[q] - m);      // (a part without keys has sum 0)
+      sum = fmaf(f, ls[q], sum);
+      o[0] = fmaf(f, v[q].x, o[0]); o[1] = fmaf(f, v[q].y, o[1]); o[2] = fmaf(f, v[q].z, o[2]); o[3] = fmaf(f, v[q].w, o[3]);
+    }
+    const int64_t at = (w.first_row + token) * p.out_stride + (int64_t)(kvh * p.group + pair - token * p.group) * D + d;
+#pragma unroll
+    for (int j = 0; j < 4; j++) store_as(p.out, p.out_dtype, at + j, sum == 0.f ? 0.f : o[j] / sum);
   }
 }
 
