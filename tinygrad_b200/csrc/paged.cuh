@@ -48,19 +48,26 @@ struct PagedTables {
   int n_seqs, table_stride, n_rows, max_new, max_len, n_pages, page_size;
 };
 
-// The sequence of a row, by a whole warp: the number of sequences that end at or before it.  One token of every sequence is the usual case: asked first.
-__device__ __forceinline__ int seq_of_row(const PagedTables& t, int row) {
-  const int lane = threadIdx.x & 31, guess = min(row, t.n_seqs - 1);
-  const int g0 = t.row_off[guess], g1 = t.row_off[guess + 1];
-  if (g0 <= row && row < g1) return guess;
-  int seq = 0;
-  for (int s0 = 0; s0 < t.n_seqs; s0 += 32) {
-    const bool before = s0 + lane < t.n_seqs && t.row_off[s0 + lane + 1] <= row;
-    const int c = __popc(__ballot_sync(0xffffffffu, before));
-    seq += c;
-    if (c < 32) break;
+// The sequence of a row, its rows and its length, by a whole warp; begin > row: of no sequence.  One token of every sequence is the usual case of large batches and asked first; up to 32 sequences are
+// asked all at once, so that this is one load's latency either way.
+struct SeqOfRow { int seq, begin, end, length; };
+__device__ __forceinline__ SeqOfRow seq_of_row(const PagedTables& t, int row) {
+  const int lane = threadIdx.x & 31;
+  if (t.n_seqs > 32) {
+    const int g = min(row, t.n_seqs - 1);
+    const SeqOfRow w{g, t.row_off[g], t.row_off[g + 1], t.length[g]};
+    if (w.begin <= row && row < w.end) return w;
   }
-  return min(seq, t.n_seqs - 1);
+  for (int s0 = 0; s0 < t.n_seqs; s0 += 32) {
+    int b = 0, e = 0, l = 0;
+    if (s0 + lane < t.n_seqs) { b = t.row_off[s0 + lane]; e = t.row_off[s0 + lane + 1]; l = t.length[s0 + lane]; }
+    const unsigned here = __ballot_sync(0xffffffffu, b <= row && row < e);
+    if (here) {
+      const int src = __ffs(here) - 1;
+      return SeqOfRow{s0 + src, __shfl_sync(0xffffffffu, b, src), __shfl_sync(0xffffffffu, e, src), __shfl_sync(0xffffffffu, l, src)};
+    }
+  }
+  return SeqOfRow{0, INT32_MAX, 0, 0};
 }
 
 // ---- checks of what all entry points take ----

@@ -16,33 +16,43 @@ from .runtime import DeviceBuffer, ptr_of, stream_ptr, synchronize
 DTYPES = {"float32": F32, "float16": F16, "bfloat16": BF16}
 _NP = {F32: np.float32, F16: np.float16, BF16: np.uint16}
 _SIZE = {F32: 4, F16: 2, BF16: 2}
+_TYPE = {**DTYPES, **{t: t for t in _SIZE}}
+# The calls of a decode step are as long as what Python does for them: types are looked up, not taken apart, and the library's entries are bound once.
+_entry = {}
+WORKSPACE_HEAD = 16384      # bytes of b200q_paged_attention's workspace that begin as zeros
+
+
+def _fn(name: str):
+  f = _entry.get(name)
+  if f is None: f = _entry[name] = getattr(_lib.load(), name)
+  return f
 
 
 def _dtype(d) -> int:
-  t = DTYPES.get(d, d)
-  if not isinstance(t, int) or t not in _SIZE: raise ValueError(f"unknown element type {d!r}: float32, float16 or bfloat16")
+  t = _TYPE.get(d)
+  if t is None: raise ValueError(f"unknown element type {d!r}: float32, float16 or bfloat16")
   return t
 
 
 def _ptr(o) -> int:
+  if type(o) is DeviceBuffer: return o.ptr
   try: return o.data_ptr()
   except AttributeError: return ptr_of(o)
 
 
-def _nbytes(o):      # None: not known (a raw address)
-  if o is None or isinstance(o, int): return None
-  n = getattr(o, "nbytes", None)
-  return n if isinstance(n, int) else None
+def _short(o, nbytes: int, what: str) -> None:
+  have = getattr(o, "nbytes", None)      # (a raw address says nothing)
+  if type(have) is int and have < nbytes: raise ValueError(f"{what} has {have} bytes, needs {nbytes}")
 
 
-def _holds(o, nbytes: int, what: str) -> None:
-  have = _nbytes(o)
-  if have is not None and have < nbytes: raise ValueError(f"{what} has {have} bytes, needs {nbytes}")
+_words = set()     # types that have been seen to be int32
 
 
 def _int32(o, what: str):
-  d = str(getattr(o, "dtype", "int32"))
-  if not d.endswith("int32") or d.endswith("uint32"): raise TypeError(f"{what} is a table of int32, got {d}")
+  t = getattr(o, "dtype", None)
+  if t is not None and t not in _words:
+    if not str(t).endswith("int32") or str(t).endswith("uint32"): raise TypeError(f"{what} is a table of int32, got {t}")
+    _words.add(t)
   return o
 
 
@@ -57,7 +67,7 @@ class PagedCache:
     if min(self.strides) < head_dim: raise ValueError(f"strides {self.strides} are shorter than a head")
     last = (n_pages - 1) * page + (n_kv_heads - 1) * head + (page_size - 1) * row + head_dim
     if k is None: k, v = (DeviceBuffer.empty((last,), _NP[self.dtype], zero=True) for _ in range(2))
-    _holds(k, last * _SIZE[self.dtype], "k"), _holds(v, last * _SIZE[self.dtype], "v")
+    _short(k, last * _SIZE[self.dtype], "k"), _short(v, last * _SIZE[self.dtype], "v")
     self.k, self.v = k, v
     self.desc = _lib.PagedCacheDesc(_ptr(k), _ptr(v), self.dtype, n_pages, page_size, n_kv_heads, head_dim, page, head, row)
     self.ref, self._key = ctypes.byref(self.desc), (self.dtype, page_size, n_kv_heads, head_dim)
@@ -77,17 +87,18 @@ class PagedBatch:
     self.n_seqs, self.n_rows, self.max_new, self.max_len = n_seqs, n_rows, max_new, max_len
     self.desc = _lib.PagedBatchDesc(_ptr(row_off), _ptr(length), _ptr(pages), n_seqs, table, n_rows, max_new, max_len)
     self.ref = ctypes.byref(self.desc)
-    self._ws, self._need, self._old = None, {}, []
+    self._ws, self._ready, self._old = None, set(), []
 
   def reserve(self, cache: PagedCache, n_heads: int, q_dtype="float32") -> None:
     """Allocates the workspace that `attention` needs for such a cache (done by its first call otherwise; a call under capture allocates nothing)."""
     _dtype(q_dtype)
-    need = self._need.get((cache._key, n_heads))
-    if need is None: need = self._need[(cache._key, n_heads)] = _lib.load().b200q_paged_attention_workspace_bytes(cache.ref, self.ref, n_heads)
+    need = _fn("b200q_paged_attention_workspace_bytes")(cache.ref, self.ref, n_heads)
     if need and (self._ws is None or self._ws.nbytes < need):
       if self._ws is not None: self._old.append(self._ws)      # graphs may hold it
-      self._ws = DeviceBuffer(need, zero=True)
+      self._ws = DeviceBuffer(need)
+      check(_lib.load().b200q_memset(self._ws.ptr, 0, WORKSPACE_HEAD, None))
       synchronize()
+    self._ready.add((cache._key, n_heads))
 
 
 def append(cache: PagedCache, batch: PagedBatch, x, q, n_heads: int, x_dtype="float32", q_dtype=None, rope=None, q_norm=None, k_norm=None, norm_eps: float = 0.0, x_stride: int = 0,
@@ -99,12 +110,13 @@ def append(cache: PagedCache, batch: PagedBatch, x, q, n_heads: int, x_dtype="fl
   n, d = batch.n_rows, cache.head_dim
   if n:
     row, q_row = (n_heads + 2 * cache.n_kv_heads) * d, n_heads * d
-    _holds(x, ((n - 1) * (x_stride or row) + row) * _SIZE[xt], "x"), _holds(q, ((n - 1) * (q_stride or q_row) + q_row) * _SIZE[qt], "q")
-  _check_norm(q_norm, d), _check_norm(k_norm, d)
-  rope_len, rope_dim = rope.shape if rope is not None else (0, 0)
-  a = _lib.PagedAppendArgs(_ptr(x), _ptr(q), xt, qt, x_stride, q_stride, n_heads, norm_eps, _ptr(q_norm) if q_norm is not None else None, _ptr(k_norm) if k_norm is not None else None,
-                           _ptr(rope) if rope is not None else None, rope_dim, rope_len)
-  check(_lib.load().b200q_paged_append(cache.ref, batch.ref, ctypes.byref(a), flags, stream_ptr(stream)))
+    _short(x, ((n - 1) * (x_stride or row) + row) * _SIZE[xt], "x")
+    _short(q, ((n - 1) * (q_stride or q_row) + q_row) * _SIZE[qt], "q")
+  rope_len, rope_dim = (0, 0) if rope is None else rope.shape
+  a = _lib.PagedAppendArgs(_ptr(x), _ptr(q), xt, qt, x_stride, q_stride, n_heads, norm_eps, None if q_norm is None else _norm(q_norm, d), None if k_norm is None else _norm(k_norm, d),
+                           None if rope is None else _ptr(rope), rope_dim, rope_len)
+  rc = _fn("b200q_paged_append")(cache.ref, batch.ref, ctypes.byref(a), flags, 0 if stream is None else stream_ptr(stream))
+  if rc: check(rc)
 
 
 def attention(cache: PagedCache, batch: PagedBatch, q, out, n_heads: int, q_dtype="float32", out_dtype=None, scale: float = 0.0, q_stride: int = 0, out_stride: int = 0, flags: int = 0,
@@ -115,18 +127,25 @@ def attention(cache: PagedCache, batch: PagedBatch, q, out, n_heads: int, q_dtyp
   n = batch.n_rows
   if n:
     row = n_heads * cache.head_dim
-    _holds(q, ((n - 1) * (q_stride or row) + row) * _SIZE[qt], "q"), _holds(out, ((n - 1) * (out_stride or row) + row) * _SIZE[ot], "out")
-  batch.reserve(cache, n_heads)
+    _short(q, ((n - 1) * (q_stride or row) + row) * _SIZE[qt], "q")
+    _short(out, ((n - 1) * (out_stride or row) + row) * _SIZE[ot], "out")
+  if (cache._key, n_heads) not in batch._ready: batch.reserve(cache, n_heads)
   ws = batch._ws
-  a = _lib.PagedAttnArgs(_ptr(q), _ptr(out), qt, ot, q_stride, out_stride, n_heads, scale, ws.ptr if ws is not None else None, ws.nbytes if ws is not None else 0)
-  check(_lib.load().b200q_paged_attention(cache.ref, batch.ref, ctypes.byref(a), flags, stream_ptr(stream)))
+  a = _lib.PagedAttnArgs(_ptr(q), _ptr(out), qt, ot, q_stride, out_stride, n_heads, scale, *((None, 0) if ws is None else (ws.ptr, ws.nbytes)))
+  rc = _fn("b200q_paged_attention")(cache.ref, batch.ref, ctypes.byref(a), flags, 0 if stream is None else stream_ptr(stream))
+  if rc: check(rc)
 
 
-def _check_norm(w, d: int) -> None:
-  if w is None: return
-  t = str(getattr(w, "dtype", "float16"))
-  if not t.endswith("float16") or t.endswith("bfloat16"): raise TypeError(f"norm weights are float16, got {t}")
-  _holds(w, 2 * d, "a norm weight")
+_half = set()      # types that have been seen to be float16
+
+
+def _norm(w, d: int) -> int:
+  t = getattr(w, "dtype", None)
+  if t is not None and t not in _half:
+    if not str(t).endswith("float16") or str(t).endswith("bfloat16"): raise TypeError(f"norm weights are float16, got {t}")
+    _half.add(t)
+  _short(w, 2 * d, "a norm weight")
+  return _ptr(w)
 
 
 def head_norm_rope(x, out, n_rows: int, n_heads: int, n_kv_heads: int, head_dim: int, x_dtype="float32", out_dtype=None, q_norm=None, k_norm=None, norm_eps: float = 0.0, rope=None,
@@ -137,10 +156,11 @@ def head_norm_rope(x, out, n_rows: int, n_heads: int, n_kv_heads: int, head_dim:
   ot = xt if out_dtype is None else _dtype(out_dtype)
   row = (n_heads + n_kv_heads) * head_dim
   if n_rows > 0:
-    _holds(x, ((n_rows - 1) * (x_stride or row) + row) * _SIZE[xt], "x"), _holds(out, ((n_rows - 1) * (out_stride or row) + row) * _SIZE[ot], "out")
-    if positions is not None: _holds(_int32(positions, "positions"), 4 * n_rows, "positions")
-  _check_norm(q_norm, head_dim), _check_norm(k_norm, head_dim)
-  rope_len, rope_dim = rope.shape if rope is not None else (0, 0)
-  a = _lib.HeadNormArgs(_ptr(x), _ptr(out), xt, ot, x_stride, out_stride, n_rows, n_heads, n_kv_heads, head_dim, norm_eps, _ptr(q_norm) if q_norm is not None else None,
-                        _ptr(k_norm) if k_norm is not None else None, _ptr(rope) if rope is not None else None, rope_dim, rope_len, _ptr(positions) if positions is not None else None)
-  check(_lib.load().b200q_head_norm_rope(ctypes.byref(a), flags, stream_ptr(stream)))
+    _short(x, ((n_rows - 1) * (x_stride or row) + row) * _SIZE[xt], "x")
+    _short(out, ((n_rows - 1) * (out_stride or row) + row) * _SIZE[ot], "out")
+    if positions is not None: _short(_int32(positions, "positions"), 4 * n_rows, "positions")
+  rope_len, rope_dim = (0, 0) if rope is None else rope.shape
+  a = _lib.HeadNormArgs(_ptr(x), _ptr(out), xt, ot, x_stride, out_stride, n_rows, n_heads, n_kv_heads, head_dim, norm_eps, None if q_norm is None else _norm(q_norm, head_dim),
+                        None if k_norm is None else _norm(k_norm, head_dim), None if rope is None else _ptr(rope), rope_dim, rope_len, None if positions is None else _ptr(positions))
+  rc = _fn("b200q_head_norm_rope")(ctypes.byref(a), flags, 0 if stream is None else stream_ptr(stream))
+  if rc: check(rc)
