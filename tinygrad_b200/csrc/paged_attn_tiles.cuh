@@ -32,17 +32,19 @@ __device__ __forceinline__ void a_commit(uint64_t* b) { asm volatile("tcgen05.co
 
 // Operands in the 128-byte-swizzle layout: sub-tiles of 64 values (128 bytes) a row, 8 rows = 1024 bytes.  Q and K are read along a row (rows 1024 bytes per 8 apart); V, whose reduction runs over
 // its rows, across them: then the distance between sub-tiles stands in the other field.
-__device__ __forceinline__ uint64_t desc_128(uint32_t addr, uint32_t other) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(other >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
+// A descriptor's low word (start, the other distance); the high one is the same for all.  Steps along an operand are added to the low word (16 bytes), so that the issuing thread has few values to keep.
+constexpr uint32_t DESC_HI = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_128(uint32_t addr, uint32_t other) { return ((addr >> 4) & 0x3FFF) | (other >> 4) << 16; }
 template <bool BF, bool ACROSS> __host__ __device__ constexpr uint32_t idesc_of(int n) {
   return 1u << 4 | (BF ? 1u << 7 | 1u << 10 : 0u) | (ACROSS ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (uint32_t)(T_ROWS >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss_a(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+__device__ __forceinline__ void mma_ss_a(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n.reg .pred p;\n.reg .b64 x, y;\nmov.b64 x, {%1, %5};\nmov.b64 y, {%2, %5};\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}"
+               ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(DESC_HI) : "memory");
 }
-__device__ __forceinline__ void mma_ts_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+__device__ __forceinline__ void mma_ts_a(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile("{\n.reg .pred p;\n.reg .b64 y;\nmov.b64 y, {%2, %5};\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}"
+               ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(DESC_HI) : "memory");
 }
 __device__ __forceinline__ void ld32(uint32_t a, uint32_t* v) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -55,6 +57,15 @@ __device__ __forceinline__ void st32(uint32_t a, const uint32_t* v) {
                ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]),
                  "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]),
                  "r"(v[29]), "r"(v[30]), "r"(v[31]) : "memory");
+}
+__device__ __forceinline__ void ld16(uint32_t a, uint32_t* v) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+                 "=r"(v[14]), "=r"(v[15]) : "r"(a));
+}
+__device__ __forceinline__ void st8(uint32_t a, const uint32_t* v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
 }
 __device__ __forceinline__ void st16(uint32_t a, const uint32_t* v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
@@ -69,20 +80,6 @@ __device__ __forceinline__ uint4 ld_s4(uint32_t a) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
   return v;
-}
-
-// 64 values from element i on, as fp32 (all loads before the first use)
-__device__ __forceinline__ void load64(const void* base, int type, int64_t i, bool wide, float (&f)[64]) {
-  if (wide && type == B200Q_F32) {
-    float4 x[16];
-#pragma unroll
-    for (int c = 0; c < 16; c++) x[c] = reinterpret_cast<const float4*>(static_cast<const float*>(base) + i)[c];
-#pragma unroll
-    for (int c = 0; c < 16; c++) { f[c * 4] = x[c].x; f[c * 4 + 1] = x[c].y; f[c * 4 + 2] = x[c].z; f[c * 4 + 3] = x[c].w; }
-  } else {
-#pragma unroll
-    for (int c = 0; c < 64; c++) f[c] = load_as_f(base, type, i + c);
-  }
 }
 
 template <bool V> struct Switch { static constexpr bool value = V; };
@@ -116,16 +113,21 @@ __device__ __forceinline__ uint64_t pow2_poly(uint64_t x) {
 
 struct RowOf { int64_t row, head; int last; bool live; };      // of a thread: its row of the arrays, its head, the position it sees up to
 
-// What rows that see keys [lo, hi] with values that are not finite get of them (their finite values are in the products already).
-template <int D, bool BF>
-__device__ __forceinline__ void add_not_finite(const AttnParams& p, int seq, int kvh, int lo, int hi, int d0, float* o) {
+// What a row that sees keys [lo, hi] with values that are not finite gets of them (their finite values are in the products already): added to its 32 columns from d0 on, which wait in shared memory.
+template <bool BF>
+__device__ __forceinline__ void add_not_finite(const AttnParams& p, int seq, int kvh, int lo, int hi, int d0, uint32_t row, int swizzle) {
+#pragma unroll 1
   for (int key = lo; key <= hi; key++) {
     const int64_t at = key_at(p, seq, key);
     if (at < 0) continue;
     const uint16_t* v = static_cast<const uint16_t*>(p.v) + kvh * p.head_stride + at + d0;
+#pragma unroll 1
     for (int d = 0; d < 32; d++) {
-      const uint32_t x = v[d];
-      if (finite_only<BF>(x) != x) o[d] += unpack2(x, BF).x;
+      const uint32_t x = v[d], a = row + (((d >> 2) ^ swizzle) << 4) + (d & 3) * 4;
+      if (finite_only<BF>(x) == x) continue;
+      float y;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(a) : "memory");
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(y + unpack2(x, BF).x) : "memory");
     }
   }
 }
@@ -186,51 +188,75 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
     }
     float qs = p.scale;
     if (t == 0 || two) {
-      // its row of queries: N parts, chunks of 16 bytes in the swizzled places
-      const int64_t at = me.row * p.q_stride + me.head * D;
-      const uint32_t to = s_q + t * TILE + r * 128;
-      const int size = type_size(p.q_dtype);
+      // the warp's 32 rows of queries, whole rows at a time: N parts, chunks of 16 bytes in the swizzled places.  PER values a lane.
+      constexpr int PER = N == 1 ? 8 : 4, LANES = D / PER, AT_ONCE = 32 / LANES;
+      const int size = type_size(p.q_dtype), l = lane % LANES;
       const bool wide = (((uintptr_t)p.q | (uintptr_t)(p.q_stride * size)) & 15) == 0;
-      float up = 1.f;
-      if constexpr (N == 2) {
-        float amax = 0.f, down;
+      auto row_at = [&](int i) {      // where this lane's values of the i-th run of rows are; -1: no row
+        const int pair = w.r0 + t * T_ROWS + (warp & 3) * 32 + i * AT_ONCE + lane / LANES, token = p.by_group.div(pair);
+        return pair < pairs ? (w.first_row + token) * p.q_stride + (int64_t)(kvh * p.group + pair - token * p.group) * D + l * PER : (int64_t)-1;
+      };
+      auto place = [&](int i, int part) {      // and where they go
+        const int row = (warp & 3) * 32 + i * AT_ONCE + lane / LANES, chunk = l * PER / 8;
+        return s_q + (part * 2 + t) * TILE + (chunk >> 3) * SUB + row * 128 + (((chunk & 7) ^ (row & 7)) << 4) + (PER == 4 ? (l & 1) * 8 : 0);
+      };
+      if constexpr (N == 1) {
+        constexpr int RUNS = 32 / AT_ONCE;
+        if (wide) {
 #pragma unroll 1
-        for (int b = 0; me.live && b < D; b += 64) {
-          float f[64];
-          load64(p.q, p.q_dtype, at + b, wide, f);
+          for (int i0 = 0; i0 < RUNS; i0 += 8) {
+            uint4 v[8];
 #pragma unroll
-          for (int i = 0; i < 64; i++) amax = fmaxf(amax, fabsf(f[i]));
-        }
-        pow2_scale(amax, up, down);
-        if (amax > 0.f) qs *= down;
-      }
-      qs = fmaxf(qs, 1.1754944e-38f);
-#pragma unroll 1
-      for (int b = 0; b < D; b += 64) {
-        uint4 v[N][8];
-        if (N == 1 && wide && me.live) {
-#pragma unroll
-          for (int c = 0; c < 8; c++) v[0][c] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at + b + c * 8);
-        } else {
-          float f[64];
-          if (me.live) load64(p.q, p.q_dtype, at + b, wide, f);
-#pragma unroll
-          for (int c = 0; c < 8; c++) {
-            uint32_t x[4][N];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const int i = c * 8 + j * 2;
-              parts_of<N, BF>(me.live ? f[i] * up : 0.f, me.live ? f[i + 1] * up : 0.f, x[j]);
+            for (int i = 0; i < 8; i++) {
+              const int64_t at = row_at(i0 + i);
+              v[i] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
-            for (int i = 0; i < N; i++) v[i][c] = make_uint4(x[0][i], x[1][i], x[2][i], x[3][i]);
+            for (int i = 0; i < 8; i++) st_s4(place(i0 + i, 0), v[i]);
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < RUNS; i++) {
+            const int64_t at = row_at(i);
+            uint32_t x[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = at >= 0 ? pack2(load_as_f(p.q, p.q_dtype, at + 2 * j), load_as_f(p.q, p.q_dtype, at + 2 * j + 1), BF ? B200Q_BF16 : B200Q_F16) : 0u;
+            st_s4(place(i, 0), make_uint4(x[0], x[1], x[2], x[3]));
           }
         }
+      } else {
+        float mine = 1.f;      // what undoes this thread's row's scaling
+#pragma unroll 1
+        for (int i0 = 0; i0 < 32 / AT_ONCE; i0 += 8) {
+          float4 v[8];
 #pragma unroll
-        for (int i = 0; i < N; i++)
+          for (int i = 0; i < 8; i++) {
+            const int64_t at = row_at(i0 + i);
+            v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (at >= 0) {
+              if (wide && p.q_dtype == B200Q_F32) v[i] = *reinterpret_cast<const float4*>(static_cast<const float*>(p.q) + at);
+              else v[i] = make_float4(load_as_f(p.q, p.q_dtype, at), load_as_f(p.q, p.q_dtype, at + 1), load_as_f(p.q, p.q_dtype, at + 2), load_as_f(p.q, p.q_dtype, at + 3));
+            }
+          }
 #pragma unroll
-          for (int c = 0; c < 8; c++) st_s4(to + i * 2 * TILE + (b / 64) * SUB + ((c ^ (r & 7)) << 4), v[i][c]);
+          for (int i = 0; i < 8; i++) {
+            float amax = fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))), up, down;
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+            pow2_scale(amax, up, down);
+            if (amax == 0.f) down = 1.f;
+            const float d = __shfl_sync(0xffffffffu, down, lane % AT_ONCE * LANES);
+            if (lane / AT_ONCE == i0 + i) mine = d;
+            uint32_t x[N], y[N];
+            parts_of<N, BF>(v[i].x * up, v[i].y * up, x);
+            parts_of<N, BF>(v[i].z * up, v[i].w * up, y);
+#pragma unroll
+            for (int q = 0; q < N; q++) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(place(i0 + i, q)), "r"(x[q]), "r"(y[q]) : "memory");
+          }
+        }
+        qs *= mine;
       }
+      qs = fmaxf(qs, 1.1754944e-38f);
     }
     fence_async();
     __syncwarp();
@@ -322,48 +348,55 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
         // the tile before: its weighted sum is complete (the scores behind it in the tensor core's queue are)
         if (j > 0) {
 #pragma unroll
-          for (int c = 0; c < D / 32; c++) {
-            uint32_t o[32];
-            ld32(to + c * 32, o);
+          for (int c = 0; c < D / 16; c++) {
+            uint32_t o[16];
+            ld16(to + c * 16, o);
             wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; i++) acc[c * 32 + i] = fmaf(acc[c * 32 + i], scaled, __uint_as_float(o[i]));
+            for (int i = 0; i < 16; i++) acc[c * 16 + i] = fmaf(acc[c * 16 + i], scaled, __uint_as_float(o[i]));
           }
         }
 #pragma unroll 1
         for (int c = 0; c < 4; c++) {
-          uint32_t s[32];
-          ld32(ts + c * 32, s);
+          float s[32];
+          ld32(ts + c * 32, reinterpret_cast<uint32_t*>(s));
           wait_ld();
+          if (masked) {
 #pragma unroll
-          for (int i = 0; i < 32; i++) top = fmaxf(top, masked && c * 32 + i > lim ? -INFINITY : __uint_as_float(s[i]));
+            for (int i = 0; i < 32; i++) s[i] = c * 32 + i <= lim ? s[i] : -INFINITY;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) top = max3(top, s[i], s[i + 1]);
         }
         top *= qs;
+        if (!(top < INFINITY)) { l = __uint_as_float(0x7FC00000u); top = m; }
         const float mn = fmaxf(m, top);
         scaled = mn == -INFINITY ? 1.f : pow2(m - mn);
         m = mn;
         l *= scaled;
         const float sub = m == -INFINITY ? 0.f : T_BASE + 7 - m;
         float sum = 0.f;
-#pragma unroll 1
-        for (int c = 0; c < 4; c++) {
-          uint32_t s[32], pk[32];
-          ld32(ts + c * 32, s);
+#pragma unroll 2
+        for (int c = 0; c < 8; c++) {                      // 16 keys: their high parts, then the low ones
+          float s[16];
+          uint32_t hi[8], lo[8];
+          ld16(ts + c * 16, reinterpret_cast<uint32_t*>(s));
           wait_ld();
           if (masked) {
 #pragma unroll
-            for (int i = 0; i < 32; i++) s[i] = c * 32 + i <= lim ? s[i] : __float_as_uint(-INFINITY);
+            for (int i = 0; i < 16; i++) s[i] = c * 16 + i <= lim ? s[i] : -INFINITY;
           }
 #pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const float a = pow2(fmaf(__uint_as_float(s[2 * i]), qs, sub)), b = pow2(fmaf(__uint_as_float(s[2 * i + 1]), qs, sub));
+          for (int i = 0; i < 8; i++) {
+            const float a = pow2(fmaf(s[2 * i], qs, sub)), b = pow2(fmaf(s[2 * i + 1], qs, sub));
             sum += a + b;
             uint32_t x[N];
             parts_of<N, BF>(a, b, x);
-#pragma unroll
-            for (int q = 0; q < N; q++) pk[q * 16 + i] = x[q];
+            hi[i] = x[0];
+            lo[i] = x[N - 1];
           }
-          st32(ts + c * 32, pk);
+          st8(ts + c * 16, hi);
+          st8(ts + c * 16 + 8, lo);
         }
         l += sum;
         wait_st();
@@ -380,49 +413,59 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
       float* part = p.parts + ((int64_t)unit * p.n_split + split) * PART<T_R, D>;
       const int pr = t * T_ROWS + r;
       if (n_parts > 1 && me.live) { __stcg(part + pr, m); __stcg(part + T_R + pr, l); }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float inv = n_parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       const int64_t at = me.row * p.out_stride + me.head * D;
-      const bool wide = (((uintptr_t)p.out | (uintptr_t)(p.out_stride * (p.out_dtype == B200Q_F32 ? 4 : 2))) & 15) == 0;
+      const bool words = n_parts > 1 || p.out_dtype == B200Q_F32;      // 32-bit values leave
+      const bool wide = n_parts > 1 || (((uintptr_t)p.out | (uintptr_t)(p.out_stride * (words ? 4 : 2))) & 15) == 0;
+      const unsigned live = __ballot_sync(0xffffffffu, me.live);
+      if constexpr (N == 2) {      // all of it in tensor memory, as of N == 1
 #pragma unroll
+        for (int c = 0; c < D / 16; c++) {
+          uint32_t x[16];
+          if (tiles) {
+            ld16(to + c * 16, x);
+            wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = __float_as_uint(fmaf(acc[c * 16 + i], scaled, __uint_as_float(x[i])));
+            st16(to + c * 16, x);
+          }
+        }
+        wait_st();
+      }
+      // 32 columns at a time through the place of the warp's queries, so that a store writes whole pieces of rows.  (Short loops: this runs once a CTA, and unrolled it took 12000 cycles, which its
+      // instructions needed to come.)
+      const uint32_t stage = s_q + t * TILE + (warp & 3) * (32 * 128);
+      const float factor = l == 0.f ? 0.f : inv;
+#pragma unroll 1
       for (int c = 0; c < D / 32; c++) {
         uint32_t x[32];
-        float o[32];
         if (tiles) { ld32(to + c * 32, x); wait_ld(); }
+        __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 32; i++) {
-          const float f = tiles ? __uint_as_float(x[i]) : 0.f;
-          if constexpr (N == 2) o[i] = fmaf(acc[c * 32 + i], scaled, f);
-          else o[i] = f;
+        for (int i = 0; i < 32; i += 4) {
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (tiles && l != 0.f) v = make_float4(__uint_as_float(x[i]) * factor, __uint_as_float(x[i + 1]) * factor, __uint_as_float(x[i + 2]) * factor, __uint_as_float(x[i + 3]) * factor);
+          st_s4(stage + lane * 128 + (((i >> 2) ^ (lane & 7)) << 4), make_uint4(__float_as_uint(v.x), __float_as_uint(v.y), __float_as_uint(v.z), __float_as_uint(v.w)));
         }
-        if (bad_lo <= bad_hi && me.live) {
-          float y[32];
-#pragma unroll
-          for (int i = 0; i < 32; i++) y[i] = o[i];
-          add_not_finite<D, BF>(p, w.seq, kvh, bad_lo, bad_hi, c * 32, y);
-#pragma unroll
-          for (int i = 0; i < 32; i++) o[i] = y[i];
-        }
-        if (!me.live) continue;
-        if (n_parts > 1) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) __stcg(reinterpret_cast<float4*>(part + 2 * T_R + pr * D + c * 32 + i), make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]));
-          continue;
-        }
-#pragma unroll
-        for (int i = 0; i < 32; i++) o[i] = l == 0.f ? 0.f : o[i] * inv;
-        if (!wide) {
-#pragma unroll
-          for (int i = 0; i < 32; i++) store_as(p.out, p.out_dtype, at + c * 32 + i, o[i]);
-        } else if (p.out_dtype == B200Q_F32) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at + c * 32 + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint32_t y[4];
-#pragma unroll
-            for (int q = 0; q < 4; q++) y[q] = pack2(o[i + 2 * q], o[i + 2 * q + 1], p.out_dtype);
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + at + c * 32 + i) = make_uint4(y[0], y[1], y[2], y[3]);
+        if (bad_lo <= bad_hi && me.live) add_not_finite<BF>(p, w.seq, kvh, bad_lo, bad_hi, c * 32, stage + lane * 128, lane & 7);
+        __syncwarp();
+        const int per_row = !wide ? 32 : words ? 8 : 4, piece = lane % per_row;
+#pragma unroll 2
+        for (int i = 0; i < per_row; i++) {
+          const int row = i * (32 / per_row) + lane / per_row;
+          const int64_t to_row = __shfl_sync(0xffffffffu, at, row) + c * 32;
+          if (!(live >> row & 1)) continue;
+          auto quad = [&](int q) { return ld_s4(stage + row * 128 + ((q ^ (row & 7)) << 4)); };
+          if (n_parts > 1) __stcg(reinterpret_cast<uint4*>(part + 2 * T_R + (t * T_ROWS + (warp & 3) * 32 + row) * D + c * 32 + piece * 4), quad(piece));
+          else if (!wide) {
+            float y;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(stage + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4) : "memory");
+            store_as(p.out, p.out_dtype, to_row + lane, y);
+          } else if (words) *reinterpret_cast<uint4*>(static_cast<float*>(p.out) + to_row + piece * 4) = quad(piece);
+          else {
+            const uint4 a = quad(piece * 2), b = quad(piece * 2 + 1);
+            auto two_of = [&](uint32_t u, uint32_t v) { return pack2(__uint_as_float(u), __uint_as_float(v), p.out_dtype); };
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to_row + piece * 8) = make_uint4(two_of(a.x, a.y), two_of(a.z, a.w), two_of(b.x, b.y), two_of(b.z, b.w));
           }
         }
       }
@@ -433,13 +476,15 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
     // ---- products ----
     if (elect_one()) {
       constexpr uint32_t ID_S = idesc_of<BF, false>(T_KEYS), ID_O = idesc_of<BF, true>(D);
+      const uint32_t q0 = desc_128(s_q, 16), k0 = desc_128(s_k, 16), v0 = desc_128(s_v, SUB);
       auto scores = [&](int t, int ks) {
+        const uint32_t q = q0 + t * (TILE >> 4), k = k0 + ks * (TILE >> 4);
 #pragma unroll
         for (int i = N - 1; i >= 0; i--)
 #pragma unroll
           for (int kk = 0; kk < KK; kk++) {
-            const uint32_t o = (kk / 4) * SUB + (kk % 4) * 32;
-            mma_ss_a(tmem + t * 128, desc_128(s_q + (i * 2 + t) * TILE + o, 16), desc_128(s_k + ks * TILE + o, 16), ID_S, i < N - 1 || kk > 0);
+            const uint32_t o = ((kk / 4) * SUB + (kk % 4) * 32) >> 4;
+            mma_ss_a(tmem + t * 128, q + i * (2 * TILE >> 4) + o, k + o, ID_S, i < N - 1 || kk > 0);
           }
         a_commit(&sh.s_full[t]);
       };
@@ -452,6 +497,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
       }
       for (int j = 0; ok && j < tiles; j++) {
         const int vs = j % VS, kn = (j + 1) % KS;
+        const uint32_t v = v0 + vs * (TILE >> 4);
         ok = a_wait(sh, &sh.v_clean[vs], (j / VS) & 1);
         for (int t = 0; ok && t < 1 + two; t++) {
           // N == 1: the probabilities come in two halves; N == 2: the parts one after the other, small ones first
@@ -466,7 +512,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
 #pragma unroll
               for (int k = 0; k < (N == 1 ? 4 : 8); k++) {
                 const int kk = N == 1 ? h * 4 + k : k;
-                mma_ts_a(tmem + 256 + t * 128, tmem + t * 128 + (kk / 2) * 32 + i * 16 + (kk & 1) * 8, desc_128(s_v + vs * TILE + kk * 2048, SUB), ID_O, i < N - 1 || kk > 0 || (N == 1 && j > 0));
+                mma_ts_a(tmem + 256 + t * 128, tmem + t * 128 + (N == 1 ? (kk / 2) * 32 + (kk & 1) * 8 : kk * 16 + i * 8), v + kk * (2048 >> 4), ID_O, i < N - 1 || kk > 0 || (N == 1 && j > 0));
               }
           }
           if (!ok) break;
