@@ -24,7 +24,7 @@ struct AttnParams {
   Divisor by_group, by_kv, by_page;
   int tiles_per_seq;         // 0: tiles are counted sequence by sequence
   int above, up_to;          // sequences with above < new tokens <= up_to (those with others are another kernel's)
-  int n_split, split_len, n_sm;
+  int n_split, split_len, n_sm, late;
   int* counters;
   float* parts;
   PagedTables t;
@@ -316,7 +316,7 @@ Plan rows_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group
   return p;
 }
 
-constexpr int FEW_PAIRS = 32;      // (token, head) pairs of a sequence that the rows kernel takes
+constexpr int FEW_PAIRS = 64;      // (token, head) pairs of a sequence that the rows kernel takes
 // The kernels of a call and their shares of it.  many: sequences of more than FEW_PAIRS pairs go to the tiles kernel.
 struct Deal { bool many; int n; Plan plan[2]; size_t bytes; };
 Deal deal_of(const b200q_paged_cache* c, const b200q_paged_batch* b, int group, bool tiles_take) {
@@ -420,14 +420,15 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
   for (int i = 0; i < deal.n; i++)
     if (deal.plan[i].rounds > INT32_MAX || deal.plan[i].n_split > 65535 || n_kv > 65535 || (int64_t)deal.plan[i].tiles * n_kv > INT32_MAX) return B200Q_ERR_TOO_LARGE;
   const cudaStream_t st = (cudaStream_t)stream;
-  for (int i = 0; i < deal.n; i++) {
+  for (int k = 0; k < deal.n; k++) {
+    const int i = deal.n - 1 - k, late = k > 0;      // few rows first: their CTAs are short, and the tiles' begin where they leave room
     const Plan& plan = deal.plan[i];
     int* const counters = (int*)a->workspace + i * MAX_UNITS;
     float* const parts_at = (float*)((char*)a->workspace + COUNTERS_BYTES + (i ? deal.plan[0].bytes : 0));
     const AttnParams p{a->q, cache->k, cache->v, a->out, a->q_dtype, a->out_dtype, a->q_stride ? a->q_stride : row, a->out_stride ? a->out_stride : row, cache->page_stride,
                        cache->head_stride, cache->row_stride, a->n_heads, n_kv, group, (a->scale > 0.f ? a->scale : 1.f / sqrtf((float)dim)) * LOG2E, divisor_of(group), divisor_of(n_kv), divisor_of(cache->page_size), plan.tiles_per_seq, plan.above, plan.up_to,
-                       plan.n_split, plan.split_len, N_SM, counters, parts_at, tables_of(cache, batch)};
-    const bool pdl = i == 0 && (flags & B200Q_FLAG_PDL);
+                       plan.n_split, plan.split_len, N_SM, late, counters, parts_at, tables_of(cache, batch)};
+    const bool pdl = late || (flags & B200Q_FLAG_PDL);
     const int type = cache->dtype == B200Q_BF16;
     if (deal.many && i == 0) {
       int smem;
@@ -435,7 +436,7 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
       static PerDeviceFlag allowed[2][2][2];
       if ((rc = allow_smem(kernel, smem, allowed[type][parts - 1][dim == 128])) != B200Q_OK) return rc;
       B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles * n_kv, plan.n_split), dim3(T_THREADS), (size_t)smem, st, pdl, p, boxes[2], boxes[3], box_rows_of(cache)));
-      if (plan.n_split > 1) B200Q_CHECK_CUDA(launch_k(dim == 64 ? join_tiles_kernel<64> : join_tiles_kernel<128>, dim3(plan.tiles * n_kv, T_R / J_ROWS), dim3(J_THREADS), 0, st, true, p));
+      if (plan.n_split > 1) B200Q_CHECK_CUDA(launch_k(dim == 64 ? join_tiles_kernel<64> : join_tiles_kernel<128>, dim3(plan.tiles * n_kv, J_SLICES), dim3(J_THREADS), 0, st, true, p));
       continue;
     }
     if (cache->dtype == B200Q_F32) {

@@ -15,7 +15,7 @@
 
 namespace {
 
-constexpr int T_ROWS = 128, T_R = 2 * T_ROWS, T_KEYS = 128, T_THREADS = 384, T_BASE = 7, T_PARTS = 8;      // probabilities up to 2^(7 + 8)
+constexpr int T_ROWS = 128, T_R = 2 * T_ROWS, T_KEYS = 128, T_THREADS = 384, T_BASE = 7, T_PARTS = 16;      // probabilities up to 2^(7 + 8)
 template <int D> constexpr int T_TILE = T_KEYS * D * 2;                                     // bytes of 128 rows of 16-bit values
 template <int D, int N> constexpr int T_KS = D == 64 ? 3 : N == 1 ? 2 : 1;
 template <int D, int N> constexpr int T_VS = D == 64 ? 3 : N == 1 ? 3 : 2;
@@ -137,15 +137,18 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
   constexpr int SUBS = D / 64, TILE = T_TILE<D>, SUB = T_KEYS * 128, KS = T_KS<D, N>, VS = T_VS<D, N>, KK = D / 16;
   extern __shared__ unsigned char raw[];
   __shared__ SharedA sh;
-  pdl_wait();
+  // Behind the kernel for few rows of the same call (late): both read what was there before that one began and write rows of their own, so that this one waits for it only at its end.
+  if (!p.late) pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int order = p.by_kv.div(blockIdx.x), kvh = blockIdx.x - order * p.n_kv, split = blockIdx.y;
   const int tile_index = p.by_kv.div(gridDim.x) - 1 - order;      // long ones first
   const TilePlace w = place_of_tile<T_R>(p, tile_index);
-  if (w.n == 0) return;
-  const int n_parts = max(1, (w.keys + p.split_len - 1) / p.split_len), k_begin = split * p.split_len, k_end = min(w.keys, k_begin + p.split_len);
-  if (split >= n_parts) return;
+  const int n_parts = w.n == 0 ? 0 : max(1, (w.keys + p.split_len - 1) / p.split_len), k_begin = split * p.split_len, k_end = min(w.keys, k_begin + p.split_len);
+  if (split >= n_parts) {
+    if (p.late) pdl_wait();
+    return;
+  }
   const int tiles = max(0, (k_end - k_begin + T_KEYS - 1) / T_KEYS);
   const int pairs = w.n * p.group;
   const bool two = w.r0 + T_ROWS < pairs;                      // the second tile of rows has some
@@ -600,43 +603,41 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
   __syncthreads();
   fence_after();
   if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  if (p.late) pdl_wait();
 }
 
-// The parts of tiles whose keys are split, added in the order of the keys: a CTA 32 rows of a (tile, KV head).
-constexpr int J_ROWS = 32, J_THREADS = 256;
+// The parts of tiles whose keys are split, added in the order of the keys: J_SLICES CTAs for a (tile, KV head); a warp a row, a lane a part for the parts' shares and D / 32 values for the sum.
+constexpr int J_SLICES = 8, J_THREADS = 256;
+static_assert(T_PARTS <= 32, "a lane a part");
 template <int D>
 __global__ void __launch_bounds__(J_THREADS) join_tiles_kernel(const AttnParams p) {
+  constexpr int V = D / 32;
   pdl_wait();
   pdl_launch_dependents();
-  const int order = p.by_kv.div(blockIdx.x), kvh = blockIdx.x - order * p.n_kv, tile_index = p.by_kv.div(gridDim.x) - 1 - order;
+  const int order = p.by_kv.div(blockIdx.x), kvh = blockIdx.x - order * p.n_kv, tile_index = p.by_kv.div(gridDim.x) - 1 - order, lane = threadIdx.x & 31;
   const TilePlace w = place_of_tile<T_R>(p, tile_index);
   const int n_parts = (w.keys + p.split_len - 1) / p.split_len, end = min(T_R, w.n * p.group - w.r0);
   if (w.n == 0 || n_parts <= 1) return;
   const float* first = p.parts + (int64_t)(tile_index * p.n_kv + kvh) * p.n_split * PART<T_R, D>;
-  for (int i = threadIdx.x; i < J_ROWS * (D / 4); i += J_THREADS) {
-    const int r = blockIdx.y * J_ROWS + i / (D / 4), d = i % (D / 4) * 4, pair = w.r0 + r, token = p.by_group.div(pair);
-    if (r >= end) return;
-    float ms[T_PARTS], ls[T_PARTS], m = -INFINITY, sum = 0.f, o[4] = {};
-    float4 v[T_PARTS];
+#pragma unroll 1
+  for (int r = blockIdx.y * (J_THREADS / 32) + (threadIdx.x >> 5); r < end; r += J_SLICES * (J_THREADS / 32)) {
+    float m = -INFINITY, l = 0.f, o[V] = {};
+    if (lane < n_parts) { m = __ldcg(first + lane * PART<T_R, D> + r); l = __ldcg(first + lane * PART<T_R, D> + T_R + r); }
+    const float top = warp_max(m), f = l == 0.f ? 0.f : pow2(m - top), sum = warp_sum(f * l);      // (a part without keys has sum 0)
+#pragma unroll 4
+    for (int q = 0; q < n_parts; q++) {
+      const float* b = first + q * PART<T_R, D> + 2 * T_R + r * D + lane * V;
+      const float g = __shfl_sync(0xffffffffu, f, q);
+      float v[V];
+      if constexpr (V == 4) { const float4 y = __ldcg(reinterpret_cast<const float4*>(b)); v[0] = y.x; v[1] = y.y; v[2] = y.z; v[3] = y.w; }
+      else { const float2 y = __ldcg(reinterpret_cast<const float2*>(b)); v[0] = y.x; v[1] = y.y; }
 #pragma unroll
-    for (int q = 0; q < T_PARTS; q++) {
-      const float* b = first + (int64_t)min(q, n_parts - 1) * PART<T_R, D>;
-      ms[q] = __ldcg(b + r);
-      ls[q] = __ldcg(b + T_R + r);
-      v[q] = __ldcg(reinterpret_cast<const float4*>(b + 2 * T_R + r * D + d));
+      for (int i = 0; i < V; i++) o[i] = fmaf(g, v[i], o[i]);
     }
+    const int pair = w.r0 + r, token = p.by_group.div(pair);
+    const int64_t at = (w.first_row + token) * p.out_stride + (int64_t)(kvh * p.group + pair - token * p.group) * D + lane * V;
 #pragma unroll
-    for (int q = 0; q < T_PARTS; q++) m = fmaxf(m, ms[q]);
-#pragma unroll
-    for (int q = 0; q < T_PARTS; q++) {
-      if (q >= n_parts) break;
-      const float f = ls[q] == 0.f ? 0.f : pow2(ms[q] - m);      // (a part without keys has sum 0)
-      sum = fmaf(f, ls[q], sum);
-      o[0] = fmaf(f, v[q].x, o[0]); o[1] = fmaf(f, v[q].y, o[1]); o[2] = fmaf(f, v[q].z, o[2]); o[3] = fmaf(f, v[q].w, o[3]);
-    }
-    const int64_t at = (w.first_row + token) * p.out_stride + (int64_t)(kvh * p.group + pair - token * p.group) * D + d;
-#pragma unroll
-    for (int j = 0; j < 4; j++) store_as(p.out, p.out_dtype, at + j, sum == 0.f ? 0.f : o[j] / sum);
+    for (int i = 0; i < V; i++) store_as(p.out, p.out_dtype, at + i, sum == 0.f ? 0.f : o[i] / sum);
   }
 }
 
