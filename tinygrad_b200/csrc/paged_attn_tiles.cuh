@@ -83,6 +83,7 @@ __device__ __forceinline__ uint4 ld_s4(uint32_t a) {
 }
 
 template <bool V> struct Switch { static constexpr bool value = V; };
+template <int V> struct Count { static constexpr int value = V; };
 // two fp32 values at a time
 __device__ __forceinline__ uint64_t pair_of(float a, float b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
 __device__ __forceinline__ float2 floats_of(uint64_t r) { float2 f; asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(r)); return f; }
@@ -206,17 +207,14 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
       if constexpr (N == 1) {
         constexpr int RUNS = 32 / AT_ONCE;
         if (wide) {
-#pragma unroll 1
-          for (int i0 = 0; i0 < RUNS; i0 += 8) {
-            uint4 v[8];
+          uint4 v[RUNS];
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-              const int64_t at = row_at(i0 + i);
-              v[i] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at) : make_uint4(0, 0, 0, 0);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) st_s4(place(i0 + i, 0), v[i]);
+          for (int i = 0; i < RUNS; i++) {
+            const int64_t at = row_at(i);
+            v[i] = at >= 0 ? *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + at) : make_uint4(0, 0, 0, 0);
           }
+#pragma unroll
+          for (int i = 0; i < RUNS; i++) st_s4(place(i, 0), v[i]);
         } else {
 #pragma unroll 1
           for (int i = 0; i < RUNS; i++) {
@@ -452,25 +450,35 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
         }
         if (bad_lo <= bad_hi && me.live) add_not_finite<BF>(p, w.seq, kvh, bad_lo, bad_hi, c * 32, stage + lane * 128, lane & 7);
         __syncwarp();
-        const int per_row = !wide ? 32 : words ? 8 : 4, piece = lane % per_row;
-#pragma unroll 2
-        for (int i = 0; i < per_row; i++) {
-          const int row = i * (32 / per_row) + lane / per_row;
-          const int64_t to_row = __shfl_sync(0xffffffffu, at, row) + c * 32;
-          if (!(live >> row & 1)) continue;
-          auto quad = [&](int q) { return ld_s4(stage + row * 128 + ((q ^ (row & 7)) << 4)); };
-          if (n_parts > 1) __stcg(reinterpret_cast<uint4*>(part + 2 * T_R + (t * T_ROWS + (warp & 3) * 32 + row) * D + c * 32 + piece * 4), quad(piece));
-          else if (!wide) {
+        // PER_ROW lanes a row; body(row, its place in the outputs)
+        auto rows = [&](auto lanes, auto body) {
+          constexpr int PER_ROW = lanes.value;
+#pragma unroll
+          for (int i = 0; i < PER_ROW; i++) {
+            const int row = i * (32 / PER_ROW) + lane / PER_ROW;
+            const int64_t to_row = __shfl_sync(0xffffffffu, at, row) + c * 32;
+            if (live >> row & 1) body(row, to_row);
+          }
+        };
+        auto quad = [&](int row, int q) { return ld_s4(stage + row * 128 + ((q ^ (row & 7)) << 4)); };
+        if (n_parts > 1)
+          rows(Count<8>{}, [&](int row, int64_t) { __stcg(reinterpret_cast<uint4*>(part + 2 * T_R + (t * T_ROWS + (warp & 3) * 32 + row) * D + c * 32 + (lane & 7) * 4), quad(row, lane & 7)); });
+        else if (wide && !words)
+          rows(Count<4>{}, [&](int row, int64_t to_row) {
+            const uint4 x = quad(row, (lane & 3) * 2), y = quad(row, (lane & 3) * 2 + 1);
+            auto two_of = [&](uint32_t u, uint32_t v) { return pack2(__uint_as_float(u), __uint_as_float(v), p.out_dtype); };
+            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to_row + (lane & 3) * 8) = make_uint4(two_of(x.x, x.y), two_of(x.z, x.w), two_of(y.x, y.y), two_of(y.z, y.w));
+          });
+        else if (wide)
+          rows(Count<8>{}, [&](int row, int64_t to_row) { *reinterpret_cast<uint4*>(static_cast<float*>(p.out) + to_row + (lane & 7) * 4) = quad(row, lane & 7); });
+        else
+#pragma unroll 1
+          for (int row = 0; row < 32; row++) {
+            const int64_t to_row = __shfl_sync(0xffffffffu, at, row) + c * 32;
             float y;
             asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(stage + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4) : "memory");
-            store_as(p.out, p.out_dtype, to_row + lane, y);
-          } else if (words) *reinterpret_cast<uint4*>(static_cast<float*>(p.out) + to_row + piece * 4) = quad(piece);
-          else {
-            const uint4 a = quad(piece * 2), b = quad(piece * 2 + 1);
-            auto two_of = [&](uint32_t u, uint32_t v) { return pack2(__uint_as_float(u), __uint_as_float(v), p.out_dtype); };
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + to_row + piece * 8) = make_uint4(two_of(a.x, a.y), two_of(a.z, a.w), two_of(b.x, b.y), two_of(b.z, b.w));
+            if (live >> row & 1) store_as(p.out, p.out_dtype, to_row + lane, y);
           }
-        }
       }
     }
   } else {
@@ -571,25 +579,39 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
       const int k0 = k_begin + j * T_KEYS;
       ok = __all_sync(0xffffffffu, a_wait(sh, &sh.v_full[st], use & 1));
       if (!ok) break;
-      const int from = max(0, min(first_last + 1, k_end) - k0);      // the first row that somebody does not see
+      const int from = max(0, min(first_last + 1, k_end) - k0), behind = max(0, min(T_KEYS, k_end - k0));      // the first row that somebody does not see, that nobody sees
       if (from < T_KEYS) {
-        bool changed = false;
-#pragma unroll 4
-        for (int i = from * 8 + lane; i < T_KEYS * 8; i += 32) {
-          const int key = k0 + i / 8;
+        // (Looking must be quick: the tile's product waits for it, and where it was not, the last product of a CTA came 8000 cycles late.  A value is not finite where its exponent and one more overflow.)
+        constexpr uint32_t E = BF ? 0x7F807F80u : 0x7C007C00u, ONE = BF ? 0x00800080u : 0x04000400u;
+        uint32_t odd = 0;
+#pragma unroll 8
+        for (int i = from * 8 + lane; i < behind * 8; i += 32) {
 #pragma unroll
           for (int s = 0; s < SUBS; s++) {
-            const uint32_t a = s_v + st * TILE + s * SUB + i * 16;
-            const uint4 x = ld_s4(a);
-            uint4 y = make_uint4(finite_only<BF>(x.x), finite_only<BF>(x.y), finite_only<BF>(x.z), finite_only<BF>(x.w));
-            const bool behind = key >= k_end;
-            if (behind) y = make_uint4(0, 0, 0, 0);
-            if (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w) {
+            const uint4 x = ld_s4(s_v + st * TILE + s * SUB + i * 16);
+            odd |= ((x.x & E) + ONE) | ((x.y & E) + ONE) | ((x.z & E) + ONE) | ((x.w & E) + ONE);
+          }
+        }
+        bool changed = false;
+        if (odd & 0x80008000u) {
+#pragma unroll 1
+          for (int i = from * 8 + lane; i < behind * 8; i += 32) {
+#pragma unroll 1
+            for (int s = 0; s < SUBS; s++) {
+              const uint32_t a = s_v + st * TILE + s * SUB + i * 16;
+              const uint4 x = ld_s4(a), y = make_uint4(finite_only<BF>(x.x), finite_only<BF>(x.y), finite_only<BF>(x.z), finite_only<BF>(x.w));
+              if (x.x == y.x && x.y == y.y && x.z == y.z && x.w == y.w) continue;
               st_s4(a, y);
               changed = true;
-              if (!behind) { atomicMin(&sh.bad_lo, key); atomicMax(&sh.bad_hi, key); }
+              atomicMin(&sh.bad_lo, k0 + i / 8);
+              atomicMax(&sh.bad_hi, k0 + i / 8);
             }
           }
+        }
+        for (int i = behind * 8 + lane; i < T_KEYS * 8; i += 32) {
+#pragma unroll
+          for (int s = 0; s < SUBS; s++) st_s4(s_v + st * TILE + s * SUB + i * 16, make_uint4(0, 0, 0, 0));
+          changed = true;
         }
         if (changed) fence_async();
       }
