@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
         const float sub = m == -INFINITY ? 0.f : T_BASE + 7 - m;
         float sum = 0.f;
 #pragma unroll 2
-        for (int c = 0; c < 8; c++) {                      // 16 keys: their high parts, then the low ones
+        for (int c = 0; c < 8; c++) {                      // 16 keys: their high parts, then the low ones (8 columns each); half of the tile is handed over as soon as it is there
           float s[16];
           uint32_t hi[8], lo[8];
           ld16(ts + c * 16, reinterpret_cast<uint32_t*>(s));
@@ -398,12 +398,13 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
           }
           st8(ts + c * 16, hi);
           st8(ts + c * 16 + 8, lo);
+          if (c & 3 ^ 3) continue;
+          wait_st();
+          fence_before();
+          __syncwarp();
+          if (lane == 0) a_bar_arrive(&sh.p_full[t][c >> 2]);
         }
         l += sum;
-        wait_st();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) { a_bar_arrive(&sh.p_full[t][0]); a_bar_arrive(&sh.p_full[t][1]); }
       }
     }
     if (ok && tiles) ok = __all_sync(0xffffffffu, a_wait(sh, &sh.o_full, 0));
@@ -511,20 +512,18 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
         const uint32_t v = v0 + vs * (TILE >> 4);
         ok = a_wait(sh, &sh.v_clean[vs], (j / VS) & 1);
         for (int t = 0; ok && t < 1 + two; t++) {
-          // N == 1: the probabilities come in two halves; N == 2: the parts one after the other, small ones first
+          // the probabilities come in two halves; their small parts first
 #pragma unroll
           for (int h = 0; h < 2; h++) {
             ok = ok && a_wait(sh, &sh.p_full[t][h], j & 1);
             if (!ok) break;
             fence_after();
-            if (N == 2 && h == 1) break;
 #pragma unroll
             for (int i = N - 1; i >= 0; i--)
 #pragma unroll
-              for (int k = 0; k < (N == 1 ? 4 : 8); k++) {
-                const int kk = N == 1 ? h * 4 + k : k;
-                mma_ts_a(tmem + 256 + t * 128, tmem + t * 128 + (N == 1 ? (kk / 2) * 32 + (kk & 1) * 8 : kk * 16 + i * 8), v + kk * (2048 >> 4), ID_O, i < N - 1 || kk > 0 || (N == 1 && j > 0));
-              }
+              for (int kk = h * 4; kk < h * 4 + 4; kk++)
+                mma_ts_a(tmem + 256 + t * 128, tmem + t * 128 + (N == 1 ? (kk / 2) * 32 + (kk & 1) * 8 : kk * 16 + i * 8), v + kk * (2048 >> 4), ID_O,
+                         h > 0 || i < N - 1 || kk > 0 || (N == 1 && j > 0));
           }
           if (!ok) break;
           if (t == two) a_commit(&sh.v_empty[vs]);
