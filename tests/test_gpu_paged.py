@@ -273,6 +273,10 @@ ATTEND = [   # seqs' (new, length), heads, KV heads, dim, page size, types of q 
   ([(300, 5000)], 4, 1, 128, 16, "float16", "float16", None),
   ([(90, 4000)], 16, 1, 64, 256, "float16", "float16", "float32"),
   ([(150, 150), (2, 60)], 7, 1, 128, 64, "bfloat16", "bfloat16", "float16"),
+  ([(1, 300), (3, 90)], 40, 1, 64, 32, "float32", "float16", None),                                     # more heads to a key head than a tile of 16 rows has
+  ([(1 + i % 3, 20 + 7 * i) for i in range(70)], 4, 2, 64, 16, "float16", "float16", None),             # more sequences than a warp has lanes
+  ([(i % 2 * (1 + i), 5 + 9 * i) for i in range(40)], 2, 1, 128, 16, "float32", "float16", None),       # many without new tokens, few and many rows in one batch
+  ([(260, 900), (1, 3000), (0, 7), (33, 33)], 8, 8, 128, 16, "float32", "float16", "float16"),
 ]
 
 
@@ -369,6 +373,162 @@ def test_attention_gives_the_same_bits_again():
   for args in (([(1, 3000), (1, 70)], 8, 2, 128, 16, "float32", "float16"), ([(300, 4000)], 8, 2, 128, 16, "float16", "float16"), ([(3, 2500)], 4, 2, 64, 16, "bfloat16", "bfloat16")):
     a, b = attend(*args, seed=1), attend(*args, seed=1)
     assert (a == b).all()
+
+
+@pytest.mark.parametrize("qt,ct", [("float16", "float16"), ("bfloat16", "bfloat16"), ("float32", "float16")])
+@pytest.mark.parametrize("seqs", [[(1, 200), (2, 33)], [(140, 300), (1, 90)]], ids=["tokens", "chunks"])
+def test_attention_of_rows_on_odd_boundaries(qt, ct, seqs):
+  """Queries and outputs one element off, with strides that are no multiple of 16 bytes: the same values as on whole boundaries."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  from tinygrad_b200.runtime import DeviceBuffer
+  rng = np.random.default_rng(3)
+  h, hk, d, ps = 4, 2, 64, 16
+  new, length = [n for n, _ in seqs], [l for _, l in seqs]
+  off, n = np.concatenate([[0], np.cumsum(new)]), sum(new)
+  t, n_pages = table(rng, length, ps)
+  (k, _), (v, _) = (put(rng.standard_normal((n_pages, hk, ps, d)), ct) for _ in "kv")
+  x = rng.standard_normal((n, h * d))
+  cache = paged.PagedCache(n_pages, ps, hk, d, ct, k=k, v=v)
+  batch = paged.PagedBatch(i32(off), i32(length), i32(t), n_rows=n, max_new=max(new), max_len=max(length))
+  q, out = put(x, qt)[0], put(np.zeros((n, h * d)), qt)[0]
+  paged.attention(cache, batch, q, out, h, qt)
+  size, stride = 4 if qt == "float32" else 2, h * d + 3
+  wide = np.zeros((n * stride + 1,))
+  np.lib.stride_tricks.as_strided(wide[1:], (n, h * d), (8 * stride, 8))[:] = x
+  q2, out2 = put(wide, qt)[0], put(np.full(n * stride + 1, 5.0), qt)[0]
+  paged.attention(cache, batch, q2.ptr + size, out2.ptr + size, h, qt, q_stride=stride, out_stride=stride)
+  got = get(out2, (n * stride + 1,), qt)
+  rows = np.lib.stride_tricks.as_strided(got[1:], (n, h * d), (8 * stride, 8))
+  assert (rows == get(out, (n, h * d), qt)).all()
+  rows[:] = 5
+  assert (got == 5).all(), "what lies between the rows is as it was"
+
+
+def test_one_workspace_for_calls_of_any_shape():
+  """A batch's workspace serves one call after the other, of any cache and number of heads: no call finds what another has left."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(13)
+  new, length = [1, 130, 2], [3000, 1500, 700]
+  off, n = np.concatenate([[0], np.cumsum(new)]), sum(new)
+  calls = []
+  t, n_pages = table(rng, length, 16)
+  tables = [i32(off), i32(length), i32(t)]
+  for h, hk, d, qt, ct in ((8, 2, 128, "float16", "float16"), (4, 4, 64, "float32", "float32"), (28, 4, 128, "float32", "float16"), (4, 1, 32, "bfloat16", "bfloat16"), (2, 1, 64, "float16", "float16")):
+    (k, _), (v, _) = (put(rng.standard_normal((n_pages, hk, 16, d)), ct) for _ in "kv")
+    q, out = put(rng.standard_normal((n, h, d)), qt)[0], put(np.zeros((n, h, d)), qt)[0]
+    calls.append((paged.PagedCache(n_pages, 16, hk, d, ct, k=k, v=v), q, out, h, d, qt))
+  alone = []
+  for cache, q, out, h, d, qt in calls:
+    paged.attention(cache, paged.PagedBatch(*tables, n_rows=n, max_new=130, max_len=3000), q, out, h, qt)
+    alone.append(get(out, (n, h, d), qt))
+  batch = paged.PagedBatch(*tables, n_rows=n, max_new=130, max_len=3000)
+  for _ in range(2):
+    for (cache, q, out, h, d, qt), want in zip(calls, alone):
+      out.zero_()
+      paged.attention(cache, batch, q, out, h, qt)
+      assert (get(out, (n, h, d), qt) == want).all(), (h, d, qt)
+  assert status() == 0
+
+
+def test_two_streams_at_once():
+  """A batch (and workspace) for each stream: calls that run at the same time do not disturb each other."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  from tinygrad_b200.runtime import Stream
+  rng = np.random.default_rng(14)
+  h, hk, d, ps, new, length = 8, 2, 128, 16, [1, 200], [20000, 4000]
+  t, n_pages = table(rng, length, ps)
+  (k, _), (v, _) = (put(rng.standard_normal((n_pages, hk, ps, d)), "float16") for _ in "kv")
+  cache = paged.PagedCache(n_pages, ps, hk, d, k=k, v=v)
+  q = [put(rng.standard_normal((201, h, d)), "float16")[0] for _ in range(2)]
+  out = [put(np.zeros((201, h, d)), "float16")[0] for _ in range(2)]
+  batches = [paged.PagedBatch(i32([0, 1, 201]), i32(length), i32(t), n_rows=201, max_new=200, max_len=20000) for _ in range(2)]
+  want = []
+  for i in range(2):
+    paged.attention(cache, batches[i], q[i], out[i], h, "float16")
+    want.append(get(out[i], (201, h, d), "float16"))
+    out[i].zero_()
+  streams = [Stream(), Stream()]
+  for _ in range(10):
+    for i in range(2): paged.attention(cache, batches[i], q[i], out[i], h, "float16", stream=streams[i])
+  for s in streams: s.synchronize()
+  for i in range(2): assert (get(out[i], (201, h, d), "float16") == want[i]).all()
+
+
+def test_pools_past_32_bits():
+  """Pages 2^28 elements apart, ten of them: offsets pass 2^31 elements and 2^32 bytes, for appending and for every attention kernel."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  from tinygrad_b200.runtime import DeviceBuffer
+  rng = np.random.default_rng(15)
+  h, hk, d, ps, apart = 4, 2, 64, 16, 1 << 28
+  size = 9 * apart + hk * ps * d
+  k, v = DeviceBuffer(2 * size), DeviceBuffer(2 * size)
+  far = paged.PagedCache(10, ps, hk, d, k=k, v=v, strides=(apart, ps * d, d))
+  near = paged.PagedCache(10, ps, hk, d)
+  x, _ = put(rng.standard_normal((150, h + 2 * hk, d)), "float16")
+  pages = i32(rng.permutation(10)[None])
+  outs = []
+  for cache in (near, far):
+    q, out = put(np.zeros((150, h, d)), "float16")[0], put(np.zeros((150, h, d)), "float16")[0]
+    batch = paged.PagedBatch(i32([0, 150]), i32([150]), pages, n_rows=150, max_new=150, max_len=150)
+    paged.append(cache, batch, x, q, h, "float16")
+    paged.attention(cache, batch, q, out, h, "float16")
+    one = put(np.zeros((1, h, d)), "float16")[0]
+    paged.attention(cache, paged.PagedBatch(i32([0, 1]), i32([150]), pages, n_rows=1, max_new=1, max_len=150), q, one, h, "float16")
+    outs.append((get(out, (150, h, d), "float16"), get(one, (1, h, d), "float16")))
+  assert (outs[0][0] == outs[1][0]).all() and (outs[0][1] == outs[1][1]).all() and outs[0][0].any()
+  assert status() == 0
+
+
+@pytest.mark.parametrize("qt,ct", [("float32", "float16"), ("float16", "float16"), ("bfloat16", "bfloat16"), ("float32", "float32")])
+@pytest.mark.parametrize("new", [2, 150])
+def test_queries_that_are_not_finite(qt, ct, new):
+  """A row of queries that is NaN or infinite gives a row of NaN; the others are what they were.  A row of zeros gives the mean of the values."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(new)
+  h, hk, d, ps, length = 2, 1, 64, 16, 200
+  t, n_pages = table(rng, [length], ps)
+  (k, _), (v, vv) = (put(rng.standard_normal((n_pages, hk, ps, d)), ct) for _ in "kv")
+  cache = paged.PagedCache(n_pages, ps, hk, d, ct, k=k, v=v)
+  batch = paged.PagedBatch(i32([0, new]), i32([length]), i32(t), n_rows=new, max_new=new, max_len=length)
+  x = rng.standard_normal((new, h, d))
+  x[new - 1, 1] = 0
+  outs = []
+  for bad in (None, np.nan, np.inf):
+    if bad is not None: x[0, 0, 3] = bad
+    out = put(np.zeros((new, h, d)), qt)[0]
+    paged.attention(cache, batch, put(x, qt)[0], out, h, qt)
+    outs.append(get(out, (new, h, d), qt))
+  for got in outs[1:]:
+    assert np.isnan(got[0, 0]).all()
+    got[0, 0] = outs[0][0, 0]
+    assert (got == outs[0]).all()
+  mean = ref.gather(vv, t[0], length, ps)[0].mean(0)
+  spread = np.abs(ref.gather(vv, t[0], length, ps)[0]).mean(0)
+  assert (np.abs(outs[0][new - 1, 1] - mean) <= spread * (2.0 ** -21 + 4 * length ** 0.5 * 2.0 ** -23 + EPS[qt]) + EPS[qt] / 2 * np.abs(mean)).all()
+
+
+def test_append_of_more_sequences_than_a_warp_has_lanes():
+  need_gpu()
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(16)
+  h, hk, d, ps = 2, 1, 32, 8
+  new = [int(x) for x in rng.integers(0, 4, 100)]
+  length = [n + int(x) for n, x in zip(new, rng.integers(0, 30, 100))]
+  off, n = np.concatenate([[0], np.cumsum(new)]), sum(new)
+  t, n_pages = table(rng, length, ps)
+  x, xv = put(rng.standard_normal((n, h + 2 * hk, d)), "float32")
+  cache = paged.PagedCache(n_pages, ps, hk, d, "float32")
+  q = put(np.zeros((n, h, d)), "float32")[0]
+  paged.append(cache, paged.PagedBatch(i32(off), i32(length), i32(t), n_rows=n, max_new=3, max_len=max(length)), x, q, h)
+  assert (get(q, (n, h, d), "float32") == xv[:, :h]).all()
+  k = get(cache.k, (n_pages, hk, ps, d), "float32")
+  for row, (s, p) in enumerate(ref.rows_of(off, length)): assert (k[t[s][p // ps], :, p % ps] == xv[row, h:h + hk]).all()
+  assert (k != 0).any(-1).sum() == n
 
 
 def test_nothing_to_do():
