@@ -368,6 +368,40 @@ def test_attention_where_the_tables_are_wrong():
       assert (got[-1] == 9).all() and not (got[-2] == 9).any() and status() == 2
 
 
+@pytest.mark.parametrize("ct", ["float16", "float32"])
+def test_attention_of_rows_that_go_back(ct):
+  """row_off 0, 3, 1, 4: sequences overlap.  Status 2, nothing outside the rows is written, and the work stays what the bounds allow."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(21)
+  (k, _), (v, _), (q, _) = (put(rng.standard_normal(s), t) for s, t in (((4, 2, 16, 64), ct), ((4, 2, 16, 64), ct), ((5, 4, 64), "float32")))
+  out = put(np.full((5, 4, 64), 9.0), "float32")[0]
+  batch = paged.PagedBatch(i32([0, 3, 1, 4]), i32([40, 50, 60]), i32(rng.integers(0, 4, (3, 4))), n_rows=5, max_new=3, max_len=60)
+  status()
+  paged.attention(paged.PagedCache(4, 16, 2, 64, ct, k=k, v=v), batch, q, out, 4)
+  assert (get(out, (5, 4, 64), "float32")[4] == 9).all() and status() == 2
+
+
+def test_attention_of_views():
+  """Rows of torch tensors that lie apart, in and out."""
+  need_gpu()
+  import torch
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(22)
+  n, h, hk, d, length = 3, 4, 2, 64, 45
+  (k, kv), (v, vv) = (put(rng.standard_normal((4, hk, 16, d)), "float16") for _ in range(2))
+  q, out = torch.from_numpy(rng.standard_normal((n, h * d + 40))).half().cuda()[:, 40:], torch.full((n, h * d + 8), 9.0, device="cuda")[:, :h * d]
+  t = rng.integers(0, 4, (1, 3)).astype(np.int32)
+  cache, batch = paged.PagedCache(4, 16, hk, d, "float16", k=k, v=v), paged.PagedBatch(i32([0, n]), i32([length]), i32(t), n_rows=n, max_new=n, max_len=length)
+  torch.cuda.synchronize()
+  paged.attention(cache, batch, q, out, h, "float16", "float32", q_stride=h * d + 40, out_stride=h * d + 8)
+  from tinygrad_b200 import runtime
+  runtime.synchronize()
+  want, weight, reach = ref.attention(q.cpu().double().numpy().reshape(n, h, d), kv, vv, [0, n], [length], t, 16, d ** -0.5)
+  close_attention(out.cpu().double().numpy().reshape(n, h, d), want, weight, reach, d, length, "float16", "float32", "views")
+  assert (out._base[:, h * d:] == 9).all()
+
+
 def test_attention_gives_the_same_bits_again():
   need_gpu()
   for args in (([(1, 3000), (1, 70)], 8, 2, 128, 16, "float32", "float16"), ([(300, 4000)], 8, 2, 128, 16, "float16", "float16"), ([(3, 2500)], 4, 2, 64, 16, "bfloat16", "bfloat16")):

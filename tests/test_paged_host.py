@@ -76,6 +76,16 @@ def test_head_norm_rope_refuses(lib, change, code):
   assert lib.b200q_head_norm_rope(ctypes.byref(a), 0, None) == code
 
 
+@pytest.mark.parametrize("kv_dtype", [F16, F32])
+@pytest.mark.parametrize("n_heads,change", [(64, dict(n_seqs=(1 << 31) - 1, n_rows=(1 << 31) - 1, max_new=1)),
+                                            (2, dict(n_seqs=(1 << 31) - 1, n_rows=(1 << 31) - 1, max_new=100, max_len=(1 << 31) - 1))])
+def test_work_past_31_bits_is_refused(lib, kv_dtype, n_heads, change):
+  """Tiles and rounds that no launch can have: an error, not a count that wrapped around (to 0: a division by it)."""
+  c, b = cache(dtype=kv_dtype), batch(**change)
+  lib.b200q_paged_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(b), n_heads)
+  assert call(lib.b200q_paged_attention, c, b, _lib.PagedAttnArgs(P, P, F32, F32, 0, 0, n_heads, 0.0, P, (1 << 63) - 1)) == -6
+
+
 def test_nothing_to_do_is_fine(lib):
   for b in (batch(n_seqs=0, row_off=None, length=None, pages=None), batch(n_rows=0)):
     assert call(lib.b200q_paged_append, cache(), b, _lib.PagedAppendArgs(None, None, F32, F32, 0, 0, 4)) == 0
@@ -125,3 +135,16 @@ def test_python_side_refuses(lib):
   with pytest.raises(ValueError, match="out has"): paged.attention(c, b, P, Fake((2, 4, 63), np.float32), 4)
   with pytest.raises(ValueError, match="positions has"): paged.head_norm_rope(P, P, 5, 4, 2, 64, rope=Fake((9, 64), np.float32), positions=i(4))
   with pytest.raises(_lib.B200QError): paged.attention(c, b, P, P, 3)
+  for big in ((1 << 31, 1, 9), (2, 1 << 32, 9), (2, 1, (1 << 32) + 9)):
+    with pytest.raises(ValueError, match="31 bits"): paged.PagedBatch(i(3), i(2), i(2, 5), *big)
+  with pytest.raises(ValueError, match="31 bits"): paged.PagedCache((1 << 32) + 4, 16, 2, 64, k=P, v=P)
+
+
+def test_views_of_rows_that_lie_apart():
+  """A foreign tensor's nbytes counts its values, not what lies between its rows."""
+  import torch
+  big = torch.zeros(3, 100)
+  paged._short(big[:, :64], (2 * 100 + 64) * 4, "x")
+  paged._short(big[:, 36:], (2 * 100 + 64) * 4, "x")
+  with pytest.raises(ValueError, match="x has"): paged._short(big[:, 37:], (2 * 100 + 64) * 4, "x")
+  with pytest.raises(ValueError, match="x has"): paged._short(big[1:, :64], (2 * 100 + 64) * 4, "x")

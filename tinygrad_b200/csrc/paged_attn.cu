@@ -12,6 +12,7 @@ namespace {
 
 __device__ int g_paged_attn_status = 0;
 
+constexpr int N_SM = 148;      // of a B200
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct AttnParams {
@@ -24,7 +25,8 @@ struct AttnParams {
   Divisor by_group, by_kv, by_page;
   int tiles_per_seq;         // 0: tiles are counted sequence by sequence
   int above, up_to;          // sequences with above < new tokens <= up_to (those with others are another kernel's)
-  int n_split, split_len, n_sm, late;
+  int n_split, split_len, late;      // late: behind the kernel for few rows of the same call
+  uint32_t most_rounds;      // of the rows kernel, by the host's bounds
   int* counters;
   float* parts;
   PagedTables t;
@@ -41,8 +43,9 @@ __device__ __forceinline__ SeqPlace place_of_seq(const AttnParams& p, int s) {
   const int64_t room = (int64_t)t.table_stride * t.page_size;
   return SeqPlace{b, n > p.above && n <= p.up_to ? n : 0, (int)min((int64_t)min(max(length, 0), t.max_len), room), length - (e - b)};
 }
+__device__ __forceinline__ bool goes_back(const PagedTables& t, int s) { return t.row_off[s + 1] < t.row_off[s]; }
 __device__ __forceinline__ void check_place(const AttnParams& p, int s, const SeqPlace& q) {      // what the tables promise and the bounds do not hold
-  if (min(max(p.t.row_off[s + 1], q.first_row), p.t.n_rows) - q.first_row > q.n || p.t.length[s] > q.cap) atomicExch(&g_paged_attn_status, 2);
+  if (q.n == 0 ? goes_back(p.t, s) : min(max(p.t.row_off[s + 1], q.first_row), p.t.n_rows) - q.first_row > q.n || p.t.length[s] > q.cap) atomicExch(&g_paged_attn_status, 2);
 }
 template <int R>
 __device__ __forceinline__ TilePlace tile_of_seq(const AttnParams& p, int s, const SeqPlace& q, int tile) {
@@ -64,6 +67,7 @@ __device__ __forceinline__ TilePlace place_of_tile(const AttnParams& p, int tile
   } else {
     bool found = false;
     for (int s0 = 0; s0 < t.n_seqs && !found; s0 += 32) {
+      if (s0 + lane < t.n_seqs && goes_back(t, s0 + lane)) atomicExch(&g_paged_attn_status, 2);
       const int mine = s0 + lane < t.n_seqs ? (place_of_seq(p, s0 + lane).n * p.group + R - 1) / R : 0;
       int sum = mine;
 #pragma unroll
@@ -79,8 +83,8 @@ __device__ __forceinline__ TilePlace place_of_tile(const AttnParams& p, int tile
     if (!found) return TilePlace{};
   }
   const SeqPlace q = place_of_seq(p, s);
-  if (tile * R >= q.n * p.group) return TilePlace{};
   if (lane == 0 && tile == 0) check_place(p, s, q);
+  if (tile * R >= q.n * p.group) return TilePlace{};
   return tile_of_seq<R>(p, s, q, tile);
 }
 
@@ -281,7 +285,7 @@ namespace {
 
 // ---- how the work is dealt ----
 constexpr int MAX_PARTS = 296;      // of a tile's keys: their shares of 16 rows take 19 KB of shared memory (of 256 rows, 64 parts at most, 64 KB)
-struct Plan { int tiles, tiles_per_seq, n_split, split_len, above, up_to, ctas; int64_t rounds; size_t bytes; };      // bytes: of the parts in the workspace
+struct Plan { int64_t tiles; int tiles_per_seq, n_split, split_len, above, up_to, ctas; int64_t rounds; size_t bytes; };      // tiles x KV heads past 2^31 and rounds of -1: too large; bytes: of the parts in the workspace
 
 // Tiles of `rows` pairs: those of all sequences at their largest, or (ragged batches, if that is less) the pairs' tiles and a broken one for each sequence.  Keys are split until
 // there are about `want` CTAs, in parts of at least `least` keys.
@@ -291,9 +295,9 @@ Plan make_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group
   Plan p{};
   p.above = above; p.up_to = up_to;
   p.tiles_per_seq = even <= ragged ? (int)per : 0;
-  p.tiles = (int)(even <= ragged ? even : ragged);
+  p.tiles = even <= ragged ? even : ragged;
   const int64_t len = b->max_len > 0 ? b->max_len : 1, most = (len + least - 1) / least;
-  const int64_t parts = want / ((int64_t)p.tiles * n_kv);
+  const int64_t parts = p.tiles > INT32_MAX / n_kv ? 0 : want / (p.tiles * n_kv);
   const int64_t n = std::min(std::max(std::min(parts, most), (int64_t)1), (int64_t)most_parts);
   p.split_len = (int)(((len + n - 1) / n + unit - 1) / unit * unit);
   p.n_split = (int)((len + p.split_len - 1) / p.split_len);      // at most want
@@ -303,15 +307,15 @@ Plan make_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group
 
 // The workspace begins with the counters of the tiles that are split, MAX_UNITS for each kernel of a call: a fixed place, whatever calls share the workspace.  Tiles x KV heads are split only
 // where they are at most half of the CTAs that are wanted.
-constexpr int N_SM = 148, MAX_UNITS = 2048, ROWS_CTAS = 2 * N_SM, MOST_CTAS = 4 * N_SM;      // of a B200
+constexpr int MAX_UNITS = 2048, ROWS_CTAS = 2 * N_SM, MOST_CTAS = 4 * N_SM;
 constexpr size_t COUNTERS_BYTES = 2 * MAX_UNITS * sizeof(int);
 static_assert(MOST_CTAS / 2 <= MAX_UNITS && ROWS_CTAS <= MAX_UNITS, "counters");
 
 // The rows kernel: as many CTAs as run at once, or as there is work for; parts of every CTA
 Plan rows_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group, int above, int up_to) {
   Plan p = make_plan(c, b, group, above, up_to, 16, 1, 1, ROUND, 1);
-  p.rounds = (int64_t)p.tiles * c->n_kv_heads * (std::max<int64_t>(1, ((int64_t)b->max_len + ROUND - 1) / ROUND) + R_EXTRA);
-  p.ctas = (int)std::min(p.rounds, (int64_t)ROWS_CTAS);
+  p.rounds = p.tiles > INT32_MAX / c->n_kv_heads ? -1 : p.tiles * c->n_kv_heads * (std::max<int64_t>(1, ((int64_t)b->max_len + ROUND - 1) / ROUND) + R_EXTRA);
+  p.ctas = (int)std::min<uint64_t>(p.rounds, ROWS_CTAS);
   p.bytes = (size_t)p.ctas * 2 * 16 * (c->head_dim + 2) * 4;
   return p;
 }
@@ -409,16 +413,19 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
   memset(boxes, 0, sizeof(boxes));
   bool have_boxes = pages_have_boxes(cache);
   Deal deal = deal_of(cache, batch, group, pages_for_tiles(cache) && (parts == 1 || cache->dtype == B200Q_F16));
-  if (a->workspace_bytes < deal.bytes || (deal.bytes && !a->workspace)) return B200Q_ERR_TOO_LARGE;
+  auto fits = [&](const Deal& d) {
+    for (int i = 0; i < d.n; i++)
+      if (d.plan[i].rounds < 0 || d.plan[i].rounds > INT32_MAX || d.plan[i].n_split > 65535 || n_kv > 65535 || d.plan[i].tiles > INT32_MAX / n_kv) return B200Q_ERR_TOO_LARGE;
+    return a->workspace_bytes < d.bytes || (d.bytes && !a->workspace) ? B200Q_ERR_TOO_LARGE : B200Q_OK;
+  };
+  if ((rc = fits(deal)) != B200Q_OK) return rc;
   for (int i = 0; i < 4 && have_boxes; i++) {
     if (i < 2 ? deal.many && deal.n == 1 : !deal.many) continue;
     rc = make_page_map(boxes + i, cache, i & 1 ? cache->v : cache->k, i < 2 ? KB : box_rows_of(cache));
     if (rc == B200Q_ERR_UNSUPPORTED) { have_boxes = false; deal = deal_of(cache, batch, group, false); }      // strides that no map can have; b200q_paged_attention_workspace_bytes knows both deals
     else if (rc != B200Q_OK) return rc;
   }
-  if (a->workspace_bytes < deal.bytes) return B200Q_ERR_TOO_LARGE;
-  for (int i = 0; i < deal.n; i++)
-    if (deal.plan[i].rounds > INT32_MAX || deal.plan[i].n_split > 65535 || n_kv > 65535 || (int64_t)deal.plan[i].tiles * n_kv > INT32_MAX) return B200Q_ERR_TOO_LARGE;
+  if ((rc = fits(deal)) != B200Q_OK) return rc;
   const cudaStream_t st = (cudaStream_t)stream;
   for (int k = 0; k < deal.n; k++) {
     const int i = deal.n - 1 - k, late = k > 0;      // few rows first: their CTAs are short, and the tiles' begin where they leave room
@@ -427,7 +434,7 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
     float* const parts_at = (float*)((char*)a->workspace + COUNTERS_BYTES + (i ? deal.plan[0].bytes : 0));
     const AttnParams p{a->q, cache->k, cache->v, a->out, a->q_dtype, a->out_dtype, a->q_stride ? a->q_stride : row, a->out_stride ? a->out_stride : row, cache->page_stride,
                        cache->head_stride, cache->row_stride, a->n_heads, n_kv, group, (a->scale > 0.f ? a->scale : 1.f / sqrtf((float)dim)) * LOG2E, divisor_of(group), divisor_of(n_kv), divisor_of(cache->page_size), plan.tiles_per_seq, plan.above, plan.up_to,
-                       plan.n_split, plan.split_len, N_SM, late, counters, parts_at, tables_of(cache, batch)};
+                       plan.n_split, plan.split_len, late, (uint32_t)plan.rounds, counters, parts_at, tables_of(cache, batch)};
     const bool pdl = late || (flags & B200Q_FLAG_PDL);
     const int type = cache->dtype == B200Q_BF16;
     if (deal.many && i == 0) {
@@ -435,12 +442,12 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
       const TilesKernel kernel = dim == 64 ? pick_tiles<64>(cache->dtype, parts, &smem) : pick_tiles<128>(cache->dtype, parts, &smem);
       static PerDeviceFlag allowed[2][2][2];
       if ((rc = allow_smem(kernel, smem, allowed[type][parts - 1][dim == 128])) != B200Q_OK) return rc;
-      B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.tiles * n_kv, plan.n_split), dim3(T_THREADS), (size_t)smem, st, pdl, p, boxes[2], boxes[3], box_rows_of(cache)));
-      if (plan.n_split > 1) B200Q_CHECK_CUDA(launch_k(dim == 64 ? join_tiles_kernel<64> : join_tiles_kernel<128>, dim3(plan.tiles * n_kv, J_SLICES), dim3(J_THREADS), 0, st, true, p));
+      B200Q_CHECK_CUDA(launch_k(kernel, dim3((unsigned)plan.tiles * n_kv, plan.n_split), dim3(T_THREADS), (size_t)smem, st, pdl, p, boxes[2], boxes[3], box_rows_of(cache)));
+      if (plan.n_split > 1) B200Q_CHECK_CUDA(launch_k(dim == 64 ? join_tiles_kernel<64> : join_tiles_kernel<128>, dim3((unsigned)plan.tiles * n_kv, J_SLICES), dim3(J_THREADS), 0, st, true, p));
       continue;
     }
     if (cache->dtype == B200Q_F32) {
-      B200Q_CHECK_CUDA(launch_k(pick_simple(dim), dim3(plan.tiles, n_kv, plan.n_split), dim3(S_THREADS), (size_t)(plan.n_split * S_R * 4), st, pdl, p));
+      B200Q_CHECK_CUDA(launch_k(pick_simple(dim), dim3((unsigned)plan.tiles, n_kv, plan.n_split), dim3(S_THREADS), (size_t)(plan.n_split * S_R * 4), st, pdl, p));
       continue;
     }
     const int d = dim == 16 ? 0 : dim == 32 ? 1 : dim == 64 ? 2 : 3, smem = R_RING_OF[d] + (parts == 1 ? 1 : type ? 3 : 2) * 16 * dim * 2 + 1024;

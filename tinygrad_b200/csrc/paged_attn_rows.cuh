@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
     Work v{0, 0};
     if (s < p.t.n_seqs) {
       const SeqPlace q = place_of_seq(p, s);
-      if (blockIdx.x == 0 && warp == 0 && q.n) check_place(p, s, q);
+      if (blockIdx.x == 0 && warp == 0) check_place(p, s, q);
       v.units = units_of(q);
       v.rounds = v.units * rounds_of(q);
     }
@@ -154,8 +154,9 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
     all.units += __shfl_sync(0xffffffffu, sums.units, 31);
     all.rounds += __shfl_sync(0xffffffffu, sums.rounds, 31);
   }
+  if (all.rounds > p.most_rounds) return;                  // row_off goes back (check_place reports it), so that sequences overlap: work that has no bound
   // A unit costs its rounds and, where shares are long, what it takes to begin and end one.  A share that would begin or end in that part does so where the unit begins.
-  const uint32_t ctas = min(gridDim.x, max(min(all.rounds, (uint32_t)p.n_sm), all.rounds / R_LEAST)), c = blockIdx.x;
+  const uint32_t ctas = min(gridDim.x, max(min(all.rounds, (uint32_t)N_SM), all.rounds / R_LEAST)), c = blockIdx.x;
   if (c >= ctas) return;
   const uint32_t extra = all.rounds / ctas >= R_LONG ? R_EXTRA : 0, total = all.rounds + extra * all.units;
   const uint32_t share = total / ctas, more = total - share * ctas, x_end = (c + 1) * share + min(c + 1, more);      // one more for the first `more` CTAs

@@ -42,7 +42,13 @@ def _ptr(o) -> int:
 
 def _short(o, nbytes: int, what: str) -> None:
   have = getattr(o, "nbytes", None)      # (a raw address says nothing)
-  if type(have) is int and have < nbytes: raise ValueError(f"{what} has {have} bytes, needs {nbytes}")
+  if type(have) is int and have < nbytes:
+    if hasattr(o, "untyped_storage"): have = o.untyped_storage().nbytes() - o.storage_offset() * o.element_size()      # a view of rows that lie apart: nbytes counts its values alone
+    if have < nbytes: raise ValueError(f"{what} has {have} bytes, needs {nbytes}")
+
+
+def _fits(*values) -> None:
+  if max(values) >= 1 << 31: raise ValueError(f"{max(values)} does not fit into 31 bits")
 
 
 _words = set()     # types that have been seen to be int32
@@ -61,6 +67,7 @@ class PagedCache:
   slot; the default is [page][head][slot][head_dim]."""
   def __init__(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype="float16", k=None, v=None, strides: tuple = None):
     if min(n_pages, page_size, n_kv_heads, head_dim) <= 0: raise ValueError("pages, page size, heads and head size are at least 1")
+    _fits(n_pages, page_size, n_kv_heads, head_dim)
     if (k is None) != (v is None): raise ValueError("give both pools or neither")
     self.n_pages, self.page_size, self.n_kv_heads, self.head_dim, self.dtype = n_pages, page_size, n_kv_heads, head_dim, _dtype(dtype)
     page, head, row = self.strides = tuple(strides) if strides is not None else (n_kv_heads * page_size * head_dim, page_size * head_dim, head_dim)
@@ -79,6 +86,7 @@ class PagedBatch:
   graph); n_rows (rows of the row arrays), max_new and max_len (of any sequence) are bounds that hold for all of them."""
   def __init__(self, row_off, length, pages, n_rows: int, max_new: int, max_len: int):
     if min(n_rows, max_new, max_len) < 0: raise ValueError("bounds are not negative")
+    _fits(n_rows, max_new, max_len)
     (n_seqs,), (seqs, table) = length.shape, pages.shape
     if seqs != n_seqs or tuple(row_off.shape) != (n_seqs + 1,): raise ValueError(f"row_off {tuple(row_off.shape)}, length {tuple(length.shape)} and pages {tuple(pages.shape)} do not match")
     if n_seqs and table < 1: raise ValueError("a sequence has at least one entry in the table of pages")
@@ -95,9 +103,9 @@ class PagedBatch:
     need = _fn("b200q_paged_attention_workspace_bytes")(cache.ref, self.ref, n_heads)
     if need and (self._ws is None or self._ws.nbytes < need):
       if self._ws is not None: self._old.append(self._ws)      # graphs may hold it
-      self._ws = DeviceBuffer(need)
+      self._ws = DeviceBuffer.result((need,), np.uint8)          # (from the pool: a batch may live as briefly as a step)
       check(_lib.load().b200q_memset(self._ws.ptr, 0, WORKSPACE_HEAD, None))
-      synchronize()
+      synchronize()                                              # whatever stream the first call is on
     self._ready.add((cache._key, n_heads))
 
 
