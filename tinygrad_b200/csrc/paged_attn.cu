@@ -3,8 +3,9 @@
 // in one pass over the keys with the running maximum and sums of the softmax (32-bit); KV head h / G serves the G query heads of its group.
 //
 // Work is dealt as (tile of rows, KV head, part of the keys).  A tile is R consecutive (token, head of the group) pairs of one sequence, token-major, so the group's heads share every key
-// that is loaded.  The keys are split over CTAs where the tiles alone do not fill the GPU: parts leave (m, sum, weighted sum) in the workspace and the one that is done
-// last adds them, in the order of the keys (results do not depend on timing), and puts its counter back.
+// that is loaded.  Three kernels share the work: sequences of few rows (paged_attn_rows.cuh), of many (paged_attn_tiles.cuh), and what neither takes (fp32 pages; below).  The keys are split over
+// CTAs where the tiles alone do not fill the GPU: parts leave (m, sum, weighted sum) in the workspace, and the one that is done last (a kernel behind it, for the tiles of many rows)
+// adds them in the order of the keys, so that results do not depend on timing, and puts the counter back.
 #include "paged.cuh"
 #include <algorithm>
 
@@ -320,7 +321,9 @@ Plan rows_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group
   return p;
 }
 
-constexpr int FEW_PAIRS = 64;      // (token, head) pairs of a sequence that the rows kernel takes
+// (token, head) pairs of a sequence that the rows kernel takes.  It reads the keys again for every 16 of them; the tiles kernel's tiles are 256 pairs of which few may be rows.  us with 16 / 32 / 64 / 128: 8
+// sequences of up to 16 new tokens x 4 heads and 4000 positions 59 / 66 / 43 / 43, 12 of up to 700 and 3000 62 / 62 / 62 / 70.
+constexpr int FEW_PAIRS = 64;
 // The kernels of a call and their shares of it.  many: sequences of more than FEW_PAIRS pairs go to the tiles kernel.
 struct Deal { bool many; int n; Plan plan[2]; size_t bytes; };
 Deal deal_of(const b200q_paged_cache* c, const b200q_paged_batch* b, int group, bool tiles_take) {

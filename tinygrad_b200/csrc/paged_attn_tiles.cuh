@@ -1,10 +1,17 @@
 // Attention over pages for many rows (prompts and chunks): paged_attn.cu includes this.
 //
-// Bound by the tensor core and, as much, by the exponentials: 256 rows x 128 keys are 2 x 256 x 128 x D multiply-adds (2048 cycles of the tensor core at D = 128) and 32768 powers (2048
-// cycles of the special-function units).  So a CTA has two tiles of 128 rows whose products and softmaxes take turns: while one's scores are turned into probabilities, the other's
-// products run.  Warps 0-3 and 4-7 are the tiles' softmax, a thread a row (scores are read from tensor memory as it holds them, no exchange between threads); one
-// thread issues the products, S = Q K^T from shared memory and O += P V with P from tensor memory, where it takes the place of the scores; one warp brings keys and values (TMA boxes of a page's
-// rows, 128-byte swizzle), two look after the values that a product must not see.  Tensor memory: S0 S1 O0 O1, 128 columns each.
+// Bound by the tensor core and, as much, by what turns scores into probabilities: 256 rows x 128 keys are 2 x 256 x 128 x D multiply-adds (2048 cycles of the tensor core at D = 128), 32768 powers
+// (2048 cycles of the special-function units) and some 600 instructions of each of the eight warps that see them.  So a CTA has two tiles of 128 rows whose products and softmaxes take turns: while one's
+// scores are turned into probabilities, the other's products run.  Warps 0-3 and 4-7 are the tiles' softmax, a thread a row (scores are read from tensor memory as it holds them, no exchange between
+// threads; two threads a row, half of its scores each, were slower); one thread issues the products, S = Q K^T from shared memory and O += P V with P from tensor memory; one warp brings keys, one values (TMA
+// boxes of a page's rows, 128-byte swizzle), one looks after the values that a product must not see.  With heads of 128 a quarter of the powers is a polynomial on the multiply-adders (none, a quarter, a third,
+// half of them: 372, 367, 364, 405 us below; with heads of 64, whose time is issued instructions, 302, 312, 318, 342).  A tile's product begins with half of its probabilities.
+//
+// Tensor memory: S0 S1 O0 O1, 128 columns each, a tile's probabilities in the place of its scores.  Heads of 64 leave room for probabilities of their own (T_APART): the next scores
+// are then computed as soon as these have been read, not behind their product (4096 rows of 32 heads of 64, 8192 positions: 302 us, 315 in place).
+//
+// 4096 rows of 32 heads of 128 at 8192 positions: 365 to 400 us, as the power limit has the clock (1.0 to 1.1 PFLOP/s).  CTAs that stay and share the work evenly took 442 us there,
+// softmaxes that are kept apart by barriers 406 against 391, a running maximum looked for behind the first powers 399 against 388.
 //
 // The running maximum moves only when it has grown by 2^8: until then probabilities are relative to an older one, which the quotient does not notice, and the weighted sums
 // in tensor memory stay as they are.
@@ -18,11 +25,12 @@ namespace {
 constexpr int T_ROWS = 128, T_R = 2 * T_ROWS, T_KEYS = 128, T_THREADS = 384, T_BASE = 7, T_PARTS = 16;      // probabilities up to 2^(7 + 8)
 template <int D> constexpr int T_TILE = T_KEYS * D * 2;                                     // bytes of 128 rows of 16-bit values
 template <int D, int N> constexpr int T_KS = D == 64 ? 3 : N == 1 ? 2 : 1;
+template <int D, int N> constexpr bool T_APART = D == 64 && N == 1;      // probabilities have columns of their own
 template <int D, int N> constexpr int T_VS = D == 64 ? 3 : N == 1 ? 3 : 2;
 template <int D, int N> constexpr int T_SMEM = (2 * N + T_KS<D, N> + T_VS<D, N>) * T_TILE<D> + 1024;
 
 struct SharedA {
-  uint64_t k_full[3], k_empty[3], v_full[3], v_clean[3], v_empty[3], s_full[2], p_full[2][2], q_full, o_full;
+  uint64_t k_full[3], k_empty[3], v_full[3], v_clean[3], v_empty[3], s_full[2], s_free[2], p_full[2][2], p_free[2], q_full, o_full;
   uint32_t tmem;
   int abort, flag, bad_lo, bad_hi;
 };
@@ -136,6 +144,8 @@ __device__ __forceinline__ void add_not_finite(const AttnParams& p, int seq, int
 template <int D, int N, bool BF>
 __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, int box_rows) {
   constexpr int SUBS = D / 64, TILE = T_TILE<D>, SUB = T_KEYS * 128, KS = T_KS<D, N>, VS = T_VS<D, N>, KK = D / 16;
+  constexpr bool APART = T_APART<D, N>, POLY = D == 128;
+  constexpr int O_AT = 256, O_STEP = APART ? 64 : 128, P_AT = APART ? 384 : 0, P_STEP = APART ? 64 : 128, P_CHUNK = APART ? 16 : 32;      // columns of tensor memory
   extern __shared__ unsigned char raw[];
   __shared__ SharedA sh;
   // Behind the kernel for few rows of the same call (late): both read what was there before that one began and write rows of their own, so that this one waits for it only at its end.
@@ -164,7 +174,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
     for (int i = 0; i < 3; i++) {
       a_bar_init(&sh.k_full[i], 1); a_bar_init(&sh.k_empty[i], 1); a_bar_init(&sh.v_full[i], 1); a_bar_init(&sh.v_clean[i], 1); a_bar_init(&sh.v_empty[i], 1);
     }
-    for (int i = 0; i < 2; i++) { a_bar_init(&sh.s_full[i], 1); a_bar_init(&sh.p_full[i][0], 4); a_bar_init(&sh.p_full[i][1], 4); }
+    for (int i = 0; i < 2; i++) { a_bar_init(&sh.s_full[i], 1); a_bar_init(&sh.s_free[i], 4); a_bar_init(&sh.p_free[i], 1); a_bar_init(&sh.p_full[i][0], 4); a_bar_init(&sh.p_full[i][1], 4); }
     a_bar_init(&sh.q_full, 8); a_bar_init(&sh.o_full, 1);
     sh.abort = sh.flag = 0; sh.bad_lo = INT32_MAX; sh.bad_hi = -1;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -268,7 +278,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
 #pragma unroll
       for (int d = 0; d < D; d++) acc[d] = 0.f;
     }
-    const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * 128, to = ts + 256;
+    const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * 128, to = ts + O_AT - t * (128 - O_STEP), tp = ts + P_AT - t * (128 - P_STEP);
     const int warp_first = __shfl_sync(0xffffffffu, me.last, 0);      // no row of the warp sees less (rows without a token see nothing, and are not stored)
     bool ok = t == 0 || two;
     float scaled = 1.f;      // N == 2: what the sum in registers is multiplied by before a tile's is added
@@ -286,6 +296,11 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
 #pragma unroll
         for (int c = 0; c < 4; c++) ld32(ts + c * 32, reinterpret_cast<uint32_t*>(s) + c * 32);
         wait_ld();
+        if constexpr (APART) {
+          fence_before();
+          __syncwarp();
+          if (lane == 0) a_bar_arrive(&sh.s_free[t]);
+        }
         if (masked) {
 #pragma unroll
           for (int i = 0; i < 128; i++) s[i] = i <= lim ? s[i] : -INFINITY;
@@ -300,6 +315,11 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
         for (int q = 0; q < 4; q++) tops[q] = max3(tops[q], s[124 + q], s[124 + q]);
         top = max3(tops[0], tops[1], max3(tops[2], tops[3], tops[3])) * qs;
         if (!(top < INFINITY)) { l = __uint_as_float(0x7FC00000u); top = m; }      // a score that is infinite or NaN: the row is NaN, whatever takes its exponentials
+        if constexpr (APART) {      // the product of the tile before has its probabilities, and its sum is there
+          if (j > 0) ok = __all_sync(0xffffffffu, a_wait(sh, &sh.p_free[t], (j - 1) & 1));
+          if (!ok) break;
+          fence_after();
+        }
         const bool moves = j == 0 || top > m + 8.f;
         if (__any_sync(0xffffffffu, moves)) {
           const float mn = fmaxf(m, top), f = mn == -INFINITY ? 1.f : pow2(m - mn);
@@ -327,13 +347,13 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
 #pragma unroll
             for (int i = 0; i < 16; i++) {
               uint64_t x = fma2(pair_of(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), qs2, sub2);
-              if (some.value && i % 4 == 3) x = pow2_poly<BF>(x);
+              if (POLY && some.value && i % 4 == 3) x = pow2_poly<BF>(x);
               else { const float2 y = floats_of(x); x = pair_of(pow2(y.x), pow2(y.y)); }
               sums[i & 1] = add2(sums[i & 1], x);
               const float2 y = floats_of(x);
               pk[i] = pack2(y.x, y.y, BF ? B200Q_BF16 : B200Q_F16);
             }
-            st16(ts + c * 32, pk);
+            st16(tp + c * P_CHUNK, pk);
             if (c & 1) {      // half of the tile's probabilities: the product begins with them
               wait_st();
               fence_before();
@@ -510,8 +530,18 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
       for (int j = 0; ok && j < tiles; j++) {
         const int vs = j % VS, kn = (j + 1) % KS;
         const uint32_t v = v0 + vs * (TILE >> 4);
-        ok = a_wait(sh, &sh.v_clean[vs], (j / VS) & 1);
+        if constexpr (!APART) ok = a_wait(sh, &sh.v_clean[vs], (j / VS) & 1);
         for (int t = 0; ok && t < 1 + two; t++) {
+          if constexpr (APART) {      // the next scores as soon as these have been read
+            if (j + 1 < tiles) {
+              ok = (t == 1 || a_wait(sh, &sh.k_full[kn], ((j + 1) / KS) & 1)) && a_wait(sh, &sh.s_free[t], j & 1);
+              if (!ok) break;
+              fence_after();
+              scores(t, kn);
+              if (t == two) a_commit(&sh.k_empty[kn]);
+            }
+            if (t == 0) ok = a_wait(sh, &sh.v_clean[vs], (j / VS) & 1);
+          }
           // the probabilities come in two halves; their small parts first
 #pragma unroll
           for (int h = 0; h < 2; h++) {
@@ -522,12 +552,13 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
             for (int i = N - 1; i >= 0; i--)
 #pragma unroll
               for (int kk = h * 4; kk < h * 4 + 4; kk++)
-                mma_ts_a(tmem + 256 + t * 128, tmem + t * 128 + (N == 1 ? (kk / 2) * 32 + (kk & 1) * 8 : kk * 16 + i * 8), v + kk * (2048 >> 4), ID_O,
+                mma_ts_a(tmem + O_AT + t * O_STEP, tmem + P_AT + t * P_STEP + (N == 1 ? (kk / 2) * P_CHUNK + (kk & 1) * 8 : kk * 16 + i * 8), v + kk * (2048 >> 4), ID_O,
                          h > 0 || i < N - 1 || kk > 0 || (N == 1 && j > 0));
           }
           if (!ok) break;
           if (t == two) a_commit(&sh.v_empty[vs]);
-          if (j + 1 < tiles) {
+          if constexpr (APART) a_commit(&sh.p_free[t]);
+          else if (j + 1 < tiles) {
             if (t == 0) { ok = a_wait(sh, &sh.k_full[kn], ((j + 1) / KS) & 1); if (!ok) break; fence_after(); }
             scores(t, kn);
             if (t == two) a_commit(&sh.k_empty[kn]);
