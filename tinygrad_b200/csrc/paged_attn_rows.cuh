@@ -34,14 +34,15 @@ __device__ __forceinline__ bool bar_ready(uint64_t* b, uint32_t parity) {
   asm volatile("{\n.reg .pred p;\nmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(s_addr(b)), "r"(parity) : "memory");
   return ok;
 }
-// Bounded wait: false once another role has given up, or when the time is over (then the others are told).
+// Bounded wait: false when the time is over (then the others are told), or once another has given up and a little longer has not helped: what was in flight has had its time before
+// anything else happens to its place, or the kernel ends.
 __device__ __forceinline__ bool a_wait_on(uint32_t bar, uint32_t parity, uint32_t abort) {
   for (int i = 0; i < (1 << 20); i++) {
     uint32_t ok, gone;
     asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(ok) : "r"(bar), "r"(parity), "r"(2000) : "memory");
     if (ok) return true;
     asm volatile("ld.volatile.shared::cta.u32 %0, [%1];" : "=r"(gone) : "r"(abort) : "memory");
-    if (gone) return false;
+    if (gone && i >= 1000) return false;
   }
   asm volatile("st.volatile.shared::cta.u32 [%0], 1;" ::"r"(abort) : "memory");
   atomicExch(&g_paged_attn_status, 1);
