@@ -321,8 +321,8 @@ Plan rows_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group
   return p;
 }
 
-// (token, head) pairs of a sequence that the rows kernel takes.  It reads the keys again for every 16 of them; the tiles kernel's tiles are 256 pairs of which few may be rows.  us with 16 / 32 / 64 / 128: 8
-// sequences of up to 16 new tokens x 4 heads and 4000 positions 59 / 66 / 43 / 43, 12 of up to 700 and 3000 62 / 62 / 62 / 70.
+// (token, head) pairs of a sequence that the rows kernel takes.  It reads the keys again for every 16 of them, mostly from L2; the tiles kernel's tiles are 256 pairs of which few may be rows.  us with 16 / 32 / 64
+// / 128: 8 sequences of up to 16 new tokens x 4 heads and 4000 positions 58 / 62 / 44 / 44, of up to 32 tokens 57 / 63 / 68 / 62, 12 of up to 700 and 3000 positions 60 / 60 / 60 / 69.
 constexpr int FEW_PAIRS = 64;
 // The kernels of a call and their shares of it.  many: sequences of more than FEW_PAIRS pairs go to the tiles kernel.
 struct Deal { bool many; int n; Plan plan[2]; size_t bytes; };

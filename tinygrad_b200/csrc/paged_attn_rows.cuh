@@ -23,8 +23,11 @@ constexpr int RW = 4, R_THREADS = RW * 32, KB = 16;
 template <int D> constexpr int R_BLOCK = KB * D * 2;                                      // bytes of a block's keys (or values)
 template <int D> constexpr int R_STAGES = D == 128 ? 3 : D == 64 ? 6 : 8;
 template <int D> constexpr int R_RING = RW * R_STAGES<D> * 2 * R_BLOCK<D> > RW * 16 * D * 4 ? RW * R_STAGES<D> * 2 * R_BLOCK<D> : RW * 16 * D * 4;
-constexpr int ROUND = RW * KB, R_LEAST = 4;                // positions of a round; rounds that a CTA has at least, where there are enough for an SM each
-constexpr uint32_t R_LONG = 12, R_EXTRA = 4;           // rounds of a share from which the beginning and end of a unit count as R_EXTRA rounds
+// ROUND: positions of a round.  R_LEAST: rounds that a CTA has at least, where there are enough for an SM each.  R_LONG: rounds of a share from which the beginning and end of a unit count as R_EXTRA
+// rounds.  us with 4 KV heads of 7 x 128, sequences of one new token, at 64 x 1000 / 32 x 1000 / 64 x 200 / 16 x 1000 / 3 x 8000 positions at most: R_LONG 12, R_LEAST 4 44.1 / 26.9 / 24.9 / 22.8 / 20.7 (units cut
+// wherever a share ends, each in its two parts); R_LONG 2 27.7 / 20.7 / 22.2 / 18.7 / 20.7; R_LEAST 2 with it 27.6 / 18.8 / 18.7 / 16.7 / 22.8.  R_EXTRA 3 to 5 within 3 % of one another, 8: 31.0 / 22.8.
+constexpr int ROUND = RW * KB, R_LEAST = 2;
+constexpr uint32_t R_LONG = 2, R_EXTRA = 4;
 
 __device__ __forceinline__ uint32_t s_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void a_bar_init(uint64_t* b, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s_addr(b)), "r"(n) : "memory"); }
