@@ -499,12 +499,12 @@ int b200q_tc_status_read_clear(int* status);
  *   max_new rows and max_len tokens of any sequence.
  * What the tables say is checked on the device; nothing outside the arrays is read or written, and the status word (b200q_status_read_clear) becomes 2 where they
  * are wrong: a page that does not exist takes no writes and reads as zeros; a position outside the table's row, below 0 or (append) outside the
- * rotation's table has no cache row; tokens past max_len are not attended; rows past max_new of a sequence get no attention.  Rows that belong to no sequence (n_rows >
+ * rotation's table has no cache row; tokens past max_len are not attended; rows past max_new of a sequence get no attention; row offsets that go back leave it open which rows do.  Rows that belong to no sequence (n_rows >
  * row_off[n_seqs]: a padded batch in a captured graph) are left as they were.
  *
  * b200q_paged_append: rows x = [q | k | v] (x_dtype; x_stride elements apart, 0: back to back) -> per head RMSNorm(q) * q_norm, RMSNorm(k) * k_norm (fp16 [head_dim], NULL: no norm;
  *   tinygrad/nn/__init__.py:300-304 over the head's values), RoPE with half-split pairs in the first rope_dim values (model.py:29-33; rope fp32 [rope_len][rope_dim] cos || sin, NULL: none), then q to
- *   the rows of q (q_dtype, q_stride; may be x's own q part if types and strides agree) and k, v to the sequence's pages.  32-bit arithmetic, each value rounded once.  A row whose position has no
+ *   the rows of q (q_dtype, q_stride; may be x's own q part if types and strides agree) and k, v to the sequence's pages (which no other sequence of the call appends to).  32-bit arithmetic, each value rounded once.  A row whose position has no
  *   entry in `rope` gets zeros in q.
  * b200q_head_norm_rope: the same norms and rotation of the first n_heads + n_kv_heads heads of every row, from x to out (may be x), for callers whose cache is not paged
  *   (b200q_attn_prefill and _decode rotate themselves: rope NULL).  positions [n_rows] (device) is asked for with rope only; one outside the table gives zeros and status 2.
