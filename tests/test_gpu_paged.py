@@ -667,3 +667,65 @@ def test_against_the_contiguous_cache():
   kc = k.numpy()[:, :n].astype(np.float64)
   assert (np.abs(kp[:, :n].astype(np.float64) - kc) <= EPS["float16"] * np.abs(kc) + 2 * TINY["float16"]).all()
   np.testing.assert_allclose(out.numpy(), want, rtol=0, atol=2e-5)
+
+
+@pytest.mark.parametrize("qt,ct,d,seqs", [("float16", "float16", 128, [(200, 700), (1, 300), (9, 60)]), ("bfloat16", "bfloat16", 64, [(90, 3000), (2, 40)]), ("float32", "float16", 128, [(40, 2000)])],
+                         ids=["both kernels", "keys in parts beside tokens", "keys in parts"])
+def test_captured_chunks(qt, ct, d, seqs):
+  """A call of several kernels in a graph: the eager call's bits, and those of other tables after they have changed on the device."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  from tinygrad_b200.runtime import Graph, Stream
+  rng = np.random.default_rng(31)
+  h, hk, ps = 8, 2, 16
+  new, length = [n for n, _ in seqs], [l for _, l in seqs]
+  off, n = np.concatenate([[0], np.cumsum(new)]), sum(new)
+  t, n_pages = table(rng, length, ps)
+  t = np.maximum(t, 0)
+  (k, _), (v, _), (q, _) = (put(rng.standard_normal(s), c) for s, c in (((n_pages, hk, ps, d), ct), ((n_pages, hk, ps, d), ct), ((n, h, d), qt)))
+  cache, lens, pages, stream = paged.PagedCache(n_pages, ps, hk, d, ct, k=k, v=v), i32(length), i32(t), Stream()
+  batch, out = paged.PagedBatch(i32(off), lens, pages, n_rows=n, max_new=max(new), max_len=max(length)), put(np.zeros((n, h, d)), qt)[0]
+  status()
+  batch.reserve(cache, h)
+  graph = Graph(stream)
+  with graph:
+    paged.attention(cache, batch, q, out, h, qt, stream=stream)
+  for now in (length, [max(m, l - 70) for m, l in seqs]):
+    lens.copy_from(np.asarray(now, np.int32))
+    pages.copy_from(np.ascontiguousarray(t[:, ::-1] if now is not length else t))
+    paged.attention(cache, batch, q, out, h, qt)
+    want = out.numpy((n, h, d), np.uint32 if qt == "float32" else np.uint16)
+    for _ in range(3):
+      out.copy_from(np.zeros((n, h, d), want.dtype))
+      graph.launch()
+      stream.synchronize()
+      assert (out.numpy((n, h, d), want.dtype) == want).all()
+  assert status() == 0
+
+
+@pytest.mark.parametrize("seqs", [[(1, 300)] * 5, [(150, 400), (3, 90), (1, 1200)], [(70, 2500)]], ids=["tokens", "both kernels", "keys in parts"])
+def test_a_chain_of_dependent_launches(seqs):
+  """append and attention in turn, each told that the launch before it is the library's own: bits of the calls without that."""
+  need_gpu()
+  from tinygrad_b200 import _lib, paged
+  from tinygrad_b200.runtime import synchronize
+  rng = np.random.default_rng(32)
+  h, hk, d, ps, layers = 8, 2, 64, 16, 6
+  new, length = [n for n, _ in seqs], [l for _, l in seqs]
+  off, n = np.concatenate([[0], np.cumsum(new)]), sum(new)
+  t, n_pages = table(rng, length, ps)
+  old = rng.standard_normal((2, layers, n_pages, hk, ps, d))
+  xs = [put(rng.standard_normal((n, (h + 2 * hk) * d)), "float16")[0] for _ in range(layers)]
+  batch = paged.PagedBatch(i32(off), i32(length), i32(t), n_rows=n, max_new=max(new), max_len=max(length))
+  got = []
+  for flags in (0, _lib.FLAG_PDL):
+    caches = [paged.PagedCache(n_pages, ps, hk, d, "float16", k=put(old[0, i], "float16")[0], v=put(old[1, i], "float16")[0]) for i in range(layers)]
+    q, outs = put(np.zeros((n, h * d)), "float16")[0], [put(np.zeros((n, h * d)), "float16")[0] for _ in range(layers)]
+    batch.reserve(caches[0], h)
+    synchronize()
+    for i in range(layers):      # (q and the workspace are every layer's)
+      paged.append(caches[i], batch, xs[i], q, h, "float16", flags=flags if i else 0)
+      paged.attention(caches[i], batch, q, outs[i], h, "float16", flags=flags)
+    got.append([o.numpy((n, h * d), np.uint16) for o in outs])
+  for a, b in zip(*got): assert (a == b).all()
+  assert any(a.any() for a in got[0])
