@@ -53,8 +53,13 @@ template <int VEC> __device__ __forceinline__ void store_vec(void* base, int typ
     for (int j = 0; j < VEC / 4; j++) d[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
   } else {
     uint32_t w[VEC / 2];
+    if (type == B200Q_F16) {
 #pragma unroll
-    for (int j = 0; j < VEC / 2; j++) w[j] = pack2(f[2 * j], f[2 * j + 1], type);
+      for (int j = 0; j < VEC / 2; j++) w[j] = pack2(f[2 * j], f[2 * j + 1], B200Q_F16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC / 2; j++) w[j] = pack2(f[2 * j], f[2 * j + 1], B200Q_BF16);
+    }
     void* d = static_cast<uint16_t*>(base) + i;
     if constexpr (VEC == 8) *static_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
     else *static_cast<uint2*>(d) = make_uint2(w[0], w[1]);
@@ -146,7 +151,7 @@ __device__ __forceinline__ void do_head(const RowsParams& p, const Pairs<D, VEC>
     for (int o = Pairs<D, VEC>::TPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     const __half* wn = is_q ? p.q_norm : is_k ? p.k_norm : nullptr;
     if (wn) {
-      const float r = 1.f / sqrtf(ss * (1.f / D) + p.eps);
+      const float r = rsqrtf(ss * (1.f / D) + p.eps);      // (within two units of the last place; with a root and a quotient 4096 rows took 1 us more: instructions are half of what bounds this)
 #pragma unroll
       for (int g = 0; g < NG; g++) {
         float wa[VEC], wb[VEC];
@@ -230,7 +235,7 @@ __global__ void __launch_bounds__(ROW_THREADS, IT == 1 && ROWS == 1 ? 6 : IT <= 
 }
 
 // Few rows: a head a thread group.  Many: all heads of a row (of two rows, where nothing has to be looked up) in a CTA, with up to four heads a thread.  us, 4096 rows of 48 fp32 heads of 128,
-// normed, / 4017 of 48 bf16 heads of 64 / norms alone of 8191 x 32 fp16 heads of 128: three heads a thread and five CTAs an SM 38.8 / - / -, one head and six / four 43.7, - / 14.8, 16.6 / 30.9, 29.9, two rows
+// normed, / 4017 of 48 bf16 heads of 64 / norms alone of 8191 x 32 fp16 heads of 128: three heads a thread and five CTAs an SM 37.5 / - / -, one head and six / four 43.7, - / 14.8, 16.6 / 30.9, 29.9, two rows
 // and four CTAs - / 16.6 / 27.8, four rows and two CTAs - / 25.0 / 39.3; rows streamed through shared memory by bulk copies, a warp looking up places ahead, 42.6 / 21.2 / 35.2.
 template <typename X, int D, int VEC>
 int launch_vec(const RowsParams& p, int n_rows, bool pdl, cudaStream_t st) {
