@@ -26,7 +26,7 @@ struct AttnParams {
   Divisor by_group, by_kv, by_page;
   int tiles_per_seq;         // 0: tiles are counted sequence by sequence
   int above, up_to;          // sequences with above < new tokens <= up_to (those with others are another kernel's)
-  int n_split, split_len, late;      // late: behind the kernel for few rows of the same call
+  int n_split, split_len, late;      // late: behind the tiles kernel of the same call
   uint32_t most_rounds;      // of the rows kernel, by the host's bounds
   int* counters;
   float* parts;
@@ -430,15 +430,20 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
   }
   if ((rc = fits(deal)) != B200Q_OK) return rc;
   const cudaStream_t st = (cudaStream_t)stream;
-  for (int k = 0; k < deal.n; k++) {
-    const int i = deal.n - 1 - k, late = k > 0;      // few rows first: their CTAs are short, and the tiles' begin where they leave room
+  auto params = [&](int i, int late) {
     const Plan& plan = deal.plan[i];
     int* const counters = (int*)a->workspace + i * MAX_UNITS;
     float* const parts_at = (float*)((char*)a->workspace + COUNTERS_BYTES + (i ? deal.plan[0].bytes : 0));
-    const AttnParams p{a->q, cache->k, cache->v, a->out, a->q_dtype, a->out_dtype, a->q_stride ? a->q_stride : row, a->out_stride ? a->out_stride : row, cache->page_stride,
+    return AttnParams{a->q, cache->k, cache->v, a->out, a->q_dtype, a->out_dtype, a->q_stride ? a->q_stride : row, a->out_stride ? a->out_stride : row, cache->page_stride,
                        cache->head_stride, cache->row_stride, a->n_heads, n_kv, group, (a->scale > 0.f ? a->scale : 1.f / sqrtf((float)dim)) * LOG2E, divisor_of(group), divisor_of(n_kv), divisor_of(cache->page_size), plan.tiles_per_seq, plan.above, plan.up_to,
                        plan.n_split, plan.split_len, late, (uint32_t)plan.rounds, counters, parts_at, tables_of(cache, batch)};
-    const bool pdl = late || (flags & B200Q_FLAG_PDL);
+  };
+  for (int i = 0; i < deal.n; i++) {
+    // many rows first: once the last of their CTAs has a place, those for few rows begin where others leave room (12 sequences, 1 to 700 new of up to 3000 positions: 52 us, 60 the other way around; 8 of up to
+    // 32 and 4000, whose few rows take longer: 74 and 68)
+    const Plan& plan = deal.plan[i];
+    const AttnParams p = params(i, i > 0);
+    const bool pdl = i > 0 || (flags & B200Q_FLAG_PDL);
     const int type = cache->dtype == B200Q_BF16;
     if (deal.many && i == 0) {
       int smem;
@@ -446,7 +451,6 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
       static PerDeviceFlag allowed[2][2][2];
       if ((rc = allow_smem(kernel, smem, allowed[type][parts - 1][dim == 128])) != B200Q_OK) return rc;
       B200Q_CHECK_CUDA(launch_k(kernel, dim3((unsigned)plan.tiles * n_kv, plan.n_split), dim3(T_THREADS), (size_t)smem, st, pdl, p, boxes[2], boxes[3], box_rows_of(cache)));
-      if (plan.n_split > 1) B200Q_CHECK_CUDA(launch_k(dim == 64 ? join_tiles_kernel<64> : join_tiles_kernel<128>, dim3((unsigned)plan.tiles * n_kv, J_SLICES), dim3(J_THREADS), 0, st, true, p));
       continue;
     }
     if (cache->dtype == B200Q_F32) {
@@ -458,6 +462,11 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
     static PerDeviceFlag allowed[2][2][2][4];
     if ((rc = allow_smem(kernel, smem, allowed[have_boxes][type][parts - 1][d])) != B200Q_OK) return rc;
     B200Q_CHECK_CUDA(launch_k(kernel, dim3(plan.ctas), dim3(R_THREADS), (size_t)smem, st, pdl, p, boxes[0], boxes[1]));
+  }
+  if (deal.many && deal.plan[0].n_split > 1) {
+    const Plan& plan = deal.plan[0];
+    const AttnParams p = params(0, 0);
+    B200Q_CHECK_CUDA(launch_k(dim == 64 ? join_tiles_kernel<64> : join_tiles_kernel<128>, dim3((unsigned)plan.tiles * n_kv, J_SLICES), dim3(J_THREADS), 0, st, true, p));
   }
   return B200Q_OK;
 }

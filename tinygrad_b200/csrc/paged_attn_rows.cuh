@@ -113,7 +113,7 @@ __device__ __forceinline__ float2 load2_as_f(const void* base, int type, int64_t
 }
 
 template <int D, int N, bool BF, bool BOXES>
-__global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+__device__ __forceinline__ void attn_rows(const AttnParams& p, const CUtensorMap& tm_k, const CUtensorMap& tm_v) {
   constexpr int R = 16, CH = D / 8, ST = R_STAGES<D>, BLOCK = R_BLOCK<D>, KK = D / 16, PP = D >= 64 ? D / 64 : 1;
   extern __shared__ unsigned char raw[];
   __shared__ float s_m[RW][R], s_l[RW][R], s_scale[R];
@@ -128,7 +128,8 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fence_async();
   }
-  pdl_wait();
+  // Behind the tiles kernel of the same call (late): both read what was there before that one began and write rows of their own, so that this one waits for it only at its end.
+  if (!p.late) pdl_wait();
   pdl_launch_dependents();
   const int ps = p.t.page_size;
   const bool whole = BOXES || ps % KB == 0;              // a block lies in one page
@@ -500,6 +501,12 @@ __global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const AttnParam
     if constexpr (BOXES) fence_async();      // (what comes next into the ring comes through the other proxy)
     __syncthreads();
   }
+}
+
+template <int D, int N, bool BF, bool BOXES>
+__global__ void __launch_bounds__(R_THREADS, 2) attn_rows_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+  attn_rows<D, N, BF, BOXES>(p, tm_k, tm_v);
+  if (p.late) pdl_wait();
 }
 
 // The map of a pool: [page][KV head][slot][value], boxes of 64 values x box_rows slots in the 128-byte-swizzle layout.

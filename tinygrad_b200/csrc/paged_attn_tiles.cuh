@@ -148,18 +148,14 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
   constexpr int O_AT = 256, O_STEP = APART ? 64 : 128, P_AT = APART ? 384 : 0, P_STEP = APART ? 64 : 128, P_CHUNK = APART ? 16 : 32;      // columns of tensor memory
   extern __shared__ unsigned char raw[];
   __shared__ SharedA sh;
-  // Behind the kernel for few rows of the same call (late): both read what was there before that one began and write rows of their own, so that this one waits for it only at its end.
-  if (!p.late) pdl_wait();
+  pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int order = p.by_kv.div(blockIdx.x), kvh = blockIdx.x - order * p.n_kv, split = blockIdx.y;
   const int tile_index = p.by_kv.div(gridDim.x) - 1 - order;      // long ones first
   const TilePlace w = place_of_tile<T_R>(p, tile_index);
   const int n_parts = w.n == 0 ? 0 : max(1, (w.keys + p.split_len - 1) / p.split_len), k_begin = split * p.split_len, k_end = min(w.keys, k_begin + p.split_len);
-  if (split >= n_parts) {
-    if (p.late) pdl_wait();
-    return;
-  }
+  if (split >= n_parts) return;
   const int tiles = max(0, (k_end - k_begin + T_KEYS - 1) / T_KEYS);
   const int pairs = w.n * p.group;
   const bool two = w.r0 + T_ROWS < pairs;                      // the second tile of rows has some
@@ -655,7 +651,6 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
   __syncthreads();
   fence_after();
   if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
-  if (p.late) pdl_wait();
 }
 
 // The parts of tiles whose keys are split, added in the order of the keys: J_SLICES CTAs for a (tile, KV head); a warp a row, a lane a part for the parts' shares and D / 32 values for the sum.
