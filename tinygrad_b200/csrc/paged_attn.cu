@@ -321,15 +321,16 @@ Plan rows_plan(const b200q_paged_cache* c, const b200q_paged_batch* b, int group
   return p;
 }
 
-// (token, head) pairs of a sequence that the rows kernel takes.  It reads the keys again for every 16 of them, mostly from L2; the tiles kernel's tiles are 256 pairs of which few may be rows.  us with 16 / 32 / 64
-// / 128: 8 sequences of up to 16 new tokens x 4 heads and 4000 positions 58 / 62 / 44 / 44, of up to 32 tokens 57 / 63 / 68 / 62, 12 of up to 700 and 3000 positions 60 / 60 / 60 / 69.
-constexpr int FEW_PAIRS = 64;
-// The kernels of a call and their shares of it.  many: sequences of more than FEW_PAIRS pairs go to the tiles kernel.
+// Batches whose sequences have at most ROWS_PAIRS (token, head) pairs each are the rows kernel's; in others it takes those of at most FEW_PAIRS.  It reads the keys again for every 16 pairs, mostly from L2; the tiles
+// kernel's tiles are 256 pairs of which few may be rows, but another kernel for some of the sequences costs as well.  us, 8 sequences of up to 16 new tokens x 4 heads and 4000 positions: the rows kernel alone 43, both
+// 72.  FEW_PAIRS 16 / 32 / 64 / 128: 8 of up to 32 tokens 52 / 69 / 74 / 62, 12 of up to 170 85 / 98 / 101 / 134, the same of fp32 rows 158 / 159 / 168 / 167, 12 of up to 700 and 3000 positions 52 / 52 / 52 / 68.
+constexpr int ROWS_PAIRS = 64, FEW_PAIRS = 16;
+// The kernels of a call and their shares of it.  many: there is work for the tiles kernel.
 struct Deal { bool many; int n; Plan plan[2]; size_t bytes; };
 Deal deal_of(const b200q_paged_cache* c, const b200q_paged_batch* b, int group, bool tiles_take) {
   Deal d{};
   const int few = FEW_PAIRS / group > 1 ? FEW_PAIRS / group : 1;
-  d.many = tiles_take && b->max_new > few;
+  d.many = tiles_take && (int64_t)b->max_new * group > ROWS_PAIRS && b->max_new > 1;
   if (d.many) {
     d.plan[0] = make_plan(c, b, group, few, INT32_MAX, T_R, N_SM, 512, T_KEYS, T_PARTS);
     d.n = 1;
@@ -439,8 +440,7 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
                        plan.n_split, plan.split_len, late, (uint32_t)plan.rounds, counters, parts_at, tables_of(cache, batch)};
   };
   for (int i = 0; i < deal.n; i++) {
-    // many rows first: once the last of their CTAs has a place, those for few rows begin where others leave room (12 sequences, 1 to 700 new of up to 3000 positions: 52 us, 60 the other way around; 8 of up to
-    // 32 and 4000, whose few rows take longer: 74 and 68)
+    // many rows first: once the last of their CTAs has a place, those for few rows begin where others leave room (12 sequences, 1 to 700 new of up to 3000 positions: 52 us, 60 the other way around)
     const Plan& plan = deal.plan[i];
     const AttnParams p = params(i, i > 0);
     const bool pdl = i > 0 || (flags & B200Q_FLAG_PDL);
