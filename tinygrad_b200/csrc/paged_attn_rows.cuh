@@ -129,7 +129,9 @@ __device__ __forceinline__ void attn_rows(const AttnParams& p, const CUtensorMap
     fence_async();
   }
   // Behind the tiles kernel of the same call (late): both read what was there before that one began and write rows of their own, so that this one waits for it only at its end.
-  if (!p.late) pdl_wait();
+  // (The fence: what is read now must not come from a first-level cache that has seen an earlier call's values.)
+  if (p.late) __threadfence();
+  else pdl_wait();
   pdl_launch_dependents();
   const int ps = p.t.page_size;
   const bool whole = BOXES || ps % KB == 0;              // a block lies in one page
