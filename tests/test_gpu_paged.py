@@ -729,3 +729,76 @@ def test_a_chain_of_dependent_launches(seqs):
     got.append([o.numpy((n, h * d), np.uint16) for o in outs])
   for a, b in zip(*got): assert (a == b).all()
   assert any(a.any() for a in got[0])
+
+
+@pytest.mark.parametrize("qt,ct", [("bfloat16", "bfloat16"), ("float16", "float16"), ("float32", "bfloat16"), ("float32", "float32")])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new,length", [(2, 100), (2, 3000), (200, 400), (200, 3000)], ids=["tokens", "tokens, keys in parts", "chunk", "chunk, keys in parts"])
+def test_scores_of_minus_infinity(qt, ct, d, new, length):
+  """A row whose scores are all minus infinity gets zeros, one with some such scores the others' mean: keys of weight 0 leave nothing behind, however large their values are.  fp16: an infinite query
+  or key gives such a score; the wider types: 2^100 times -2^100."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(new + length)
+  h, hk, ps = 4, 2, 16
+  t, n_pages = table(rng, [length], ps)
+  out_of = np.zeros(length, bool)          # keys that no row gives a weight: the first tiles whole, some of the rest
+  out_of[:min(256, length // 3)] = True
+  out_of |= rng.random(length) < 0.3
+  big, low = (np.inf, -np.inf) if ct == "float16" else (2.0 ** 100, -2.0 ** 100)
+  k, v, q = rng.standard_normal((length, hk, d)), rng.standard_normal((length, hk, d)), rng.standard_normal((new, h, d))
+  k[:, :, 0], q[:, :, 0] = (-1.0 if ct == "float16" else low), 0.0
+  k[:, :, 1], q[:, :, 1] = np.where(out_of, low, 0.0)[:, None], (1.0 if ct == "float16" else big)
+  v[out_of, :, 3] = 60000.0 if ct == "float16" else 2.0 ** 126
+  none = [(0, 0), (new // 2, 3), (new - 1, 1)]
+  for r, j in none: q[r, j, 0] = big
+  pools = []
+  for x in (k, v):
+    pool = np.zeros((n_pages, hk, ps, d), np.float32)
+    p = np.arange(length)
+    pool[t[0][p // ps], :, p % ps] = x
+    pools.append(put(pool, ct))
+  kv = [ref.gather(val, t[0], length, ps) for _, val in pools]
+  qb, qv = put(q, qt)
+  out = put(np.full((new, h, d), 3.0), qt)[0]
+  status()
+  paged.attention(paged.PagedCache(n_pages, ps, hk, d, ct, k=pools[0][0], v=pools[1][0]), paged.PagedBatch(i32([0, new]), i32([length]), i32(t), n_rows=new, max_new=new, max_len=length), qb, out, h, qt)
+  got = get(out, (new, h, d), qt)
+  assert status() == 0
+  want, weight, reach = np.zeros((new, h, d)), np.zeros((new, h, d)), np.zeros((new, h))
+  for r in range(new):
+    sees = ~out_of & (np.arange(length) <= length - new + r)
+    for j in range(h):
+      if (r, j) in none or not sees.any():
+        assert not got[r, j].any(), (r, j)
+        continue
+      kk, vv = kv[0][j // 2][sees, 2:], kv[1][j // 2][sees]
+      s = kk @ qv[r, j, 2:] * d ** -0.5
+      e = np.exp(s - s.max())
+      e /= e.sum()
+      want[r, j], weight[r, j], reach[r, j] = e @ vv, e @ np.abs(vv), (np.abs(kk) @ np.abs(qv[r, j, 2:])).max() * d ** -0.5
+  close_attention(got, want, weight, reach, d, length, qt, qt, "rows with some scores of minus infinity")
+
+
+@pytest.mark.parametrize("qt,ct", [("float32", "float16"), ("float16", "float16"), ("bfloat16", "bfloat16"), ("float32", "bfloat16")])
+@pytest.mark.parametrize("new,length", [(2, 300), (150, 400), (150, 3000)])
+def test_queries_that_are_not_finite_in_wide_heads(qt, ct, new, length):
+  """Heads of 128, keys whole and in parts: a row of queries that is NaN or infinite gives a row of NaN, the others keep their bits."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(new)
+  h, hk, d, ps = 2, 1, 128, 16
+  t, n_pages = table(rng, [length], ps)
+  (k, _), (v, _) = (put(rng.standard_normal((n_pages, hk, ps, d)), ct) for _ in "kv")
+  cache = paged.PagedCache(n_pages, ps, hk, d, ct, k=k, v=v)
+  batch = paged.PagedBatch(i32([0, new]), i32([length]), i32(t), n_rows=new, max_new=new, max_len=length)
+  x, outs = rng.standard_normal((new, h, d)), []
+  for bad in (None, np.nan, np.inf):
+    if bad is not None: x[new // 2, 0, 3] = bad
+    out = put(np.zeros((new, h, d)), qt)[0]
+    paged.attention(cache, batch, put(x, qt)[0], out, h, qt)
+    outs.append(get(out, (new, h, d), qt))
+  for got in outs[1:]:
+    assert np.isnan(got[new // 2, 0]).all()
+    got[new // 2, 0] = outs[0][new // 2, 0]
+    assert (got == outs[0]).all()

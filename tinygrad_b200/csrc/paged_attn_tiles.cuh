@@ -4,14 +4,14 @@
 // (2048 cycles of the special-function units) and some 600 instructions of each of the eight warps that see them.  So a CTA has two tiles of 128 rows whose products and softmaxes take turns: while one's
 // scores are turned into probabilities, the other's products run.  Warps 0-3 and 4-7 are the tiles' softmax, a thread a row (scores are read from tensor memory as it holds them, no exchange between
 // threads; two threads a row, half of its scores each, were slower); one thread issues the products, S = Q K^T from shared memory and O += P V with P from tensor memory; one warp brings keys, one values (TMA
-// boxes of a page's rows, 128-byte swizzle), one looks after the values that a product must not see.  With heads of 128 a quarter of the powers is a polynomial on the multiply-adders (none, a quarter, a third,
-// half of them: 372, 367, 364, 405 us below; with heads of 64, whose time is issued instructions, 302, 312, 318, 342).  A tile's product begins with half of its probabilities.
+// boxes of a page's rows, 128-byte swizzle), one looks after the values that a product must not see.  All powers are the special-function
+// units': a quarter of them as a polynomial on the multiply-adders, whose results below 2^-126 have to be made 0, took 443 against 429 us below (heads of 64 312 against 302).  A tile's product begins with half of its probabilities.
 //
 // Tensor memory: S0 S1 O0 O1, 128 columns each, a tile's probabilities in the place of its scores.  Heads of 64 leave room for probabilities of their own (T_APART): the next scores
 // are then computed as soon as these have been read, not behind their product (4096 rows of 32 heads of 64, 8192 positions: 302 us, 315 in place).
 //
-// 4096 rows of 32 heads of 128 at 8192 positions: 365 to 400 us, as the power limit has the clock (1.0 to 1.1 PFLOP/s).  CTAs that stay and share the work evenly took 442 us there,
-// softmaxes that are kept apart by barriers 406 against 391, a running maximum looked for behind the first powers 399 against 388.
+// 4096 rows of 32 heads of 128 at 8192 positions: 365 to 430 us, as the power limit has the clock (0.96 to 1.1 PFLOP/s).  CTAs that stay and share the work evenly took 442 against
+// 388 us there, softmaxes that are kept apart by barriers 406 against 391, a running maximum looked for behind the first powers 399 against 388.
 //
 // The running maximum moves only when it has grown by 2^8: until then probabilities are relative to an older one, which the quotient does not notice, and the weighted sums
 // in tensor memory stay as they are.
@@ -90,7 +90,6 @@ __device__ __forceinline__ uint4 ld_s4(uint32_t a) {
   return v;
 }
 
-template <bool V> struct Switch { static constexpr bool value = V; };
 template <int V> struct Count { static constexpr int value = V; };
 // two fp32 values at a time
 __device__ __forceinline__ uint64_t pair_of(float a, float b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
@@ -98,27 +97,6 @@ __device__ __forceinline__ float2 floats_of(uint64_t r) { float2 f; asm("mov.b64
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 __device__ __forceinline__ float max3(float a, float b, float c) { float r; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c)); return r; }      // NaN if one is
-// 2^x of two values without the special-function units: x = n + f, n the nearest integer, 2^f by a polynomial fitted to it on [-1/2, 1/2] (least largest relative error: degree 3 2^-13.7, for
-// probabilities that bf16 rounds by 2^-9; degree 4 2^-18.5, fp16 2^-12), n added to the exponent.  Below 2^-126: 2^-126.
-template <bool BF>
-__device__ __forceinline__ uint64_t pow2_poly(uint64_t x) {
-  const float2 c = floats_of(x);
-  x = pair_of(fmaxf(c.x, -126.f), fmaxf(c.y, -126.f));
-  const uint64_t t = add2(x, pair_of(12582912.f, 12582912.f)), n = add2(t, pair_of(-12582912.f, -12582912.f)), f = fma2(n, pair_of(-1.f, -1.f), x);      // 1.5 x 2^23: t ends in n
-  uint64_t y;
-  if constexpr (BF) {
-    y = fma2(pair_of(0.055171665f, 0.055171665f), f, pair_of(0.24261113f, 0.24261113f));
-    y = fma2(y, f, pair_of(0.69326097f, 0.69326097f));
-    y = fma2(y, f, pair_of(0.99992806f, 0.99992806f));
-  } else {
-    y = fma2(pair_of(0.009570101f, 0.009570101f), f, pair_of(0.05591786f, 0.05591786f));
-    y = fma2(y, f, pair_of(0.24024744f, 0.24024744f));
-    y = fma2(y, f, pair_of(0.6931218f, 0.6931218f));
-    y = fma2(y, f, pair_of(0.9999993f, 0.9999993f));
-  }
-  const float2 tn = floats_of(t), yf = floats_of(y);
-  return pair_of(__uint_as_float(__float_as_uint(yf.x) + (__float_as_uint(tn.x) << 23)), __uint_as_float(__float_as_uint(yf.y) + (__float_as_uint(tn.y) << 23)));
-}
 
 struct RowOf { int64_t row, head; int last; bool live; };      // of a thread: its row of the arrays, its head, the position it sees up to
 
@@ -144,7 +122,7 @@ __device__ __forceinline__ void add_not_finite(const AttnParams& p, int seq, int
 template <int D, int N, bool BF>
 __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnParams p, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, int box_rows) {
   constexpr int SUBS = D / 64, TILE = T_TILE<D>, SUB = T_KEYS * 128, KS = T_KS<D, N>, VS = T_VS<D, N>, KK = D / 16;
-  constexpr bool APART = T_APART<D, N>, POLY = D == 128;
+  constexpr bool APART = T_APART<D, N>;
   constexpr int O_AT = 256, O_STEP = APART ? 64 : 128, P_AT = APART ? 384 : 0, P_STEP = APART ? 64 : 128, P_CHUNK = APART ? 16 : 32;      // columns of tensor memory
   extern __shared__ unsigned char raw[];
   __shared__ SharedA sh;
@@ -336,29 +314,24 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
         const float sub = m == -INFINITY ? 0.f : T_BASE - m;
         const uint64_t qs2 = pair_of(qs, qs), sub2 = pair_of(sub, sub);
         uint64_t sums[2] = {0, 0};
-        auto powers = [&](auto some) {
 #pragma unroll
-          for (int c = 0; c < 4; c++) {
-            uint32_t pk[16];
+        for (int c = 0; c < 4; c++) {
+          uint32_t pk[16];
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-              uint64_t x = fma2(pair_of(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), qs2, sub2);
-              if (POLY && some.value && i % 4 == 3) x = pow2_poly<BF>(x);
-              else { const float2 y = floats_of(x); x = pair_of(pow2(y.x), pow2(y.y)); }
-              sums[i & 1] = add2(sums[i & 1], x);
-              const float2 y = floats_of(x);
-              pk[i] = pack2(y.x, y.y, BF ? B200Q_BF16 : B200Q_F16);
-            }
-            st16(tp + c * P_CHUNK, pk);
-            if (c & 1) {      // half of the tile's probabilities: the product begins with them
-              wait_st();
-              fence_before();
-              __syncwarp();
-              if (lane == 0) a_bar_arrive(&sh.p_full[t][c / 2]);
-            }
+          for (int i = 0; i < 16; i++) {
+            const float2 x = floats_of(fma2(pair_of(s[c * 32 + 2 * i], s[c * 32 + 2 * i + 1]), qs2, sub2));
+            const float a = pow2(x.x), b = pow2(x.y);      // (of minus infinity: 0, so that a row without a finite score ends with a sum of 0)
+            sums[i & 1] = add2(sums[i & 1], pair_of(a, b));
+            pk[i] = pack2(a, b, BF ? B200Q_BF16 : B200Q_F16);
           }
-        };
-        if (masked) powers(Switch<false>{}); else powers(Switch<true>{});
+          st16(tp + c * P_CHUNK, pk);
+          if (c & 1) {      // half of the tile's probabilities: the product begins with them
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) a_bar_arrive(&sh.p_full[t][c / 2]);
+          }
+        }
         const float2 y0 = floats_of(sums[0]), y1 = floats_of(sums[1]);
         l += (y0.x + y0.y) + (y1.x + y1.y);
       } else {
