@@ -148,3 +148,60 @@ def test_views_of_rows_that_lie_apart():
   paged._short(big[:, 36:], (2 * 100 + 64) * 4, "x")
   with pytest.raises(ValueError, match="x has"): paged._short(big[:, 37:], (2 * 100 + 64) * 4, "x")
   with pytest.raises(ValueError, match="x has"): paged._short(big[1:, :64], (2 * 100 + 64) * 4, "x")
+
+
+def test_tables_of_angles_that_are_refused(lib):
+  """The rotation's table is fp32, two-dimensional and dense: anything else would be read past its end, or as other angles."""
+  import torch
+  c, b = paged.PagedCache(4, 16, 2, 64, k=P, v=P), paged.PagedBatch(*(Fake(s, np.int32) for s in ((3,), (2,), (2, 5))), 2, 1, 9)
+  for rope, err, match in ((Fake((9, 64), np.float16), TypeError, "rope"), (Fake((9, 64), np.float64), TypeError, "rope"), (Fake((9, 64), np.uint16), TypeError, "rope"), (Fake((9 * 64,), np.float32), ValueError, "rope"),
+                           (Fake((9, 2, 32), np.float32), ValueError, "rope"), (P, ValueError, "rope"), (torch.zeros(9, 128)[:, :64], ValueError, "rope"), (torch.zeros(64, 9).t(), ValueError, "rope"),
+                           (torch.zeros(9, 64, dtype=torch.bfloat16), TypeError, "rope"), (torch.zeros(9, 64), ValueError, "host")):
+    with pytest.raises(err, match=match): paged.append(c, b, P, P, 4, rope=rope)
+    with pytest.raises(err, match=match): paged.head_norm_rope(P, P, 5, 4, 2, 64, rope=rope, positions=P)
+  short = Fake((9, 64), np.float32)
+  short.nbytes -= 4
+  with pytest.raises(ValueError, match="rope has"): paged.append(c, b, P, P, 4, rope=short)
+
+
+def test_buffers_of_other_types_than_named(lib):
+  """An object that says what its elements are is held to the type argument; uint16 stands for bf16, bytes and raw addresses for anything."""
+  c, b = paged.PagedCache(4, 16, 2, 64, k=P, v=P), paged.PagedBatch(*(Fake(s, np.int32) for s in ((3,), (2,), (2, 5))), 2, 1, 9)
+  pool, rows = lambda t: Fake((4, 2, 16, 64), t), lambda t: Fake((2, 8, 64), t)
+  for named, given in (("float16", np.uint16), ("float16", np.float32), ("bfloat16", np.float16), ("float32", np.float64), ("float32", np.int32)):
+    with pytest.raises(TypeError, match="k has"): paged.PagedCache(4, 16, 2, 64, named, k=Fake((8, 2, 16, 64), given), v=P)
+    with pytest.raises(TypeError, match="v has"): paged.PagedCache(4, 16, 2, 64, named, k=P, v=Fake((8, 2, 16, 64), given))
+    wide = Fake((8, 8, 64), given)
+    with pytest.raises(TypeError, match="x has"): paged.append(c, b, wide, P, 4, named)
+    with pytest.raises(TypeError, match="q has"): paged.append(c, b, P, wide, 4, "float16", q_dtype=named)
+    with pytest.raises(TypeError, match="q has"): paged.attention(c, b, wide, P, 4, named)
+    with pytest.raises(TypeError, match="out has"): paged.attention(c, b, P, wide, 4, out_dtype=named)
+    with pytest.raises(TypeError, match="x has"): paged.head_norm_rope(wide, P, 2, 4, 2, 64, named)
+    with pytest.raises(TypeError, match="out has"): paged.head_norm_rope(P, wide, 2, 4, 2, 64, out_dtype=named)
+  for named, given in (("float16", np.float16), ("bfloat16", np.uint16), ("float32", np.float32)): paged.PagedCache(4, 16, 2, 64, named, k=pool(given), v=pool(given))
+  paged.PagedCache(2, 16, 2, 64, "bfloat16", k=Fake((2, 2, 16, 64, 2), np.uint8), v=P)
+
+
+def test_tensors_that_are_not_laid_out_as_the_call_says(lib):
+  """Foreign tensors on the host, and those whose values lie apart without a stride that says so."""
+  import torch
+  class OnDevice:      # (a host tensor that passes for one of the device)
+    is_cuda = True
+    def __init__(self, t): self.t = t
+    def __getattr__(self, name): return getattr(self.t, name)
+  c, b = paged.PagedCache(4, 16, 2, 64, k=P, v=P), paged.PagedBatch(*(Fake(s, np.int32) for s in ((3,), (2,), (2, 5))), 2, 1, 9)
+  apart = OnDevice(torch.zeros(2, 1024)[:, :512])
+  with pytest.raises(ValueError, match="stride"): paged.append(c, b, apart, P, 4)
+  with pytest.raises(ValueError, match="stride"): paged.append(c, b, P, apart, 4)
+  with pytest.raises(ValueError, match="stride"): paged.attention(c, b, apart, P, 4)
+  with pytest.raises(ValueError, match="stride"): paged.attention(c, b, P, apart, 4)
+  with pytest.raises(ValueError, match="stride"): paged.head_norm_rope(apart, P, 2, 4, 2, 64)
+  with pytest.raises(ValueError, match="stride"): paged.head_norm_rope(P, apart, 2, 4, 2, 64)
+  with pytest.raises(ValueError, match="contiguous"): paged.head_norm_rope(P, P, 2, 4, 2, 64, rope=Fake((9, 64), np.float32), positions=OnDevice(torch.zeros(4, dtype=torch.int32)[::2]))
+  with pytest.raises(ValueError, match="contiguous"): paged.append(c, b, P, P, 4, q_norm=OnDevice(torch.zeros(128, dtype=torch.float16)[::2]))
+  half = torch.zeros(4, 2, 16, 128, dtype=torch.float16)
+  with pytest.raises(ValueError, match="contiguous"): paged.PagedCache(4, 16, 2, 64, k=OnDevice(half[..., :64]), v=OnDevice(half[..., 64:]))
+  paged.PagedCache(4, 16, 2, 64, k=OnDevice(half[..., :64]), v=OnDevice(half[..., 64:]), strides=(2 * 16 * 128, 16 * 128, 128))
+  for call in (lambda x: paged.append(c, b, x, P, 4), lambda x: paged.append(c, b, P, x, 4), lambda x: paged.attention(c, b, P, x, 4), lambda x: paged.head_norm_rope(x, P, 2, 4, 2, 64),
+               lambda x: paged.PagedCache(1, 1, 1, 16, "float32", k=x, v=P), lambda x: paged.PagedBatch(Fake((3,), np.int32), torch.zeros(2, dtype=torch.int32), Fake((2, 5), np.int32), 2, 1, 9)):
+    with pytest.raises(ValueError, match="host"): call(torch.zeros(2, 512))
