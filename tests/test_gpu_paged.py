@@ -802,3 +802,26 @@ def test_queries_that_are_not_finite_in_wide_heads(qt, ct, new, length):
     assert np.isnan(got[new // 2, 0]).all()
     got[new // 2, 0] = outs[0][new // 2, 0]
     assert (got == outs[0]).all()
+
+
+def test_a_new_cache_on_a_stream_of_its_own():
+  """The zeros of a cache that has just been allocated are there before any call on it, whatever stream that is on and whatever the device still has to do on another: they do not come over what a call
+  has appended."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  from tinygrad_b200.runtime import DeviceBuffer, Stream, synchronize
+  hk, d, ps = 8, 128, 16
+  x, xv = put(np.arange(3 * hk * d).reshape(1, 3 * hk, d) % 61 + 1, "float16")
+  q, stream, busy = put(np.zeros((1, hk, d)), "float16")[0], Stream(), DeviceBuffer(4 << 30)
+  batch = paged.PagedBatch(i32([0, 1]), i32([ps]), i32([[3]]), n_rows=1, max_new=1, max_len=ps)
+  kept = []                   # (freeing one waits for the device)
+  for again in range(3):      # (the first time the kernel is loaded, which may wait as well)
+    synchronize()
+    for _ in range(20): busy.zero_()
+    cache = paged.PagedCache(4, ps, hk, d)
+    kept.append(cache)
+    paged.append(cache, batch, x, q, hk, "float16", stream=stream)
+    synchronize()
+    for pool, heads in ((cache.k, xv[0, hk:2 * hk]), (cache.v, xv[0, 2 * hk:])):
+      got = get(pool, (4, hk, ps, d), "float16")
+      assert (got[3, :, -1] == heads).all() and np.count_nonzero(got) == hk * d, again

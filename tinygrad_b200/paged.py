@@ -127,7 +127,9 @@ class PagedCache:
     page, head, row = self.strides = tuple(strides) if strides is not None else (n_kv_heads * page_size * head_dim, page_size * head_dim, head_dim)
     if min(self.strides) < head_dim: raise ValueError(f"strides {self.strides} are shorter than a head")
     last = (n_pages - 1) * page + (n_kv_heads - 1) * head + (page_size - 1) * row + head_dim
-    if k is None: k, v = (DeviceBuffer.empty((last,), _NP[self.dtype], zero=True) for _ in range(2))
+    if k is None:
+      k, v = (DeviceBuffer.empty((last,), _NP[self.dtype], zero=True) for _ in range(2))
+      synchronize()                      # whatever stream the first call is on: zeros that come late would go over what it has appended
     self.k, self.v = k, v
     at = [_rows(x, self.dtype, last * _SIZE[self.dtype], strides is not None, what) for x, what in ((k, "k"), (v, "v"))]
     self.desc = _lib.PagedCacheDesc(*at, self.dtype, n_pages, page_size, n_kv_heads, head_dim, page, head, row)
