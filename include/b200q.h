@@ -94,6 +94,7 @@ int b200q_event_elapsed_ms(void* start, void* stop, float* ms);
  * the counterpart of the reference's TinyJit -> CUDAGraph replay
  * (tinygrad/engine/jit.py:241-291, tinygrad/runtime/graph/cuda.py:10-70). */
 int b200q_graph_begin(void* stream);
+int b200q_stream_is_capturing(void* stream, int* capturing);      /* 1: a capture is going on there, whoever began it */
 int b200q_graph_end(void* stream, void** graph_exec);
 int b200q_graph_launch(void* graph_exec, void* stream);
 int b200q_graph_destroy(void* graph_exec);

@@ -825,3 +825,28 @@ def test_a_new_cache_on_a_stream_of_its_own():
     for pool, heads in ((cache.k, xv[0, hk:2 * hk]), (cache.v, xv[0, 2 * hk:])):
       got = get(pool, (4, hk, ps, d), "float16")
       assert (got[3, :, -1] == heads).all() and np.count_nonzero(got) == hk * d, again
+
+
+def test_a_capture_without_a_reserved_workspace_is_refused():
+  """The capture goes on without the call, and the batch is as it was: an eager call and a reserved, captured one give the same bits."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  from tinygrad_b200.runtime import Graph, Stream
+  rng = np.random.default_rng(33)
+  h, hk, d, ps, length = 4, 2, 64, 16, 3000
+  t, n_pages = table(rng, [length], ps)
+  (k, _), (v, _), (q, _) = (put(rng.standard_normal(s), "float16") for s in ((n_pages, hk, ps, d), (n_pages, hk, ps, d), (1, h, d)))
+  cache, stream = paged.PagedCache(n_pages, ps, hk, d, k=k, v=v), Stream()
+  new = lambda: (paged.PagedBatch(i32([0, 1]), i32([length]), i32(t), n_rows=1, max_new=1, max_len=length), put(np.zeros((1, h, d)), "float16")[0])
+  (batch, out), (other, out2) = new(), new()
+  graph = Graph(stream)
+  with graph:
+    with pytest.raises(RuntimeError, match="reserve"): paged.attention(cache, batch, q, out, h, "float16", stream=stream)
+  paged.attention(cache, batch, q, out, h, "float16", stream=stream)
+  other.reserve(cache, h)
+  graph = Graph(stream)
+  with graph: paged.attention(cache, other, q, out2, h, "float16", stream=stream)
+  for _ in range(2): graph.launch()
+  stream.synchronize()
+  assert (get(out, (1, h, d), "float16") == get(out2, (1, h, d), "float16")).all() and get(out, (1, h, d), "float16").any()
+  assert status() == 0

@@ -205,3 +205,58 @@ def test_tensors_that_are_not_laid_out_as_the_call_says(lib):
   for call in (lambda x: paged.append(c, b, x, P, 4), lambda x: paged.append(c, b, P, x, 4), lambda x: paged.attention(c, b, P, x, 4), lambda x: paged.head_norm_rope(x, P, 2, 4, 2, 64),
                lambda x: paged.PagedCache(1, 1, 1, 16, "float32", k=x, v=P), lambda x: paged.PagedBatch(Fake((3,), np.int32), torch.zeros(2, dtype=torch.int32), Fake((2, 5), np.int32), 2, 1, 9)):
     with pytest.raises(ValueError, match="host"): call(torch.zeros(2, 512))
+
+
+class Workspaces:
+  """The library without a device: memory is numbers, and what is done to it is written down."""
+  def __init__(self, lib): self.lib, self.log, self.fail, self.capturing = lib, [], False, 0
+  def __getattr__(self, name): return getattr(self.lib, name)
+  def b200q_pool_alloc(self, p, nbytes, stream):
+    p._obj.value = 0x10000 * (1 + len(self.log))
+    self.log.append(("alloc", p._obj.value, stream))
+    return 0
+  def b200q_pool_free(self, ptr): return 0
+  def b200q_memset(self, ptr, value, nbytes, stream):
+    self.log.append(("memset", ptr, stream or 0))
+    return -5 if self.fail else 0
+  def b200q_device_synchronize(self):
+    self.log.append(("wait",))
+    return 0
+  def b200q_stream_is_capturing(self, stream, flag):
+    flag._obj.value = self.capturing
+    return 0
+
+
+@pytest.fixture
+def workspaces(lib, monkeypatch):
+  w = Workspaces(lib)
+  monkeypatch.setattr(_lib, "load", lambda: w)
+  monkeypatch.setattr(paged, "_entry", {**{n: getattr(lib, n) for n in ("b200q_paged_attention_workspace_bytes",)}, "b200q_paged_attention": lambda *a: 0, "b200q_paged_append": lambda *a: 0})
+  return w
+
+
+def a_batch(): return paged.PagedBatch(*(Fake(s, np.int32) for s in ((3,), (2,), (2, 500))), 2, 1, 8000)
+
+
+def test_a_workspace_that_could_not_be_zeroed_is_not_kept(workspaces):
+  """Counters that are not zero would make later calls leave rows out: a reservation that failed is made anew."""
+  c, b = paged.PagedCache(4, 16, 2, 64, k=P, v=P), a_batch()
+  workspaces.fail = True
+  with pytest.raises(_lib.B200QError): paged.attention(c, b, P, P, 4)
+  workspaces.fail = False
+  paged.attention(c, b, P, P, 4)
+  kinds = [e[0] for e in workspaces.log if e[0] != "wait"]
+  assert kinds == ["alloc", "memset"] * 2 and workspaces.log[-1 if workspaces.log[-1][0] == "memset" else -2][1] == b._ws.ptr
+  paged.attention(c, b, P, P, 4)
+  assert [e[0] for e in workspaces.log if e[0] != "wait"] == kinds
+
+
+def test_a_captured_call_is_reserved_beforehand(workspaces):
+  c, b = paged.PagedCache(4, 16, 2, 64, k=P, v=P), a_batch()
+  workspaces.capturing = 1
+  with pytest.raises(RuntimeError, match="reserve"): paged.attention(c, b, P, P, 4, stream=7)
+  assert not workspaces.log
+  workspaces.capturing = 0
+  b.reserve(c, 4)
+  workspaces.capturing = 1
+  paged.attention(c, b, P, P, 4, stream=7)

@@ -136,6 +136,7 @@ SIGNATURES = {
   "b200q_event_synchronize": (c_int, [c_void_p]),
   "b200q_event_elapsed_ms": (c_int, [c_void_p, c_void_p, POINTER(c_float)]),
   "b200q_graph_begin": (c_int, [c_void_p]),
+  "b200q_stream_is_capturing": (c_int, [c_void_p, POINTER(c_int)]),
   "b200q_graph_end": (c_int, [c_void_p, POINTER(c_void_p)]),
   "b200q_graph_launch": (c_int, [c_void_p, c_void_p]),
   "b200q_graph_destroy": (c_int, [c_void_p]),

@@ -111,6 +111,15 @@ extern "C" int b200q_graph_begin(void* stream) {
   B200Q_CHECK_CUDA(cudaStreamBeginCapture((cudaStream_t)stream, cudaStreamCaptureModeThreadLocal));
   return B200Q_OK;
 }
+extern "C" int b200q_stream_is_capturing(void* stream, int* capturing) {
+  if (!capturing) return B200Q_ERR_BAD_ARG;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  const cudaError_t e = cudaStreamIsCapturing((cudaStream_t)stream, &status);
+  if (e == cudaErrorStreamCaptureImplicit) cudaGetLastError();      // the legacy stream beside a capture: not captured itself
+  else B200Q_CHECK_CUDA(e);
+  *capturing = status != cudaStreamCaptureStatusNone;
+  return B200Q_OK;
+}
 extern "C" int b200q_graph_end(void* stream, void** graph_exec) {
   if (!stream || !graph_exec) return B200Q_ERR_BAD_ARG;
   cudaGraph_t graph = nullptr;

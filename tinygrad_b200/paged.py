@@ -154,14 +154,21 @@ class PagedBatch:
     self._ws, self._ready, self._old = None, set(), []
 
   def reserve(self, cache: PagedCache, n_heads: int, q_dtype="float32") -> None:
-    """Allocates the workspace that `attention` needs for such a cache (done by its first call otherwise; a call under capture allocates nothing)."""
+    """Allocates the workspace that `attention` needs for such a cache and such rows, of whatever type.  A call's first time does so otherwise; one that is captured cannot."""
     _dtype(q_dtype)
+    self._reserve(cache, n_heads)
+
+  def _reserve(self, cache: PagedCache, n_heads: int, stream=None) -> None:
     need = _fn("b200q_paged_attention_workspace_bytes")(cache.ref, self.ref, n_heads)
     if need and (self._ws is None or self._ws.nbytes < need):
-      if self._ws is not None: self._old.append(self._ws)      # graphs may hold it
-      self._ws = DeviceBuffer.result((need,), np.uint8)          # (from the pool: a batch may live as briefly as a step)
-      check(_lib.load().b200q_memset(self._ws.ptr, 0, WORKSPACE_HEAD, None))
+      lib, capturing = _lib.load(), ctypes.c_int()
+      if stream is not None: check(lib.b200q_stream_is_capturing(stream_ptr(stream), ctypes.byref(capturing)))
+      if capturing.value: raise RuntimeError("a captured call allocates nothing: PagedBatch.reserve goes before the capture")
+      ws = DeviceBuffer.result((need,), np.uint8)                # (from the pool: a batch may live as briefly as a step)
+      check(lib.b200q_memset(ws.ptr, 0, WORKSPACE_HEAD, None))
       synchronize()                                              # whatever stream the first call is on
+      if self._ws is not None: self._old.append(self._ws)      # graphs may hold it
+      self._ws = ws
     self._ready.add((cache._key, n_heads))
 
 
@@ -188,7 +195,7 @@ def attention(cache: PagedCache, batch: PagedBatch, q, out, n_heads: int, q_dtyp
   n, row = batch.n_rows, n_heads * cache.head_dim
   qp = _rows(q, qt, ((n - 1) * (q_stride or row) + row) * _SIZE[qt] if n else 0, q_stride, "q")
   op = _rows(out, ot, ((n - 1) * (out_stride or row) + row) * _SIZE[ot] if n else 0, out_stride, "out")
-  if (cache._key, n_heads) not in batch._ready: batch.reserve(cache, n_heads)
+  if (cache._key, n_heads) not in batch._ready: batch._reserve(cache, n_heads, stream)
   ws = batch._ws
   a = _attn_args(qp, op, qt, ot, q_stride, out_stride, n_heads, scale, *((0, 0) if ws is None else (ws.ptr, ws.nbytes)))
   rc = _fn("b200q_paged_attention")(cache.ref, batch.ref, a, flags, 0 if stream is None else stream_ptr(stream))
