@@ -850,3 +850,41 @@ def test_a_capture_without_a_reserved_workspace_is_refused():
   stream.synchronize()
   assert (get(out, (1, h, d), "float16") == get(out2, (1, h, d), "float16")).all() and get(out, (1, h, d), "float16").any()
   assert status() == 0
+
+
+def test_a_graph_whose_batch_nobody_else_holds():
+  """The graph holds cache and batch: what is allocated afterwards does not land in memory that replays write."""
+  need_gpu()
+  import gc
+  from tinygrad_b200 import paged
+  from tinygrad_b200.runtime import DeviceBuffer, Graph, Stream, synchronize
+  rng = np.random.default_rng(34)
+  h, hk, d, ps, length = 4, 2, 64, 16, 5000
+  t, n_pages = table(rng, [length], ps)
+  (k, _), (v, _), (q, _) = (put(rng.standard_normal(s), "float16") for s in ((n_pages, hk, ps, d), (n_pages, hk, ps, d), (1, h, d)))
+  out, stream = put(np.zeros((1, h, d)), "float16")[0], Stream()
+  def captured():
+    cache, batch = paged.PagedCache(n_pages, ps, hk, d, k=k, v=v), paged.PagedBatch(i32([0, 1]), i32([length]), i32(t), n_rows=1, max_new=1, max_len=length)
+    batch.reserve(cache, h)
+    graph = Graph(stream)
+    with graph: paged.attention(cache, batch, q, out, h, "float16", stream=stream)
+    return graph, batch._ws.nbytes
+  graph, size = captured()
+  gc.collect()
+  graph.launch()
+  stream.synchronize()
+  want = get(out, (1, h, d), "float16")
+  assert want.any()
+  others = [DeviceBuffer.result((size,), np.uint8) for _ in range(100)]      # (more than the pool waits for before it hands blocks out again)
+  for o in others: sevens(o)
+  synchronize()
+  graph.launch()
+  stream.synchronize()
+  assert (get(out, (1, h, d), "float16") == want).all()
+  for o in others: assert (o.numpy((size,), np.uint8) == 7).all()
+  assert status() == 0
+
+
+def sevens(buf):
+  from tinygrad_b200 import _lib
+  _lib.check(_lib.load().b200q_memset(buf.ptr, 7, buf.nbytes, None))

@@ -260,3 +260,38 @@ def test_a_captured_call_is_reserved_beforehand(workspaces):
   b.reserve(c, 4)
   workspaces.capturing = 1
   paged.attention(c, b, P, P, 4, stream=7)
+
+
+def test_a_graph_keeps_what_its_paged_calls_use(workspaces, monkeypatch):
+  """The caches and batches (tables, workspaces) of captured calls live as long as the graph; calls on other streams, or behind the capture, are nothing to it."""
+  import gc, weakref
+  from tinygrad_b200.runtime import Graph, Stream
+  monkeypatch.setattr(Workspaces, "b200q_graph_begin", lambda self, s: 0, raising=False)
+  monkeypatch.setattr(Workspaces, "b200q_graph_end", lambda self, s, p: 0, raising=False)
+  made = [(paged.PagedCache(4, 16, 2, 64, k=P, v=P), a_batch()) for _ in range(4)]
+  for c, b in made: b.reserve(c, 4)
+  stream = Stream(7)
+  graph = Graph(stream)
+  with graph:
+    paged.attention(*made[0], P, P, 4, stream=stream)
+    paged.append(*made[1], P, 2 * P, 4, stream=7)
+    paged.attention(*made[2], P, P, 4, stream=Stream(9))
+  paged.attention(*made[3], P, P, 4, stream=stream)
+  seen = [(weakref.ref(c), weakref.ref(b)) for c, b in made]
+  del made, c, b
+  gc.collect()
+  assert [(c() is not None, b() is not None) for c, b in seen] == [(True, True)] * 2 + [(False, False)] * 2
+  del graph
+  gc.collect()
+  assert not any(b() for _, b in seen)
+
+
+def test_a_capture_that_fails_keeps_nothing_open(workspaces, monkeypatch):
+  from tinygrad_b200.runtime import Graph, Stream
+  monkeypatch.setattr(Workspaces, "b200q_graph_begin", lambda self, s: 0, raising=False)
+  monkeypatch.setattr(Workspaces, "b200q_graph_end", lambda self, s, p: -5, raising=False)
+  with pytest.raises(_lib.B200QError):
+    with Graph(Stream(7)): pass
+  with pytest.raises(KeyError):
+    with Graph(Stream(7)): raise KeyError
+  assert not Graph.open

@@ -7,12 +7,13 @@ ragged batch --, `head_norm_rope` the norms and the rotation alone, for caches t
 
 Buffers are DeviceBuffers or foreign tensors of the current device, held to the type that the call names where they say theirs (bf16 values are uint16 in a DeviceBuffer), or raw addresses
 (`runtime.ptr_of`; the tables of a batch and `rope` are asked for their shapes and cannot be).  Calls launch on `stream` and return at
-once; a batch's workspace serves one call at a time: streams and graphs that may run together need a PagedBatch each."""
+once; a batch's workspace serves one call at a time: streams and graphs that may run together need a PagedBatch each.  A captured call's cache and batch live as long as the graph:
+`runtime.Graph` keeps them; under another kind of capture the caller does.  Rows, outputs and angles are the caller's to keep, as with any call."""
 import ctypes, struct
 import numpy as np
 from . import _lib
 from ._lib import check, F32, F16, BF16
-from .runtime import DeviceBuffer, ptr_of, stream_ptr, synchronize
+from .runtime import DeviceBuffer, Graph, ptr_of, stream_ptr, synchronize
 
 DTYPES = {"float32": F32, "float16": F16, "bfloat16": BF16}
 _NP = {F32: np.float32, F16: np.float16, BF16: np.uint16}
@@ -101,6 +102,12 @@ def _angles(rope) -> tuple:
   return _rows(rope, F32, 4 * n * dim, 0, "rope"), dim, n
 
 
+def _kept(stream, *objects) -> None:
+  """A graph that is being captured on the stream keeps the objects."""
+  graph = Graph.open.get(stream_ptr(stream))
+  if graph is not None: graph.kept += objects
+
+
 def _fits(*values) -> None:
   if max(values) >= 1 << 31: raise ValueError(f"{max(values)} does not fit into 31 bits")
 
@@ -183,6 +190,7 @@ def append(cache: PagedCache, batch: PagedBatch, x, q, n_heads: int, x_dtype="fl
   xp = _rows(x, xt, ((n - 1) * (x_stride or row) + row) * _SIZE[xt] if n else 0, x_stride, "x")
   qp = _rows(q, qt, ((n - 1) * (q_stride or q_row) + q_row) * _SIZE[qt] if n else 0, q_stride, "q")
   a = _append_args(xp, qp, xt, qt, x_stride, q_stride, n_heads, norm_eps, 0 if q_norm is None else _norm(q_norm, d), 0 if k_norm is None else _norm(k_norm, d), *_angles(rope))
+  if Graph.open: _kept(stream, cache, batch)
   rc = _fn("b200q_paged_append")(cache.ref, batch.ref, a, flags, 0 if stream is None else stream_ptr(stream))
   if rc: check(rc)
 
@@ -198,6 +206,7 @@ def attention(cache: PagedCache, batch: PagedBatch, q, out, n_heads: int, q_dtyp
   if (cache._key, n_heads) not in batch._ready: batch._reserve(cache, n_heads, stream)
   ws = batch._ws
   a = _attn_args(qp, op, qt, ot, q_stride, out_stride, n_heads, scale, *((0, 0) if ws is None else (ws.ptr, ws.nbytes)))
+  if Graph.open: _kept(stream, cache, batch)
   rc = _fn("b200q_paged_attention")(cache.ref, batch.ref, a, flags, 0 if stream is None else stream_ptr(stream))
   if rc: check(rc)
 

@@ -153,13 +153,17 @@ class Event:
 
 class Graph:
   """Stream capture of a fixed launch sequence, replayed with one call: the role
-  TinyJit + CUDAGraph play for the reference's decode loop (tinygrad/engine/jit.py:241-291)."""
+  TinyJit + CUDAGraph play for the reference's decode loop (tinygrad/engine/jit.py:241-291).  `kept`: objects whose memory captured calls use and their callers may not hold."""
+  open: dict = {}      # stream -> the graph that is being captured on it
+
   def __init__(self, stream: Stream):
-    self.stream, self.exec = stream, 0
+    self.stream, self.exec, self.kept = stream, 0, []
   def __enter__(self):
     check(_lib.load().b200q_graph_begin(self.stream.ptr))
+    Graph.open[self.stream.ptr] = self
     return self
   def __exit__(self, et, ev, tb):
+    Graph.open.pop(self.stream.ptr, None)
     p = ctypes.c_void_p()
     rc = _lib.load().b200q_graph_end(self.stream.ptr, ctypes.byref(p))
     if et is None: check(rc)
