@@ -295,3 +295,16 @@ def test_a_capture_that_fails_keeps_nothing_open(workspaces, monkeypatch):
   with pytest.raises(KeyError):
     with Graph(Stream(7)): raise KeyError
   assert not Graph.open
+
+
+def test_a_first_call_zeroes_its_workspace_on_its_own_stream(workspaces):
+  """No wait for the device: a batch may live as briefly as a step.  One that is reserved beforehand is ready for any stream."""
+  c, b = paged.PagedCache(4, 16, 2, 64, k=P, v=P), a_batch()
+  paged.attention(c, b, P, P, 4, stream=7)
+  assert workspaces.log == [("alloc", b._ws.ptr, 7), ("memset", b._ws.ptr, 7)]
+  b = a_batch()
+  del workspaces.log[:]
+  b.reserve(c, 4)
+  assert workspaces.log == [("alloc", b._ws.ptr, 0), ("memset", b._ws.ptr, 0), ("wait",)]
+  b.reserve(c, 4)
+  assert len(workspaces.log) == 3

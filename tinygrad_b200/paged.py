@@ -163,20 +163,22 @@ class PagedBatch:
   def reserve(self, cache: PagedCache, n_heads: int, q_dtype="float32") -> None:
     """Allocates the workspace that `attention` needs for such a cache and such rows, of whatever type.  A call's first time does so otherwise; one that is captured cannot."""
     _dtype(q_dtype)
-    self._reserve(cache, n_heads)
+    if self._reserve(cache, n_heads, None): synchronize()        # whatever stream the first call is on
 
-  def _reserve(self, cache: PagedCache, n_heads: int, stream=None) -> None:
+  def _reserve(self, cache: PagedCache, n_heads: int, stream) -> bool:
+    """True: a new workspace, whose zeros are on their way on `stream`."""
     need = _fn("b200q_paged_attention_workspace_bytes")(cache.ref, self.ref, n_heads)
-    if need and (self._ws is None or self._ws.nbytes < need):
+    fresh = need > 0 and (self._ws is None or self._ws.nbytes < need)
+    if fresh:
       lib, capturing = _lib.load(), ctypes.c_int()
       if stream is not None: check(lib.b200q_stream_is_capturing(stream_ptr(stream), ctypes.byref(capturing)))
       if capturing.value: raise RuntimeError("a captured call allocates nothing: PagedBatch.reserve goes before the capture")
-      ws = DeviceBuffer.result((need,), np.uint8)                # (from the pool: a batch may live as briefly as a step)
-      check(lib.b200q_memset(ws.ptr, 0, WORKSPACE_HEAD, None))
-      synchronize()                                              # whatever stream the first call is on
+      ws = DeviceBuffer.result((need,), np.uint8, stream)      # (from the pool: a batch may live as briefly as a step)
+      check(lib.b200q_memset(ws.ptr, 0, WORKSPACE_HEAD, stream_ptr(stream)))
       if self._ws is not None: self._old.append(self._ws)      # graphs may hold it
       self._ws = ws
     self._ready.add((cache._key, n_heads))
+    return fresh
 
 
 def append(cache: PagedCache, batch: PagedBatch, x, q, n_heads: int, x_dtype="float32", q_dtype=None, rope=None, q_norm=None, k_norm=None, norm_eps: float = 0.0, x_stride: int = 0,
