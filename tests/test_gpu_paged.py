@@ -888,3 +888,21 @@ def test_a_graph_whose_batch_nobody_else_holds():
 def sevens(buf):
   from tinygrad_b200 import _lib
   _lib.check(_lib.load().b200q_memset(buf.ptr, 7, buf.nbytes, None))
+
+
+@pytest.mark.parametrize("qt,ct", [("float16", "float16"), ("float32", "float32")])
+def test_a_length_bound_next_to_31_bits(qt, ct):
+  """max_len as good as none, keys in one part: the bits of a call whose bound is the length."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(35)
+  h, hk, d, ps, new, length = 32, 8, 64, 16, 700, 1000
+  t, n_pages = table(rng, [length], ps)
+  (k, _), (v, _), (q, _) = (put(rng.standard_normal(s), c) for s, c in (((n_pages, hk, ps, d), ct), ((n_pages, hk, ps, d), ct), ((new, h, d), qt)))
+  cache, outs = paged.PagedCache(n_pages, ps, hk, d, ct, k=k, v=v), []
+  for most in (length, (1 << 31) - 129, (1 << 31) - 128, (1 << 31) - 1):
+    out = put(np.zeros((new, h, d)), qt)[0]
+    paged.attention(cache, paged.PagedBatch(i32([0, new]), i32([length]), i32(t), n_rows=new, max_new=new, max_len=most), q, out, h, qt)
+    outs.append(get(out, (new, h, d), qt))
+  for o in outs[1:]: assert (o == outs[0]).all()
+  assert outs[0].any() and status() == 0

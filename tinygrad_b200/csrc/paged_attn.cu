@@ -96,7 +96,8 @@ __device__ __forceinline__ int64_t key_at(const AttnParams& p, int seq, int key)
   return page * p.page_stride + (int64_t)(key - index * p.t.page_size) * p.row_stride;
 }
 
-// ---- parts of the keys ----
+// ---- parts of the keys ----  (a sum of a length and a part's may pass 31 bits)
+__device__ __forceinline__ int parts_of_keys(const AttnParams& p, int keys) { return keys > 0 ? (keys - 1) / p.split_len + 1 : 1; }
 template <int R, int D> constexpr int PART = R * (D + 2);           // m [R], sum [R], weighted sum [R][D]
 
 // The tile's last part to be done adds all of them; by the whole CTA (THREADS).  m in log2.  One thread's count releases what all have stored before the barrier.  Then the first AHEAD parts of every
@@ -176,7 +177,7 @@ __global__ void __launch_bounds__(S_THREADS) attn_simple_kernel(const AttnParams
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, kvh = blockIdx.y, split = blockIdx.z;
   const TilePlace w = place_of_tile<R>(p, blockIdx.x);
   if (w.n == 0) return;
-  const int n_parts = max(1, (w.keys + p.split_len - 1) / p.split_len), k_begin = split * p.split_len, k_end = min(w.keys, k_begin + p.split_len);
+  const int n_parts = parts_of_keys(p, w.keys), k_begin = split * p.split_len, k_end = k_begin + min(w.keys - k_begin, p.split_len);
   if (split >= n_parts) return;
   const int64_t pairs = (int64_t)w.n * p.group;
   for (int i = tid; i < R * D; i += S_THREADS) {
@@ -285,6 +286,14 @@ __global__ void __launch_bounds__(S_THREADS) attn_simple_kernel(const AttnParams
 namespace {
 
 // ---- how the work is dealt ----
+// Positions that can be attended: the end of the last one's tile is an int.  Lengths past a bound of the host's are not attended and reported.
+constexpr int MAX_KEYS = INT32_MAX - (T_KEYS - 1);
+static_assert(T_KEYS % ROUND == 0, "rounds end inside");
+b200q_paged_batch bounded(const b200q_paged_batch* b) {
+  b200q_paged_batch c = *b;
+  c.max_len = std::min(c.max_len, MAX_KEYS);
+  return c;
+}
 constexpr int MAX_PARTS = 296;      // of a tile's keys: their shares of 16 rows take 19 KB of shared memory (of 256 rows, 64 parts at most, 64 KB)
 struct Plan { int64_t tiles; int tiles_per_seq, n_split, split_len, above, up_to, ctas; int64_t rounds; size_t bytes; };      // tiles x KV heads past 2^31 and rounds of -1: too large; bytes: of the parts in the workspace
 
@@ -396,7 +405,8 @@ int b200q_paged_attn_status_take(int* status) {
 extern "C" size_t b200q_paged_attention_workspace_bytes(const b200q_paged_cache* cache, const b200q_paged_batch* batch, int n_heads) {
   if (check_cache(cache) != B200Q_OK || check_batch(batch) != B200Q_OK || n_heads <= 0 || n_heads % cache->n_kv_heads || batch->n_seqs == 0 || batch->n_rows == 0) return 0;
   const int group = n_heads / cache->n_kv_heads;
-  const size_t a = deal_of(cache, batch, group, false).bytes, b = pages_for_tiles(cache) ? deal_of(cache, batch, group, true).bytes : 0;
+  const b200q_paged_batch within = bounded(batch);
+  const size_t a = deal_of(cache, &within, group, false).bytes, b = pages_for_tiles(cache) ? deal_of(cache, &within, group, true).bytes : 0;
   return a > b ? a : b;
 }
 
@@ -411,6 +421,8 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
   if (batch->n_seqs == 0 || batch->n_rows == 0) return B200Q_OK;
   if (!a->q || !a->out) return B200Q_ERR_BAD_ARG;
   if ((uintptr_t)a->q % type_size(a->q_dtype) || (uintptr_t)a->out % type_size(a->out_dtype) || (uintptr_t)a->workspace & 255) return B200Q_ERR_MISALIGNED;
+  const b200q_paged_batch within = bounded(batch);
+  batch = &within;
   // one part of 16 bits where queries, keys and outputs have 16; two (bf16 keys: three, which the rows kernel has) where something is wider
   const int parts = a->q_dtype == cache->dtype && a->out_dtype != B200Q_F32 ? 1 : 2;
   alignas(64) CUtensorMap boxes[4];      // of the rows kernel and the tiles kernel, k and v each

@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(T_THREADS, 1) attn_tiles_kernel(const AttnPara
   const int order = p.by_kv.div(blockIdx.x), kvh = blockIdx.x - order * p.n_kv, split = blockIdx.y;
   const int tile_index = p.by_kv.div(gridDim.x) - 1 - order;      // long ones first
   const TilePlace w = place_of_tile<T_R>(p, tile_index);
-  const int n_parts = w.n == 0 ? 0 : max(1, (w.keys + p.split_len - 1) / p.split_len), k_begin = split * p.split_len, k_end = min(w.keys, k_begin + p.split_len);
+  const int n_parts = w.n == 0 ? 0 : parts_of_keys(p, w.keys), k_begin = split * p.split_len, k_end = k_begin + min(w.keys - k_begin, p.split_len);
   if (split >= n_parts) return;
   const int tiles = max(0, (k_end - k_begin + T_KEYS - 1) / T_KEYS);
   const int pairs = w.n * p.group;
@@ -636,7 +636,7 @@ __global__ void __launch_bounds__(J_THREADS) join_tiles_kernel(const AttnParams 
   pdl_launch_dependents();
   const int order = p.by_kv.div(blockIdx.x), kvh = blockIdx.x - order * p.n_kv, tile_index = p.by_kv.div(gridDim.x) - 1 - order, lane = threadIdx.x & 31;
   const TilePlace w = place_of_tile<T_R>(p, tile_index);
-  const int n_parts = (w.keys + p.split_len - 1) / p.split_len, end = min(T_R, w.n * p.group - w.r0);
+  const int n_parts = parts_of_keys(p, w.keys), end = min(T_R, w.n * p.group - w.r0);
   if (w.n == 0 || n_parts <= 1) return;
   const float* first = p.parts + (int64_t)(tile_index * p.n_kv + kvh) * p.n_split * PART<T_R, D>;
 #pragma unroll 1
