@@ -500,7 +500,8 @@ int b200q_tc_status_read_clear(int* status);
  *   max_new rows and max_len tokens of any sequence.
  * What the tables say is checked on the device; nothing outside the arrays is read or written, and the status word (b200q_status_read_clear) becomes 2 where they
  * are wrong: a page that does not exist takes no writes and reads as zeros; a position outside the table's row, below 0 or (append) outside the
- * rotation's table has no cache row; tokens past max_len are not attended; rows past max_new of a sequence get no attention; row offsets that go back leave it open which rows do.  Rows that belong to no sequence (n_rows >
+ * rotation's table has no cache row; tokens past max_len are not attended; rows past max_new of a sequence get no attention; rows that the arrays do
+ * not have are passed over; row offsets that go back leave it open which rows get one.  Rows that belong to no sequence (n_rows >
  * row_off[n_seqs]: a padded batch in a captured graph) are left as they were.
  *
  * b200q_paged_append: rows x = [q | k | v] (x_dtype; x_stride elements apart, 0: back to back) -> per head RMSNorm(q) * q_norm, RMSNorm(k) * k_norm (fp16 [head_dim], NULL: no norm;

@@ -906,3 +906,26 @@ def test_a_length_bound_next_to_31_bits(qt, ct):
     outs.append(get(out, (new, h, d), qt))
   for o in outs[1:]: assert (o == outs[0]).all()
   assert outs[0].any() and status() == 0
+
+
+@pytest.mark.parametrize("qt,ct,d", [("float16", "float16", 64), ("float32", "float32", 64), ("bfloat16", "bfloat16", 32)])
+@pytest.mark.parametrize("off,held", [([0, 9], 4), ([0, 200], 130), ([0, 3, 150], 100), ([-5, 30], 30), ([0, 2, 40], 2)], ids=["token rows", "chunk", "second sequence", "before the first row", "no rows"])
+def test_row_offsets_outside_the_arrays(qt, ct, d, off, held):
+  """Sequences with rows that the arrays do not have: those they have stand at their own positions (row i of n at length - n + i, as append puts them), status 2."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(36)
+  h, hk, ps, length = 4, 2, 16, [400, 300][:len(off) - 1]
+  t, n_pages = table(rng, length, ps)
+  (k, kv), (v, vv), (q, qv) = (put(rng.standard_normal(s), c) for s, c in (((n_pages, hk, ps, d), ct), ((n_pages, hk, ps, d), ct), ((held, h, d), qt)))
+  out = put(np.full((held + 2, h, d), 3.0), qt)[0]
+  cache = paged.PagedCache(n_pages, ps, hk, d, ct, k=k, v=v)
+  batch = paged.PagedBatch(i32(off), i32(length), i32(t), n_rows=held, max_new=max(np.diff(off)), max_len=max(length))
+  status()
+  paged.attention(cache, batch, q, out, h, qt)
+  got = get(out, (held + 2, h, d), qt)
+  assert status() == 2 and (got[held:] == 3).all()
+  rows = np.zeros((off[-1] - off[0], h, d))           # the same with all of the rows
+  rows[-off[0]:held - off[0]] = qv
+  want, weight, reach = (x[-off[0]:held - off[0]] for x in ref.attention(rows, kv, vv, np.array(off) - off[0], length, t, ps, d ** -0.5))
+  close_attention(got[:held], want, weight, reach, d, max(length), qt, qt, "the rows that there are")

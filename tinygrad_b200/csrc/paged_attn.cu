@@ -42,11 +42,14 @@ __device__ __forceinline__ SeqPlace place_of_seq(const AttnParams& p, int s) {
   const int b0 = t.row_off[s], e0 = t.row_off[s + 1], length = t.length[s];
   const int b = min(max(b0, 0), t.n_rows), e = min(max(e0, b), t.n_rows), n = min(e - b, t.max_new);
   const int64_t room = (int64_t)t.table_stride * t.page_size;
-  return SeqPlace{b, n > p.above && n <= p.up_to ? n : 0, (int)min((int64_t)min(max(length, 0), t.max_len), room), length - (e - b)};
+  return SeqPlace{b, n > p.above && n <= p.up_to ? n : 0, (int)min((int64_t)min(max(length, 0), t.max_len), room), length - (e0 - b)};      // (by all of its rows, those past the arrays among them)
 }
-__device__ __forceinline__ bool goes_back(const PagedTables& t, int s) { return t.row_off[s + 1] < t.row_off[s]; }
+__device__ __forceinline__ bool rows_outside(const PagedTables& t, int s) {      // rows that go back, or that the arrays do not have
+  const int b = t.row_off[s], e = t.row_off[s + 1];
+  return e < b || b < 0 || e > t.n_rows;
+}
 __device__ __forceinline__ void check_place(const AttnParams& p, int s, const SeqPlace& q) {      // what the tables promise and the bounds do not hold
-  if (q.n == 0 ? goes_back(p.t, s) : min(max(p.t.row_off[s + 1], q.first_row), p.t.n_rows) - q.first_row > q.n || p.t.length[s] > q.cap) atomicExch(&g_paged_attn_status, 2);
+  if (rows_outside(p.t, s) || (q.n > 0 && (p.t.row_off[s + 1] - q.first_row > q.n || p.t.length[s] > q.cap))) atomicExch(&g_paged_attn_status, 2);
 }
 template <int R>
 __device__ __forceinline__ TilePlace tile_of_seq(const AttnParams& p, int s, const SeqPlace& q, int tile) {
@@ -68,7 +71,7 @@ __device__ __forceinline__ TilePlace place_of_tile(const AttnParams& p, int tile
   } else {
     bool found = false;
     for (int s0 = 0; s0 < t.n_seqs && !found; s0 += 32) {
-      if (s0 + lane < t.n_seqs && goes_back(t, s0 + lane)) atomicExch(&g_paged_attn_status, 2);
+      if (s0 + lane < t.n_seqs && rows_outside(t, s0 + lane)) atomicExch(&g_paged_attn_status, 2);
       const int mine = s0 + lane < t.n_seqs ? (place_of_seq(p, s0 + lane).n * p.group + R - 1) / R : 0;
       int sum = mine;
 #pragma unroll
