@@ -929,3 +929,32 @@ def test_row_offsets_outside_the_arrays(qt, ct, d, off, held):
   rows[-off[0]:held - off[0]] = qv
   want, weight, reach = (x[-off[0]:held - off[0]] for x in ref.attention(rows, kv, vv, np.array(off) - off[0], length, t, ps, d ** -0.5))
   close_attention(got[:held], want, weight, reach, d, max(length), qt, qt, "the rows that there are")
+
+
+def test_a_workspace_after_offsets_that_go_back():
+  """Sequences that overlap until their rounds of keys pass 2^32: status 2, and the call behind it finds the workspace as the one before had left it."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  from tinygrad_b200.runtime import DeviceBuffer
+  rng = np.random.default_rng(37)
+  h, hk, d, ps, rows, most = 32, 8, 32, 64, 16384, 131072
+  n = 129                                     # 64 of 16384 rows (2^26 rounds each), those that go back between them, one of a single row (8 x 18 rounds)
+  back, ok = np.array([0, rows] * 64 + [0, 1], np.int32), np.array([0] + [1] * n, np.int32)
+  lens, long = np.array([most] * (n - 1) + [18 * 64], np.int32), np.full(n, most, np.int32)
+  (k, _), (v, _) = (put(rng.standard_normal((3, hk, ps, d)), "float16") for _ in "kv")
+  q, out = put(rng.standard_normal((rows, h, d)), "float16")[0], put(np.zeros((rows, h, d)), "float16")[0]
+  off, length = i32(ok), i32(long)
+  batch = paged.PagedBatch(off, length, i32(rng.integers(0, 3, (n, most // ps))), n_rows=rows, max_new=rows, max_len=most)
+  cache = paged.PagedCache(3, ps, hk, d, k=k, v=v)
+  status()
+  paged.attention(cache, batch, q, out, h, "float16")
+  want = get(out, (1, h, d), "float16")
+  assert status() == 0 and want.any()
+  off.copy_from(back), length.copy_from(lens)
+  paged.attention(cache, batch, q, out, h, "float16")
+  assert status() == 2
+  off.copy_from(ok), length.copy_from(long)
+  out.copy_from(np.zeros((rows, h, d), np.float16))
+  paged.attention(cache, batch, q, out, h, "float16")
+  got = get(out, (rows, h, d), "float16")
+  assert (got[:1] == want).all() and not got[1:].any() and status() == 0
