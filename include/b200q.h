@@ -512,7 +512,7 @@ int b200q_tc_status_read_clear(int* status);
  *   (b200q_attn_prefill and _decode rotate themselves: rope NULL).  positions [n_rows] (device) is asked for with rope only; one outside the table gives zeros and status 2.
  * b200q_paged_attention: out[row][head] = softmax(scale * q . k) v over positions 0 .. the row's own, query head h on KV head h / (n_heads / n_kv_heads).  scale 0: head_dim^-1/2.  A row
  *   without a position (length < its sequence's rows) gets zeros.  Values behind a row's own position are not read into it, whatever they are (NaN among them).
- *   q, out: B200Q_F32 | F16 | BF16, strides in elements (0: back to back).  Scores, sums and the running maximum are 32-bit; rows of fp32 meet fp16 keys as two
+ *   q, out: B200Q_F32 | F16 | BF16, strides in elements (0: back to back); out may be q if types and strides agree.  Scores, sums and the running maximum are 32-bit; rows of fp32 meet fp16 keys as two
  *   fp16 halves (bf16 keys: three).  workspace: b200q_paged_attention_workspace_bytes bytes, 256-byte aligned, its first 16 KB zeroed
  *   once (and again after status 1); a call leaves it as any next one needs it, whatever that one's cache and batch.  Calls that may run at the same time (two streams, two graphs) need one each.
  * head_dim 16, 32, 64 or 128.  flags: B200Q_FLAG_PDL (the launch before it on the stream is a kernel of this library). */

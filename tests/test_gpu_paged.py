@@ -958,3 +958,23 @@ def test_a_workspace_after_offsets_that_go_back():
   paged.attention(cache, batch, q, out, h, "float16")
   got = get(out, (rows, h, d), "float16")
   assert (got[:1] == want).all() and not got[1:].any() and status() == 0
+
+
+@pytest.mark.parametrize("qt,ct,d", [("float16", "float16", 128), ("bfloat16", "bfloat16", 64), ("float32", "float16", 128), ("float32", "float32", 32)])
+@pytest.mark.parametrize("seqs", [[(1, 5000), (2, 700)], [(150, 4000)], [(1, 300), (200, 900), (9, 60)]], ids=["tokens", "keys in parts", "both kernels"])
+def test_attention_in_place(qt, ct, d, seqs):
+  """out is q: the bits of a call whose outputs are elsewhere."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(38)
+  h, hk, ps = 8, 2, 16
+  new, length = [n for n, _ in seqs], [l for _, l in seqs]
+  off, n = np.concatenate([[0], np.cumsum(new)]), sum(new)
+  t, n_pages = table(rng, length, ps)
+  (k, _), (v, _) = (put(rng.standard_normal((n_pages, hk, ps, d)), ct) for _ in "kv")
+  cache = paged.PagedCache(n_pages, ps, hk, d, ct, k=k, v=v)
+  batch = paged.PagedBatch(i32(off), i32(length), i32(t), n_rows=n, max_new=max(new), max_len=max(length))
+  q, out = put(rng.standard_normal((n, h, d)), qt)[0], put(np.zeros((n, h, d)), qt)[0]
+  paged.attention(cache, batch, q, out, h, qt)
+  paged.attention(cache, batch, q, q, h, qt)
+  assert (get(q, (n, h, d), qt) == get(out, (n, h, d), qt)).all() and status() == 0

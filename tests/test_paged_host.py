@@ -308,3 +308,11 @@ def test_a_first_call_zeroes_its_workspace_on_its_own_stream(workspaces):
   assert workspaces.log == [("alloc", b._ws.ptr, 0), ("memset", b._ws.ptr, 0), ("wait",)]
   b.reserve(c, 4)
   assert len(workspaces.log) == 3
+
+
+@pytest.mark.parametrize("change", [dict(out_dtype=F16), dict(q_stride=512), dict(out_stride=320), dict(q_dtype=BF16)])
+def test_attention_in_place_of_other_rows_is_refused(lib, change):
+  """out may be q itself; with other types or strides a row would be written where another is still to be read."""
+  a = _lib.PagedAttnArgs(P, P, F32, F32, 0, 0, 4, 0.0, P, 1 << 30)
+  for k, v in change.items(): setattr(a, k, v)
+  assert call(lib.b200q_paged_attention, cache(), batch(), a) == -1

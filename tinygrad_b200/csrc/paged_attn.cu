@@ -423,6 +423,7 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
   if (batch->n_seqs == 0 || batch->n_rows == 0) return B200Q_OK;
   if (!a->q || !a->out) return B200Q_ERR_BAD_ARG;
   if ((uintptr_t)a->q % type_size(a->q_dtype) || (uintptr_t)a->out % type_size(a->out_dtype) || (uintptr_t)a->workspace & 255) return B200Q_ERR_MISALIGNED;
+  if (a->q == a->out && (a->q_dtype != a->out_dtype || (a->q_stride ? a->q_stride : row) != (a->out_stride ? a->out_stride : row))) return B200Q_ERR_BAD_ARG;      // rows would be overwritten before they are read
   const b200q_paged_batch within = bounded(batch);
   batch = &within;
   // one part of 16 bits where queries, keys and outputs have 16; two (bf16 keys: three, which the rows kernel has) where something is wider
