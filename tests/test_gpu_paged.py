@@ -978,3 +978,45 @@ def test_attention_in_place(qt, ct, d, seqs):
   paged.attention(cache, batch, q, out, h, qt)
   paged.attention(cache, batch, q, q, h, qt)
   assert (get(q, (n, h, d), qt) == get(out, (n, h, d), qt)).all() and status() == 0
+
+
+@pytest.mark.parametrize("qt,ct,d", [("float16", "float16", 128), ("bfloat16", "bfloat16", 64), ("float32", "float16", 128), ("float32", "float32", 64), ("float32", "bfloat16", 32)])
+@pytest.mark.parametrize("seqs,bounds", [([(1, 513), (1, 70)], (1, 131072)), ([(1, 900), (3, 33), (0, 5)], (300, 5000)), ([(200, 700), (1, 300)], (4096, 131072)), ([(40, 2000)], (41, 2001)), ([(2, 2)], (2, 65536))],
+                         ids=["tokens", "tokens with room for prompts", "a step's bounds", "one more", "a short one"])
+def test_attention_with_bounds_above_its_tables(qt, ct, d, seqs, bounds):
+  """What a captured step has: the bounds decide which kernels run and how the keys are split, the tables what they do."""
+  need_gpu()
+  attend(seqs, 8, 2, d, 16, qt, ct, seed=d, bounds=bounds)
+
+
+@pytest.mark.parametrize("rotate_here", [True, False])
+def test_norms_in_front_of_the_contiguous_cache(rotate_here):
+  """head_norm_rope over the rows of b200q_attn_prefill, in place: with its rotation (prefill is told to rotate nothing: rope_dim 0) or without (prefill rotates)."""
+  need_gpu()
+  from tinygrad_b200 import _lib, paged
+  from tinygrad_b200.runtime import DeviceBuffer
+  rng = np.random.default_rng(39)
+  h, hk, d, n, start, ctx = 8, 2, 128, 90, 30, 160
+  width = (h + 2 * hk) * d
+  rope, w = cos_sin(ctx, d), rng.uniform(0.5, 1.5, (2, d)).astype(np.float16)
+  rb, wq, wk = DeviceBuffer.from_numpy(rope), DeviceBuffer.from_numpy(w[0]), DeviceBuffer.from_numpy(w[1])
+  before = rng.standard_normal((2, hk, ctx, d)).astype(np.float16)
+  k, v = DeviceBuffer.from_numpy(before[0]), DeviceBuffer.from_numpy(before[1])
+  x, xv = put(rng.standard_normal((n, h + 2 * hk, d)), "float32")
+  q, out = DeviceBuffer.empty((n, h * d), np.float32), DeviceBuffer.empty((n, h * d), np.float32)
+  paged.head_norm_rope(x, x, n, h, hk, d, q_norm=wq, k_norm=wk, norm_eps=1e-6, rope=rb if rotate_here else None, positions=i32(start + np.arange(n)) if rotate_here else None, x_stride=width, out_stride=width)
+  _lib.check(_lib.load().b200q_attn_prefill(x.ptr, k.ptr, v.ptr, _lib.F16, rb.ptr, start, n, h, hk, d, 0 if rotate_here else d, ctx, q.ptr, out.ptr, _lib.F32, None))
+  rot, now = rope[start:start + n], x.numpy((n, h + 2 * hk, d), np.float32).astype(np.float64)
+  assert (now[:, h + hk:] == xv[:, h + hk:]).all()
+  for a, b, ww in ((0, h, w[0]), (h, h + hk, w[1])):
+    here = rot if rotate_here else None
+    close_rows(now[:, a:b], ref.rotate(ref.head_norm(xv[:, a:b], ww, 1e-6), here), reach_of(xv[:, a:b], ww, 1e-6, here), "float32", "rows")
+  kc, vc = k.numpy().astype(np.float64), v.numpy().astype(np.float64)
+  new = slice(start, start + n)
+  assert (kc[:, :start] == before[0][:, :start]).all() and (vc[:, new] == xv[:, h + hk:].astype(np.float16).transpose(1, 0, 2)).all()
+  kw = ref.rotate(ref.head_norm(xv[:, h:h + hk], w[1], 1e-6), rot)
+  close_rows(kc[:, new].transpose(1, 0, 2), kw, reach_of(xv[:, h:h + hk], w[1], 1e-6, rot), "float16", "keys")
+  # queries as prefill takes them: those of the rows, or (its own rotation, 32 bits) within 2^-22 of (|a| + |b|) of them -- 64-bit values here, a score's walk covers that
+  qs = now[:, :h] if rotate_here else ref.rotate(now[:, :h], rot)
+  want, weight, reach = ref.attention(qs, kc[None], vc[None], [0, n], [start + n], np.zeros((1, 1), int), ctx, d ** -0.5)
+  close_attention(out.numpy((n, h, d), np.float32).astype(np.float64), want, weight, reach, d, start + n, "float32", "float32", "attention")
