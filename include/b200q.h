@@ -57,7 +57,9 @@ extern "C" {
 const char* b200q_strerror(int code);
 /* Device-side status word: 0 = fine, 1 = a bounded wait inside a kernel ran out (the kernel then skipped its
  * remaining work instead of spinning; its output is invalid), 2 = a decode-step kernel was handed a position outside
- * [0, max_context) and skipped its cache / token-table access.  Reads and clears it.  Synchronises the device. */
+ * [0, max_context) and skipped its cache / token-table access, or a paged-cache kernel a table that its bounds or arrays
+ * do not hold (a page, position, length or row that does not exist: what becomes of those is said there).  Reads and
+ * clears it.  Synchronises the device. */
 int b200q_status_read_clear(int* status);
 const char* b200q_last_cuda_error(void);
 int b200q_version(void);
@@ -509,11 +511,13 @@ int b200q_tc_status_read_clear(int* status);
  *   the rows of q (q_dtype, q_stride; may be x's own q part if types and strides agree) and k, v to the sequence's pages (which no other sequence of the call appends to).  32-bit arithmetic, each value rounded once.  A row whose position has no
  *   entry in `rope` gets zeros in q.
  * b200q_head_norm_rope: the same norms and rotation of the first n_heads + n_kv_heads heads of every row, from x to out (may be x), for callers whose cache is not paged
- *   (b200q_attn_prefill and _decode rotate themselves: rope NULL).  positions [n_rows] (device) is asked for with rope only; one outside the table gives zeros and status 2.
+ *   (b200q_attn_prefill and _decode rotate themselves: rope NULL here, or their rope_dim 0; their own table is asked for either way).  positions [n_rows] (device) is asked for with rope only; one outside the table gives zeros and status 2.
  * b200q_paged_attention: out[row][head] = softmax(scale * q . k) v over positions 0 .. the row's own, query head h on KV head h / (n_heads / n_kv_heads).  scale 0: head_dim^-1/2.  A row
  *   without a position (length < its sequence's rows) gets zeros.  Values behind a row's own position are not read into it, whatever they are (NaN among them).
  *   q, out: B200Q_F32 | F16 | BF16, strides in elements (0: back to back); out may be q if types and strides agree.  Scores, sums and the running maximum are 32-bit; rows of fp32 meet fp16 keys as two
- *   fp16 halves (bf16 keys: three).  workspace: b200q_paged_attention_workspace_bytes bytes, 256-byte aligned, its first 16 KB zeroed
+ *   fp16 halves (bf16 keys: three), and so do their probabilities the values: the result is as exact as 32-bit arithmetic makes it.  Where q, the pages and out are all 16-bit and q has the pages' type, a
+ *   probability is rounded to the pages' type before it meets the values (half a step, as the output loses) and batches with prompts sum their products with the values in the tensor core, which cuts
+ *   where others round; out fp32 (or another type of q than the pages') takes the exact way.  Positions from 2^31 - 128 on are not attended, whatever max_len says.  workspace: b200q_paged_attention_workspace_bytes bytes, 256-byte aligned, its first 16 KB zeroed
  *   once (and again after status 1); a call leaves it as any next one needs it, whatever that one's cache and batch.  Calls that may run at the same time (two streams, two graphs) need one each.
  * head_dim 16, 32, 64 or 128.  flags: B200Q_FLAG_PDL (the launch before it on the stream is a kernel of this library). */
 typedef struct b200q_paged_cache {

@@ -8,10 +8,6 @@ namespace {
 // ---- element types ----
 __host__ __device__ constexpr int type_size(int t) { return t == B200Q_F32 ? 4 : 2; }
 static inline bool type_known(int t) { return t == B200Q_F32 || t == B200Q_F16 || t == B200Q_BF16; }
-template <int T> struct Elem;
-template <> struct Elem<B200Q_F32> { typedef float type; };
-template <> struct Elem<B200Q_F16> { typedef __half type; };
-template <> struct Elem<B200Q_BF16> { typedef __nv_bfloat16 type; };
 
 __device__ __forceinline__ float to_f(float v) { return v; }
 __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
@@ -33,13 +29,13 @@ __device__ __forceinline__ void store_as(void* base, int type, int64_t i, float 
 
 // Division of values below 2^31 by a number that the host knows: n / d = (high word of n * mul + n) >> shift (a division proper is forty dependent instructions)
 struct Divisor {
-  uint32_t d, mul, shift;
+  uint32_t mul, shift;
   __device__ __forceinline__ int div(int n) const { return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift); }
 };
 static inline Divisor divisor_of(int d) {
   uint32_t shift = 0;
   while ((1u << shift) < (uint32_t)d) shift++;      // d <= 2^shift < 2 d; mul = 2^32 (2^shift - d) / d + 1
-  return Divisor{(uint32_t)d, (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1), shift};
+  return Divisor{(uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1), shift};
 }
 
 // ---- tables ----

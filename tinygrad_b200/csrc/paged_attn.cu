@@ -21,7 +21,7 @@ struct AttnParams {
   void* out;
   int q_dtype, out_dtype;
   int64_t q_stride, out_stride, page_stride, head_stride, row_stride;
-  int n_heads, n_kv, group;
+  int n_kv, group;
   float scale;               // times log2 e
   Divisor by_group, by_kv, by_page;
   int tiles_per_seq;         // 0: tiles are counted sequence by sequence
@@ -296,7 +296,7 @@ b200q_paged_batch bounded(const b200q_paged_batch* b) {
   c.max_len = std::min(c.max_len, MAX_KEYS);
   return c;
 }
-constexpr int MAX_PARTS = 296;      // of a tile's keys: their shares of 16 rows take 19 KB of shared memory (of 256 rows, 64 parts at most, 64 KB)
+constexpr int MAX_PARTS = 296;      // of the keys of a tile of 16 rows: their shares take 19 KB of shared memory (tiles of 256 rows have T_PARTS at most)
 struct Plan { int64_t tiles; int tiles_per_seq, n_split, split_len, above, up_to, ctas; int64_t rounds; size_t bytes; };      // tiles x KV heads past 2^31 and rounds of -1: too large; bytes: of the parts in the workspace
 
 // Tiles of `rows` pairs: those of all sequences at their largest, or (ragged batches, if that is less) the pairs' tiles and a broken one for each sequence.  Keys are split until
@@ -451,7 +451,7 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
     int* const counters = (int*)a->workspace + i * MAX_UNITS;
     float* const parts_at = (float*)((char*)a->workspace + COUNTERS_BYTES + (i ? deal.plan[0].bytes : 0));
     return AttnParams{a->q, cache->k, cache->v, a->out, a->q_dtype, a->out_dtype, a->q_stride ? a->q_stride : row, a->out_stride ? a->out_stride : row, cache->page_stride,
-                       cache->head_stride, cache->row_stride, a->n_heads, n_kv, group, (a->scale > 0.f ? a->scale : 1.f / sqrtf((float)dim)) * LOG2E, divisor_of(group), divisor_of(n_kv), divisor_of(cache->page_size), plan.tiles_per_seq, plan.above, plan.up_to,
+                       cache->head_stride, cache->row_stride, n_kv, group, (a->scale > 0.f ? a->scale : 1.f / sqrtf((float)dim)) * LOG2E, divisor_of(group), divisor_of(n_kv), divisor_of(cache->page_size), plan.tiles_per_seq, plan.above, plan.up_to,
                        plan.n_split, plan.split_len, late, counters, parts_at, tables_of(cache, batch)};
   };
   for (int i = 0; i < deal.n; i++) {

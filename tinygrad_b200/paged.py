@@ -199,7 +199,8 @@ def append(cache: PagedCache, batch: PagedBatch, x, q, n_heads: int, x_dtype="fl
 
 def attention(cache: PagedCache, batch: PagedBatch, q, out, n_heads: int, q_dtype="float32", out_dtype=None, scale: float = 0.0, q_stride: int = 0, out_stride: int = 0, flags: int = 0,
               stream=None) -> None:
-  """out[row][head] = softmax(scale q . k) v over the positions up to the row's own (scale 0: head_dim ** -0.5); out_dtype is q's unless given."""
+  """out[row][head] = softmax(scale q . k) v over the positions up to the row's own (scale 0: head_dim ** -0.5); out_dtype is q's unless given, out may be q.  16-bit queries, pages and outputs: a probability
+  is rounded to the pages' type; out_dtype "float32" keeps 32 bits throughout."""
   qt = _dtype(q_dtype)
   ot = qt if out_dtype is None else _dtype(out_dtype)
   n, row = batch.n_rows, n_heads * cache.head_dim

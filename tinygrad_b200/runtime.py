@@ -192,7 +192,8 @@ def device_props(i: int = 0) -> dict:
 
 
 def device_status() -> int:
-  """0 = fine; 1 = a bounded wait inside a kernel ran out since the last call (reads and clears the word)."""
+  """0 = fine; since the last call, 1 = a bounded wait inside a kernel ran out, 2 = a decode step or a paged-cache call was handed positions, pages, lengths or rows that do not exist (reads and clears
+  the word)."""
   st = ctypes.c_int()
   check(_lib.load().b200q_status_read_clear(ctypes.byref(st)))
   return st.value
