@@ -8,7 +8,7 @@
 // units': a quarter of them as a polynomial on the multiply-adders, whose results below 2^-126 have to be made 0, took 443 against 429 us below (heads of 64 312 against 302).  A tile's product begins with half of its probabilities.
 //
 // Tensor memory: S0 S1 O0 O1, 128 columns each, a tile's probabilities in the place of its scores.  Heads of 64 leave room for probabilities of their own (T_APART): the next scores
-// are then computed as soon as these have been read, not behind their product (4096 rows of 32 heads of 64, 8192 positions: 302 us, 315 in place).
+// are then computed as soon as these have been read, not behind their product (4096 rows of 32 heads of 64, 8192 positions: 302 us against 315 in place; 294 since the powers stand there once).
 //
 // 4096 rows of 32 heads of 128 at 8192 positions: 365 to 430 us, as the power limit has the clock (0.96 to 1.1 PFLOP/s).  CTAs that stay and share the work evenly took 442 against
 // 388 us there, softmaxes that are kept apart by barriers 406 against 391, a running maximum looked for behind the first powers 399 against 388.
