@@ -1020,3 +1020,22 @@ def test_norms_in_front_of_the_contiguous_cache(rotate_here):
   qs = now[:, :h] if rotate_here else ref.rotate(now[:, :h], rot)
   want, weight, reach = ref.attention(qs, kc[None], vc[None], [0, n], [start + n], np.zeros((1, 1), int), ctx, d ** -0.5)
   close_attention(out.numpy((n, h, d), np.float32).astype(np.float64), want, weight, reach, d, start + n, "float32", "float32", "attention")
+
+
+@pytest.mark.parametrize("qt,ct,d", [("float16", "float16", 32), ("float16", "float16", 128), ("float32", "float32", 64)])
+@pytest.mark.parametrize("new", [[1, 2], [150, 3]])
+def test_offsets_of_sequences_that_are_not_there(qt, ct, d, new):
+  """A table of more sequences than there are, whose last entries are 0: the offsets go back (status 2), nothing overlaps, and the rows get their answers."""
+  need_gpu()
+  from tinygrad_b200 import paged
+  rng = np.random.default_rng(40)
+  h, hk, ps, length, n = 4, 2, 16, [300, 2500], sum(new)
+  t, n_pages = table(rng, length, ps)
+  (k, kv), (v, vv), (q, qv) = (put(rng.standard_normal(s), c) for s, c in (((n_pages, hk, ps, d), ct), ((n_pages, hk, ps, d), ct), ((n, h, d), qt)))
+  out = put(np.zeros((n, h, d)), qt)[0]
+  batch = paged.PagedBatch(i32([0, new[0], n] + [0] * 40), i32(length + [0] * 40), i32(np.concatenate([t, np.zeros((40, t.shape[1]), int)])), n_rows=n, max_new=max(new), max_len=max(length))
+  status()
+  paged.attention(paged.PagedCache(n_pages, ps, hk, d, ct, k=k, v=v), batch, q, out, h, qt)
+  want, weight, reach = ref.attention(qv, kv, vv, [0, new[0], n], length, t, ps, d ** -0.5)
+  close_attention(get(out, (n, h, d), qt), want, weight, reach, d, max(length), qt, qt, "rows")
+  assert status() == 2

@@ -27,6 +27,7 @@ struct AttnParams {
   int tiles_per_seq;         // 0: tiles are counted sequence by sequence
   int above, up_to;          // sequences with above < new tokens <= up_to (those with others are another kernel's)
   int n_split, split_len, late;      // late: behind the tiles kernel of the same call
+  uint32_t most_rounds;      // of the rows kernel, by the host's bounds
   int* counters;
   float* parts;
   PagedTables t;
@@ -452,7 +453,7 @@ extern "C" int b200q_paged_attention(const b200q_paged_cache* cache, const b200q
     float* const parts_at = (float*)((char*)a->workspace + COUNTERS_BYTES + (i ? deal.plan[0].bytes : 0));
     return AttnParams{a->q, cache->k, cache->v, a->out, a->q_dtype, a->out_dtype, a->q_stride ? a->q_stride : row, a->out_stride ? a->out_stride : row, cache->page_stride,
                        cache->head_stride, cache->row_stride, n_kv, group, (a->scale > 0.f ? a->scale : 1.f / sqrtf((float)dim)) * LOG2E, divisor_of(group), divisor_of(n_kv), divisor_of(cache->page_size), plan.tiles_per_seq, plan.above, plan.up_to,
-                       plan.n_split, plan.split_len, late, counters, parts_at, tables_of(cache, batch)};
+                       plan.n_split, plan.split_len, late, (uint32_t)plan.rounds, counters, parts_at, tables_of(cache, batch)};
   };
   for (int i = 0; i < deal.n; i++) {
     // many rows first: once the last of their CTAs has a place, those for few rows begin where others leave room (12 sequences, 1 to 700 new of up to 3000 positions: 52 us, 60 the other way around)

@@ -140,7 +140,8 @@ __device__ __forceinline__ void attn_rows(const AttnParams& p, const CUtensorMap
   auto units_of = [&](const SeqPlace& q) { return (uint32_t)((unsigned)(q.n * p.group + R - 1) / R * p.n_kv); };
   auto rounds_of = [&](const SeqPlace& q) { return (uint32_t)max(1, (q.cap + ROUND - 1) / ROUND); };      // (without keys: somebody writes the zeros)
   struct Work { uint32_t units, rounds; };
-  bool back = false;                                     // row_off goes back
+  bool back = false;                                     // row_off goes back: sequences may overlap
+  uint64_t rounds = 0;                                   // of this lane's sequences
   auto sums_of = [&](int s) {                            // of this lane's sequence and those of the lanes before it
     Work v{0, 0};
     if (s < p.t.n_seqs) {
@@ -149,6 +150,7 @@ __device__ __forceinline__ void attn_rows(const AttnParams& p, const CUtensorMap
       if (blockIdx.x == 0 && warp == 0) check_place(p, s, q);
       v.units = units_of(q);
       v.rounds = v.units * rounds_of(q);
+      rounds += (uint64_t)v.units * rounds_of(q);
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -163,9 +165,13 @@ __device__ __forceinline__ void attn_rows(const AttnParams& p, const CUtensorMap
     all.units += __shfl_sync(0xffffffffu, sums.units, 31);
     all.rounds += __shfl_sync(0xffffffffu, sums.rounds, 31);
   }
-  // Sequences that overlap are work without a bound, and their sums may wrap around to units that no CTA ends, whose counters would wait for it in the next call.  (check_place reports them; the host's
-  // bound, which fits into 31 bits, holds for all others.)
-  if (__any_sync(0xffffffffu, back)) return;
+  // Sequences that overlap (check_place reports them) are work past the host's bound, which fits into 31 bits, and their sums may wrap around to units that no CTA ends, whose counters would wait for it in
+  // the next call.
+  if (__any_sync(0xffffffffu, back)) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) rounds += __shfl_xor_sync(0xffffffffu, rounds, o);
+    if (rounds > p.most_rounds) return;
+  }
   // A unit costs its rounds and, where shares are long, what it takes to begin and end one.  A share that would begin or end in that part does so where the unit begins.
   const uint32_t ctas = min(gridDim.x, max(min(all.rounds, (uint32_t)N_SM), all.rounds / R_LEAST)), c = blockIdx.x;
   if (c >= ctas) return;
