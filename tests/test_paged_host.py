@@ -316,3 +316,18 @@ def test_attention_in_place_of_other_rows_is_refused(lib, change):
   a = _lib.PagedAttnArgs(P, P, F32, F32, 0, 0, 4, 0.0, P, 1 << 30)
   for k, v in change.items(): setattr(a, k, v)
   assert call(lib.b200q_paged_attention, cache(), batch(), a) == -1
+
+
+def test_tables_of_different_kinds(lib):
+  """A batch's tables may be buffers and foreign tensors in any mixture; each has to be contiguous."""
+  import torch
+  class OnDevice:
+    is_cuda = True
+    def __init__(self, t): self.t = t
+    def __getattr__(self, name): return getattr(self.t, name)
+  i = lambda *s: OnDevice(torch.zeros(s, dtype=torch.int32))
+  f = lambda *s: Fake(s, np.int32)
+  for row_off, length, pages in ((i(3), f(2), f(2, 5)), (f(3), i(2), f(2, 5)), (f(3), f(2), i(2, 5)), (i(3), i(2), i(2, 5))): paged.PagedBatch(row_off, length, pages, 2, 1, 9)
+  apart = lambda *s: OnDevice(torch.zeros(*s[:-1], 2 * s[-1], dtype=torch.int32)[..., ::2])
+  for row_off, length, pages in ((apart(3), f(2), f(2, 5)), (f(3), apart(2), f(2, 5)), (f(3), f(2), apart(2, 5)), (i(3), apart(2), i(2, 5))):
+    with pytest.raises(ValueError, match="contiguous"): paged.PagedBatch(row_off, length, pages, 2, 1, 9)

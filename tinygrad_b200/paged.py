@@ -153,7 +153,7 @@ class PagedBatch:
     (n_seqs,), (seqs, table) = length.shape, pages.shape
     if seqs != n_seqs or tuple(row_off.shape) != (n_seqs + 1,): raise ValueError(f"row_off {tuple(row_off.shape)}, length {tuple(length.shape)} and pages {tuple(pages.shape)} do not match")
     if n_seqs and table < 1: raise ValueError("a sequence has at least one entry in the table of pages")
-    if hasattr(pages, "is_contiguous") and not (pages.is_contiguous() and row_off.is_contiguous() and length.is_contiguous()): raise ValueError("tables are contiguous")
+    for x, what in ((row_off, "row_off"), (length, "length"), (pages, "pages")): _dense(x, what)
     self.row_off, self.length, self.pages = _int32(row_off, "row_off"), _int32(length, "length"), _int32(pages, "pages")
     self.n_seqs, self.n_rows, self.max_new, self.max_len = n_seqs, n_rows, max_new, max_len
     self.desc = _lib.PagedBatchDesc(_ptr(row_off), _ptr(length), _ptr(pages), n_seqs, table, n_rows, max_new, max_len)
