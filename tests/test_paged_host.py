@@ -331,3 +331,14 @@ def test_tables_of_different_kinds(lib):
   apart = lambda *s: OnDevice(torch.zeros(*s[:-1], 2 * s[-1], dtype=torch.int32)[..., ::2])
   for row_off, length, pages in ((apart(3), f(2), f(2, 5)), (f(3), apart(2), f(2, 5)), (f(3), f(2), apart(2, 5)), (i(3), apart(2), i(2, 5))):
     with pytest.raises(ValueError, match="contiguous"): paged.PagedBatch(row_off, length, pages, 2, 1, 9)
+
+
+def test_page_locked_tensors_are_the_device_s_to_read(lib):
+  """The device reaches page-locked host memory: tables may stand there."""
+  import torch
+  class Pinned:
+    is_cuda, is_pinned = False, lambda self: True
+    def __init__(self, t): self.t = t
+    def __getattr__(self, name): return getattr(self.t, name)
+  length = Pinned(torch.zeros(2, dtype=torch.int32))
+  assert paged.PagedBatch(Fake((3,), np.int32), length, Fake((2, 5), np.int32), 2, 1, 9).desc.length == length.data_ptr()

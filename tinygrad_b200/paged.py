@@ -53,7 +53,7 @@ def _dtype(d) -> int:
 def _ptr(o) -> int:
   if type(o) is DeviceBuffer: return o.ptr
   try:
-    if not o.is_cuda: raise ValueError("a tensor on the host: the kernels read and write device memory")
+    if not o.is_cuda and not o.is_pinned(): raise ValueError("a tensor on the host: the kernels read and write device memory, or host memory that is page-locked")
     return o.data_ptr()
   except AttributeError: return ptr_of(o)
 
